@@ -1,0 +1,361 @@
+"""Cases for the row-wise operators of the point networks: layer norm, activations kept in 8 bits, 8-bit matrix products.
+
+Three operators that are used together, layer after layer, over the rows (texels, points, tokens) of an activation matrix:
+
+    norm      y = act(layer_norm(x)), and its gradients (input, weight, bias)
+    rows8     rows packed to 8-bit floating point, a power-of-two scale for each 128 columns: back to values, or straight
+              into the weight gradient of the layer whose input they are
+    linear8   y = Q(x) Q(W)^T + b in 8-bit floating point (scales per 128 columns of x, per 128 x 128 block of W), and its
+              gradients
+
+`run` computes them in elementary 32-bit torch operations (own = False) or through the package's entry points (own = True).
+"""
+import math
+
+import torch
+
+own = False
+
+_TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+_SIZE = {"f32": 4, "bf16": 2, "f16": 2}
+_FORMATS = {"e4m3": (torch.float8_e4m3fn, 448.0, 3, -6), "e5m2": (torch.float8_e5m2, 57344.0, 2, -14)}
+EPS = 1e-5
+
+
+def listed():
+    return [
+        # a handful of rows normalised at inference: the call's latency
+        {"name": "norm_rows_bf16", "op": "norm", "rows": 8, "cols": 1024, "type": "bf16", "act": "identity", "train": False, "kept8": False},
+        # one hidden layer of the texel decoder (512 x 512 texels, 128 channels), training
+        {"name": "norm_decoder_f32", "op": "norm", "rows": 262144, "cols": 128, "type": "f32", "act": "softplus", "train": True, "kept8": False},
+        # a ragged batch with an odd width: no row is aligned to more than its elements
+        {"name": "norm_odd_f16", "op": "norm", "rows": 4999, "cols": 771, "type": "f16", "act": "identity", "train": True, "kept8": False},
+        # a wide layer whose normalised input is kept in 8 bits for the backward pass
+        {"name": "norm_wide_kept8_bf16", "op": "norm", "rows": 16384, "cols": 4096, "type": "bf16", "act": "identity", "train": True, "kept8": True},
+        # a small ragged layer's input packed and used by its weight gradient: latency
+        {"name": "rows8_grad_small_f16", "op": "rows8", "rows": 777, "cols": 300, "out": 17, "type": "f16", "format": "e4m3", "use": "grad"},
+        # the decoder's input layer over an avatar's points: 64 features + 2 coordinates in, 128 out
+        {"name": "rows8_grad_points_f32", "op": "rows8", "rows": 202738, "cols": 66, "out": 128, "type": "f32", "format": "e4m3", "use": "grad"},
+        # a wide layer's weight gradient from its packed input
+        {"name": "rows8_grad_wide_bf16", "op": "rows8", "rows": 8192, "cols": 4096, "out": 4096, "type": "bf16", "format": "e4m3", "use": "grad"},
+        # a large activation packed and read back as values
+        {"name": "rows8_values_bf16", "op": "rows8", "rows": 16384, "cols": 4096, "out": 0, "type": "bf16", "format": "e5m2", "use": "values"},
+        # a single token through a wide layer whose weight is held in 8 bits
+        {"name": "linear8_token_bf16", "op": "linear8", "rows": 1, "cols": 4096, "out": 4096, "type": "bf16", "train": False},
+        # a few dozen rows, odd sizes
+        {"name": "linear8_rows_odd_f16", "op": "linear8", "rows": 45, "cols": 1000, "out": 2310, "type": "f16", "train": False},
+        # a hidden layer of the texel decoder, training
+        {"name": "linear8_decoder_f32", "op": "linear8", "rows": 262144, "cols": 128, "out": 128, "type": "f32", "train": True},
+        # a wide layer, training
+        {"name": "linear8_wide_bf16", "op": "linear8", "rows": 8192, "cols": 4096, "out": 8192, "type": "bf16", "train": True},
+    ]
+
+
+def _size(rng, low, high):
+    """Spread over the logarithm; two in five round to a multiple of 64, the others stay as they fall."""
+    n = int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+    if n > 96 and rng.random() < 0.4:
+        n = n // 64 * 64
+    return max(low, min(high, n))
+
+
+def draw(rng):
+    op = rng.choice(["norm", "rows8", "linear8"])
+    kind = rng.choice(["f32", "bf16", "f16"])
+    if op == "norm":
+        cols = _size(rng, 16, 16384)      # (a row of two or three leaves its gradient little but rounding)
+        rows = _size(rng, 1, max(1, min(300000, (1 << 27) // (cols * _SIZE[kind]))))
+        train = rng.random() < 0.7
+        # (in 32 bits a code that sits on a border between two grid values moves a gradient by more than 32 bits allow to compare)
+        kept8 = train and kind != "f32" and rng.random() < 0.5
+        return {"op": op, "rows": rows, "cols": cols, "type": kind, "act": rng.choice(["identity", "softplus"]), "train": train, "kept8": kept8}
+    if op == "rows8":
+        cols = _size(rng, 1, 8192)
+        if rng.random() < 0.4:
+            rows = _size(rng, 1, max(1, min(300000, (1 << 27) // (cols * _SIZE[kind]))))
+            return {"op": op, "rows": rows, "cols": cols, "out": 0, "type": kind, "format": rng.choice(["e4m3", "e5m2"]), "use": "values"}
+        out = _size(rng, 1, 8192)
+        rows = _size(rng, 1, max(1, min(300000, (1 << 27) // (max(cols, out) * _SIZE[kind]), (1 << 37) // (cols * out))))
+        return {"op": op, "rows": rows, "cols": cols, "out": out, "type": kind, "format": rng.choice(["e4m3", "e5m2"]), "use": "grad"}
+    cols, out = _size(rng, 1, 8192), _size(rng, 1, 8192)
+    if rng.random() < 0.5:
+        return {"op": op, "rows": _size(rng, 1, 4096), "cols": cols, "out": out, "type": kind, "train": False}
+    rows = _size(rng, 1, max(1, min(300000, (1 << 27) // (max(cols, out) * _SIZE[kind]), (1 << 37) // (cols * out))))
+    return {"op": op, "rows": rows, "cols": cols, "out": out, "type": kind, "train": True}
+
+
+# ---------------------------------------------------------------------------------------------- inputs
+
+
+def _activations(rows, cols, dtype, gen):
+    """Rows as a layer hands them on: columns of their own size and offset, a few of them much larger than the rest."""
+    x = torch.randn(rows, cols, device="cuda", generator=gen)
+    spread = torch.exp(torch.randn(cols, device="cuda", generator=gen) * 0.8)
+    offset = torch.randn(cols, device="cuda", generator=gen) * 0.5
+    return (x * spread + offset).to(dtype)
+
+
+def _plain_weight8(w):
+    """A weight's codes and exponents as they are held: codes [N, K up to 16] in e4m3, exponents [N / 128, K / 128 up to 4]."""
+    n, k = w.shape
+    nb, kb = -(-n // 128), -(-k // 128)
+    full = torch.nn.functional.pad(w.float(), (0, kb * 128 - k, 0, nb * 128 - n))
+    blocks = full.reshape(nb, 128, kb, 128)
+    e = _exponent(blocks.abs().amax(dim=(1, 3)), 448.0)
+    codes = _times_two_to(blocks, -e[:, None, :, None]).reshape(nb * 128, kb * 128)[:n, : -(-k // 16) * 16]
+    exps = torch.nn.functional.pad(e + 127, (0, -kb % 4), value=127).to(torch.uint8)
+    return codes.to(torch.float8_e4m3fn).contiguous(), exps.contiguous()
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(int(seed))
+    dtype = _TYPES[case["type"]]
+    rows, cols = case["rows"], case["cols"]
+    state = dict(case)
+    state["x"] = _activations(rows, cols, dtype, gen)
+    if case["op"] == "norm":
+        ln = torch.nn.LayerNorm(cols, eps=EPS, device="cuda", dtype=dtype)
+        with torch.no_grad():
+            ln.weight.copy_(torch.rand(cols, device="cuda", generator=gen) + 0.5)
+            ln.bias.copy_(torch.randn(cols, device="cuda", generator=gen) * 0.2)
+        state["ln"] = ln
+        if case["train"]:
+            state["x"].requires_grad_(True)
+            state["g"] = torch.randn(rows, cols, device="cuda", generator=gen).to(dtype)
+        return state
+    out = case["out"]
+    if case["op"] == "rows8":
+        if case["use"] == "grad":
+            state["g"] = torch.randn(rows, out, device="cuda", generator=gen).to(dtype)
+        return state
+    weight = (torch.randn(out, cols, device="cuda", generator=gen) / math.sqrt(cols)).to(dtype)
+    state["bias"] = (torch.randn(out, device="cuda", generator=gen) * 0.1).to(dtype)
+    if case["train"]:
+        state["x"].requires_grad_(True)
+        state["bias"].requires_grad_(True)
+        state["weight"] = weight.requires_grad_(True)
+        state["g"] = torch.randn(rows, out, device="cuda", generator=gen).to(dtype)
+    else:
+        state["codes"], state["exps"] = _plain_weight8(weight)
+    return state
+
+
+# ---------------------------------------------------------------------------------------------- the plain forms
+
+
+def _times_two_to(x, e):
+    """x 2^e for whole numbers e, exactly (a power function's result need not be a power of two)."""
+    two = ((e.to(torch.int64) + 1023) << 52).view(torch.float64).float()
+    return x * two
+
+
+def _rows_product(g, v):
+    """g^T v in 32 bits, 4096 rows at a time, the pieces added up in 64: the sum runs over every row."""
+    pad = -g.shape[0] % 4096 if g.shape[0] > 4096 else 0
+    step = min(4096, g.shape[0])
+    g = torch.nn.functional.pad(g, (0, 0, 0, pad)).unflatten(0, (-1, step)).transpose(1, 2).contiguous()
+    v = torch.nn.functional.pad(v, (0, 0, 0, pad)).unflatten(0, (-1, step))
+    return torch.matmul(g, v).double().sum(0).float()
+
+
+def _exponent(amax, most):
+    """The smallest e with amax <= most 2^e, most = 0.875 2^p; 0 for an empty block."""
+    m, p = torch.frexp(amax)
+    e = p - (9 if most == 448.0 else 16) + (m > 0.875).to(p.dtype)
+    return torch.where(amax > 0, e.clamp(-127, 127), torch.zeros_like(e))
+
+
+def _packed(x, fmt):
+    """The values that the rows' codes stand for, in 32 bits: blocks of 128 columns."""
+    kind, most = _FORMATS[fmt][:2]
+    rows, cols = x.shape
+    nb = -(-cols // 128)
+    blocks = torch.nn.functional.pad(x.float(), (0, nb * 128 - cols)).reshape(rows, nb, 128)
+    e = _exponent(blocks.abs().amax(dim=2), most)[..., None]
+    return _times_two_to(_times_two_to(blocks, -e).to(kind).float(), e).reshape(rows, nb * 128)[:, :cols]
+
+
+def _weight_values(codes, exps, cols):
+    """The values of a held weight, in 32 bits."""
+    n = codes.shape[0]
+    e = exps.int() - 127
+    e = e.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :cols]
+    return _times_two_to(codes[:, :cols].float(), e)
+
+
+def _plain_norm(s):
+    dtype = s["x"].dtype
+    x, w, b = s["x"].detach().float(), s["ln"].weight.detach().float(), s["ln"].bias.detach().float()
+    d = x - x.mean(1, keepdim=True)
+    rstd = torch.rsqrt((d * d).mean(1, keepdim=True) + EPS)
+    xh = d * rstd
+    u = xh * w + b
+    soft = s["act"] == "softplus"
+    e = torch.exp(u.clamp(max=20.0)) if soft else None
+    y = torch.where(u > 20.0, u, torch.log1p(e)) if soft else u
+    if not s["train"]:
+        return [y.to(dtype)]
+    if s["kept8"]:
+        k = _exponent(torch.tensor(math.sqrt(x.shape[1]), device=x.device), 448.0)
+        xh = _times_two_to(_times_two_to(xh, -k).to(torch.float8_e4m3fn).float(), k)
+    g = s["g"].float()
+    if soft:
+        u = xh * w + b
+        e = torch.exp(u.clamp(max=20.0))
+        g = g * torch.where(u > 20.0, torch.ones_like(u), e / (1.0 + e))
+    dw, db = (g * xh).double().sum(0).float(), g.double().sum(0).float()
+    gw = g * w
+    dx = rstd * (gw - gw.mean(1, keepdim=True) - xh * (gw * xh).mean(1, keepdim=True))
+    return [y.to(dtype), dx.to(dtype), dw.to(dtype), db.to(dtype)]
+
+
+def _plain_rows8(s):
+    dtype = s["x"].dtype
+    v = _packed(s["x"], s["format"])
+    if s["use"] == "values":
+        return [v.to(dtype)]
+    g = s["g"].float()
+    return [_rows_product(g, v).to(dtype), g.double().sum(0).to(dtype)]
+
+
+def _plain_linear8(s):
+    dtype = s["x"].dtype
+    x = _packed(s["x"].detach(), "e4m3")
+    codes, exps = _plain_weight8(s["weight"].detach()) if s["train"] else (s["codes"], s["exps"])
+    w = _weight_values(codes, exps, s["cols"])
+    y = x @ w.t() + s["bias"].detach().float()
+    if not s["train"]:
+        return [y.to(dtype)]
+    g = s["g"].float()
+    return [y.to(dtype), (_packed(s["g"], "e4m3") @ w).to(dtype), _rows_product(g, x).to(dtype), g.double().sum(0).to(dtype)]
+
+
+# ---------------------------------------------------------------------------------------------- the framework's calls
+
+
+def _own(s):
+    from gaussianavatar_amd import fused, rows8
+    if s["op"] == "norm":
+        if not s["train"]:
+            with torch.no_grad():
+                return [fused.layernorm_act(s["x"], s["ln"], s["act"])]
+        y = fused.layernorm_act(s["x"], s["ln"], s["act"], checkpoint8=s["kept8"])
+        return [y.detach(), *torch.autograd.grad(y, (s["x"], s["ln"].weight, s["ln"].bias), s["g"])]
+    if s["op"] == "rows8":
+        rows = rows8.quantize8(s["x"], s["format"])
+        if s["use"] == "values":
+            return [rows.dequantize(s["x"].dtype)]
+        return list(rows8.wgrad8(s["g"], rows))
+    if not s["train"]:
+        with torch.no_grad():
+            return [rows8.linear8(s["x"], rows8.Weight8(s["codes"], s["exps"], s["cols"]), s["bias"])]
+    y = rows8.linear8(s["x"], s["weight"], s["bias"])
+    return [y.detach(), *torch.autograd.grad(y, (s["x"], s["weight"], s["bias"]), s["g"])]
+
+
+def run(state):
+    if own:
+        return _own(state)
+    with torch.no_grad():
+        return {"norm": _plain_norm, "rows8": _plain_rows8, "linear8": _plain_linear8}[state["op"]](state)
+
+
+def work(case):
+    m, k, s = case["rows"], case["cols"], _SIZE[case["type"]]
+    if case["op"] == "norm":
+        if not case["train"]:
+            return {"bytes": 2 * m * k * s + 2 * k * s, "flops": 10 * m * k}
+        kept = 2 * m * k if case["kept8"] else 0                      # the codes are written by one pass and read by the other
+        return {"bytes": 4 * m * k * s + kept + 4 * k * s, "flops": 25 * m * k}
+    n = case["out"]
+    if case["op"] == "rows8":
+        if case["use"] == "values":
+            return {"bytes": 2 * m * k * s + 2 * m * k, "flops": 4 * m * k}
+        return {"bytes": m * k * s + 2 * m * k + m * n * s + n * k * s + n * s, "flops": 2 * m * n * k}
+    if not case["train"]:
+        return {"bytes": m * k * s + n * k + m * n * s + n * s, "flops": 2 * m * n * k}
+    return {"bytes": 2 * m * k * s + 2 * m * n * s + 2 * n * k * s + 2 * n * s + 2 * m * k, "flops": 6 * m * n * k}
+
+
+# ---------------------------------------------------------------------------------------------- the definition in 64 bits
+
+
+_POWERS = [2.0 ** i for i in range(-400, 401)]
+
+
+def _power64(e):
+    return torch.tensor(_POWERS, dtype=torch.float64, device=e.device)[e.long() + 400]
+
+
+def _grid64(v, fmt):
+    """The nearest value of an 8-bit format (ties to the even mantissa), by arithmetic on 64-bit numbers."""
+    _, _, mantissa, low = _FORMATS[fmt]
+    step = _power64((torch.frexp(v).exponent - 1).clamp_min(low) - mantissa)
+    return torch.round(v / step) * step
+
+
+def _scale64(amax, fmt):
+    """2^e with the smallest e such that amax fits under the format's largest value."""
+    most = _FORMATS[fmt][1]
+    e = torch.frexp(amax / most).exponent
+    e = torch.where(_power64(e - 1) * most >= amax, e - 1, e)
+    return torch.where(amax > 0, _power64(e.clamp(-127, 127)), torch.ones_like(amax))
+
+
+def _rows64(x, fmt):
+    blocks = torch.nn.functional.pad(x, (0, -x.shape[1] % 128)).unflatten(1, (-1, 128))
+    scale = _scale64(blocks.abs().amax(2), fmt).repeat_interleave(128, 1)[:, :x.shape[1]]
+    return _grid64(x / scale, fmt) * scale
+
+
+def _weight64(w):
+    n, k = w.shape
+    tall = torch.nn.functional.pad(w.abs(), (0, -k % 128, 0, -n % 128)).unflatten(0, (-1, 128)).amax(1)
+    scale = _scale64(tall.unflatten(1, (-1, 128)).amax(2), "e4m3")
+    scale = scale.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    return _grid64(w / scale, "e4m3") * scale
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    x = s["x"].detach().double()
+    if case["op"] == "norm":
+        w, b = s["ln"].weight.detach().double(), s["ln"].bias.detach().double()
+        var, mean = torch.var_mean(x, dim=1, unbiased=False, keepdim=True)
+        root = torch.sqrt(var + EPS)
+        xh = (x - mean) / root
+        soft = case["act"] == "softplus"
+        y = xh * w + b
+        if soft:
+            y = torch.logaddexp(y, torch.zeros_like(y))
+        if not case["train"]:
+            return [y]
+        if case["kept8"]:
+            scale = _scale64(torch.tensor(case["cols"], dtype=torch.float64, device=x.device).sqrt(), "e4m3")
+            xh = _grid64(xh / scale, "e4m3") * scale
+        g = s["g"].double()
+        if soft:
+            g = g * torch.sigmoid(xh * w + b)
+        dw, db = torch.einsum("mc,mc->c", g, xh), g.sum(0)
+        inner = (g * w * xh).sum(1, keepdim=True) / case["cols"]
+        dx = (g * w - (g * w).sum(1, keepdim=True) / case["cols"] - xh * inner) / root
+        return [y, dx, dw, db]
+    if case["op"] == "rows8":
+        v = _rows64(x, case["format"])
+        if case["use"] == "values":
+            return [v]
+        g = s["g"].double()
+        return [torch.matmul(g.t().contiguous(), v), g.sum(0)]
+    v = _rows64(x, "e4m3")
+    if case["train"]:
+        w = _weight64(s["weight"].detach().double())
+    else:
+        cols = torch.arange(case["cols"], device=x.device)
+        rows = torch.arange(case["out"], device=x.device)
+        w = s["codes"][:, :case["cols"]].double() * _power64(s["exps"].int() - 127)[(rows // 128)[:, None], (cols // 128)[None, :]]
+    y = torch.matmul(v, w.t().contiguous()) + s["bias"].detach().double()
+    if not case["train"]:
+        return [y]
+    g = s["g"].double()
+    return [y, torch.matmul(_rows64(g, "e4m3"), w), torch.matmul(g.t().contiguous(), v), g.sum(0)]
