@@ -163,7 +163,7 @@ def _exponent(amax, most):
     """The smallest e with amax <= most 2^e, most = 0.875 2^p; 0 for an empty block."""
     m, p = torch.frexp(amax)
     e = p - (9 if most == 448.0 else 16) + (m > 0.875).to(p.dtype)
-    return torch.where(amax > 0, e.clamp(-127, 127), torch.zeros_like(e))
+    return torch.where(amax > 0, e.clamp(-126, 127), torch.zeros_like(e))
 
 
 def _packed(x, fmt):
@@ -300,7 +300,7 @@ def _scale64(amax, fmt):
     most = _FORMATS[fmt][1]
     e = torch.frexp(amax / most).exponent
     e = torch.where(_power64(e - 1) * most >= amax, e - 1, e)
-    return torch.where(amax > 0, _power64(e.clamp(-127, 127)), torch.ones_like(amax))
+    return torch.where(amax > 0, _power64(e.clamp(-126, 127)), torch.ones_like(amax))
 
 
 def _rows64(x, fmt):
