@@ -169,7 +169,10 @@ GANET_SYMBOLS = ["ganet_linear_wgrad_workspace", "ganet_linear_wgrad", "ganet_bn
                  "ganet_unet_saved_floats", "ganet_unet_fwd_workspace", "ganet_unet_fwd",
                  "ganet_unet_bwd_workspace", "ganet_unet_bwd", "ganet_profile_create", "ganet_profile_destroy", "ganet_profile_bind", "ganet_profile_count", "ganet_profile_read", "ganet_profile_kernel_name",
                  "ganet_conv5_packed_bytes", "ganet_conv5_pack", "ganet_conv5_apply",
-                 "ganet_conv5_wgrad_workspace", "ganet_conv5_wgrad", "ganet_last_error", "ganet_abi_version"]
+                 "ganet_conv5_wgrad_workspace", "ganet_conv5_wgrad",
+                 "ganet_ln_code_exponent", "ganet_ln_fwd", "ganet_ln_bwd_workspace", "ganet_ln_bwd", "ganet_rows8_pack", "ganet_rows8_unpack",
+                 "ganet_weight8_pack", "ganet_gemm8_workspace", "ganet_gemm8", "ganet_wgrad8_workspace", "ganet_wgrad8",
+                 "ganet_last_error", "ganet_abi_version"]
 
 
 class GanetWgradJob(ctypes.Structure):
@@ -332,9 +335,32 @@ def ganet() -> ctypes.CDLL:
         lib.ganet_conv5_wgrad_workspace.argtypes = [c_int32, c_int32, c_int32]
         lib.ganet_conv5_wgrad.restype = c_int
         lib.ganet_conv5_wgrad.argtypes = [c_int32, c_int32, c_int32, P, P, P, P, c_size_t, P]
+        I, L = c_int32, c_int64
+        lib.ganet_ln_code_exponent.restype = c_int32
+        lib.ganet_ln_code_exponent.argtypes = [L]
+        lib.ganet_ln_fwd.restype = c_int
+        lib.ganet_ln_fwd.argtypes = [L, L, I, I, P, L, P, P, c_float, I, P, P, P, P, L, P]
+        lib.ganet_ln_bwd_workspace.restype = c_size_t
+        lib.ganet_ln_bwd_workspace.argtypes = [L, L, I]
+        lib.ganet_ln_bwd.restype = c_int
+        lib.ganet_ln_bwd.argtypes = [L, L, I, I, P, L, P, P, L, P, P, P, I, P, L, P, P, P, P, c_size_t, P]
+        lib.ganet_rows8_pack.restype = c_int
+        lib.ganet_rows8_pack.argtypes = [L, L, I, I, P, L, P, L, P, L, P]
+        lib.ganet_rows8_unpack.restype = c_int
+        lib.ganet_rows8_unpack.argtypes = [L, L, I, I, P, L, P, L, P, P]
+        lib.ganet_weight8_pack.restype = c_int
+        lib.ganet_weight8_pack.argtypes = [L, L, I, P, L, P, L, P, L, P, L, P, L, P]
+        lib.ganet_gemm8_workspace.restype = c_size_t
+        lib.ganet_gemm8_workspace.argtypes = [L, L, L]
+        lib.ganet_gemm8.restype = c_int
+        lib.ganet_gemm8.argtypes = [L, L, L, I, P, L, P, L, P, L, P, L, P, I, P, L, I, P, c_size_t, P]
+        lib.ganet_wgrad8_workspace.restype = c_size_t
+        lib.ganet_wgrad8_workspace.argtypes = [L, L, L, I]
+        lib.ganet_wgrad8.restype = c_int
+        lib.ganet_wgrad8.argtypes = [L, L, L, I, I, P, L, P, L, P, L, P, P, I, P, c_size_t, P]
         lib.ganet_last_error.restype = c_char_p
         lib.ganet_abi_version.restype = c_int
-        if lib.ganet_abi_version() != 9:
+        if lib.ganet_abi_version() != 10:
             raise RuntimeError("libganet_hip.so ABI version mismatch; rebuild")
         _ganet = lib
     return _ganet

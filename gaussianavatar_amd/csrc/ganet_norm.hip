@@ -1,0 +1,581 @@
+// ganet_norm.hip — layer norm over the columns of a row + activation, forward and backward (include/ganet.h: ganet_ln_*).
+//
+//   xh = (x - mean) rstd, u = w xh + b, y = act(u)
+//   g = dy act'(u), dw = sum_rows g xh, db = sum_rows g, dx = rstd (g w - mean_c(g w) - xh mean_c(g w xh))
+//
+// Bound: HBM. Forward reads x and writes y once, backward reads x (or its 8-bit xh) and dy and writes dx once: a row stays in
+// registers between its reduction and its use, the variance is taken about the mean (no E[x^2] - mean^2). A group of G lanes holds
+// a row, NC vectors of 16 bytes each: G = 1 .. 64 lanes of a wave for rows up to 4 KiB, a whole workgroup of 256 .. 1024 threads
+// up to 32 KiB, and a streaming form that reads the row three times (from cache) beyond. Groups stride over the rows, so
+// a lane always sees the same columns: w and b are loaded once, dw and db are summed in registers and leave as ONE partial row pair per workgroup,
+// added in a fixed order by a second kernel (no atomics: bit-reproducible).
+//
+// xh as 8-bit codes: |xh| <= sqrt(C) for every input (sum xh^2 <= C), so the power of two that makes sqrt(C) fit the format is
+// known before a value is seen: no maximum to take and no exponents to store.
+#include <cmath>
+
+#include "ganet_rows8.h"
+
+namespace ganet {
+using namespace rows8;
+
+namespace {
+
+constexpr int ACT_NONE = 0, ACT_RELU = 2;      // (1: softplus)
+constexpr int LN_WG = 256;
+
+// softplus = max(u, 0) + log1p(exp(-|u|)): relative accuracy on both sides (torch's threshold of 20 differs by 2e-9 of the value).
+// log1p by the series where exp(-|u|) is small: the hardware logarithm of 1 + e keeps 1e-7 absolute only.
+__device__ __forceinline__ float act_fwd(float u, int act) {
+  if (act == ACT_NONE) return u;
+  if (act == ACT_RELU) return u > 0.f || u != u ? u : 0.f;
+  const float e = __expf(-fabsf(u));
+  const float l = e < 0.0625f ? e * (1.f - e * (0.5f - e * (0.333333333f - e * (0.25f - e * 0.2f)))) : __logf(1.f + e);
+  return fmaxf(u, 0.f) + l + (u != u ? u : 0.f);
+}
+__device__ __forceinline__ float act_grad(float u, int act) {
+  if (act == ACT_NONE) return 1.f;
+  if (act == ACT_RELU) return u > 0.f ? 1.f : (u != u ? u : 0.f);
+  const float e = __expf(-fabsf(u));
+  const float r = 1.f / (1.f + e);
+  return u > 0.f ? r : (u != u ? u : e * r);
+}
+
+template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
+
+// Sum over the lanes that hold a row; every lane gets it. WIDE: over the workgroup, through LDS (two buffers in turn: a
+// buffer is written again only after a barrier that every reader of its last content has passed).
+template <bool WIDE, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int G, float* s_red, int& phase) {
+  if (!WIDE) {
+    for (int off = 1; off < G; off <<= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off);
+    }
+    return;
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off);
+  }
+  const int nw = blockDim.x >> 6, wave = threadIdx.x >> 6;
+  float* s = s_red + phase * 2 * 16;
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i * 16 + wave] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float t = 0.f;
+    for (int w = 0; w < nw; ++w) t += s[i * 16 + w];
+    v[i] = t;
+  }
+  phase ^= 1;
+}
+
+template <typename T, int NC, bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+ln_fwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
+              const void* __restrict__ b, int32_t wtype, float eps, int act, T* __restrict__ y, float* __restrict__ mean_out,
+              float* __restrict__ rstd_out, uint8_t* __restrict__ codes, int64_t ldc, float code_scale) {
+  constexpr int V = VEC<T>;
+  __shared__ float s_red[2 * 2 * 16];
+  int phase = 0;
+  const int l = WIDE ? threadIdx.x : (threadIdx.x & (G - 1));
+  const int groups = WIDE ? 1 : THREADS / G, grp = WIDE ? 0 : threadIdx.x / G;
+  const float inv = 1.0f / (float)C;
+  float wv[NC][V], bv[NC][V];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t c = (int64_t)(j * G + l) * V + i;
+      wv[j][i] = (w && c < C) ? load_param(w, wtype, c) : 1.f;
+      bv[j][i] = (b && c < C) ? load_param(b, wtype, c) : 0.f;
+    }
+  }
+  // every lane of a wave takes the same number of turns: the shuffles need whole groups, a turn without a row reads nothing
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < M; r0 += (int64_t)gridDim.x * groups) {
+    const int64_t row = r0 + grp;
+    const bool live = row < M;
+    float v[NC][V];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int64_t c = (int64_t)(j * G + l) * V;
+      load_n(x + row * ldx + c, live ? C - c : 0, v[j]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[0] += v[j][i];
+    }
+    row_sum<WIDE>(s, G, s_red, phase);
+    const float mean = s[0] * inv;
+    s[0] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int64_t c = (int64_t)(j * G + l) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[j][i] = c + i < C ? v[j][i] - mean : 0.f;
+        s[0] = fmaf(v[j][i], v[j][i], s[0]);
+      }
+    }
+    row_sum<WIDE>(s, G, s_red, phase);
+    const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+    if (live && l == 0) {
+      if (mean_out) mean_out[row] = mean;
+      if (rstd_out) rstd_out[row] = rstd;
+    }
+    if (!live) continue;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int64_t c = (int64_t)(j * G + l) * V;
+      if (c >= C) continue;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j][i] *= rstd;
+      if (codes) {
+        uint8_t* p = codes + row * ldc + c;                // c is a multiple of V: aligned to V bytes; ldc covers the last vector
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q)
+          reinterpret_cast<unsigned*>(p)[q] =
+              pack4<GANET_E4M3>(v[j][4 * q] * code_scale, v[j][4 * q + 1] * code_scale, v[j][4 * q + 2] * code_scale,
+                                v[j][4 * q + 3] * code_scale);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j][i] = act_fwd(fmaf(v[j][i], wv[j][i], bv[j][i]), act);
+      store_n(y + row * C + c, C - c, v[j]);
+    }
+  }
+}
+
+// Streaming form: rows beyond 2048 vectors. One workgroup per row, three reads of the row.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+ln_fwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
+                     const void* __restrict__ b, int32_t wtype, float eps, int act, T* __restrict__ y,
+                     float* __restrict__ mean_out, float* __restrict__ rstd_out, uint8_t* __restrict__ codes, int64_t ldc,
+                     float code_scale) {
+  constexpr int V = VEC<T>;
+  __shared__ float s_red[2 * 2 * 16];
+  int phase = 0;
+  const double inv = 1.0 / (double)C;
+  for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
+    const T* xr = x + row * ldx;
+    float v[V];
+    float s[1] = {0.f};
+    for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
+      load_n(xr + c, C - c, v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[0] += v[i];
+    }
+    row_sum<true>(s, 0, s_red, phase);
+    const float mean = (float)(s[0] * inv);
+    s[0] = 0.f;
+    for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
+      load_n(xr + c, C - c, v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = c + i < C ? v[i] - mean : 0.f;
+        s[0] = fmaf(d, d, s[0]);
+      }
+    }
+    row_sum<true>(s, 0, s_red, phase);
+    const float rstd = 1.0f / sqrtf((float)(s[0] * inv) + eps);
+    if (threadIdx.x == 0) {
+      if (mean_out) mean_out[row] = mean;
+      if (rstd_out) rstd_out[row] = rstd;
+    }
+    for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
+      load_n(xr + c, C - c, v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = (v[i] - mean) * rstd;
+      if (codes) {
+        uint8_t* p = codes + row * ldc + c;
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q)
+          reinterpret_cast<unsigned*>(p)[q] = pack4<GANET_E4M3>(v[4 * q] * code_scale, v[4 * q + 1] * code_scale,
+                                                                v[4 * q + 2] * code_scale, v[4 * q + 3] * code_scale);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float wi = (w && c + i < C) ? load_param(w, wtype, c + i) : 1.f;
+        const float bi = (b && c + i < C) ? load_param(b, wtype, c + i) : 0.f;
+        v[i] = act_fwd(fmaf(v[i], wi, bi), act);
+      }
+      store_n(y + row * C + c, C - c, v);
+    }
+  }
+}
+
+// xh of one vector: from x, or from its codes. Columns beyond C read as zero.
+template <typename T, bool KEPT8>
+__device__ __forceinline__ void load_xh(const T* xr, const uint8_t* cr, int64_t c, int64_t C, bool live, float mean, float rstd,
+                                        float code_unit, float (&xh)[VEC<T>]) {
+  constexpr int V = VEC<T>;
+  if (KEPT8) {
+    const bool in = live && c < C;
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      float t[4];
+      unpack4<GANET_E4M3>(in ? reinterpret_cast<const unsigned*>(cr + c)[q] : 0u, t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xh[4 * q + i] = c + 4 * q + i < C ? t[i] * code_unit : 0.f;
+    }
+  } else {
+    load_n(xr + c, live ? C - c : 0, xh);
+#pragma unroll
+    for (int i = 0; i < V; ++i) xh[i] = (live && c + i < C) ? (xh[i] - mean) * rstd : 0.f;
+  }
+}
+
+template <typename T, int NC, bool WIDE, int THREADS, bool KEPT8>
+__global__ void __launch_bounds__(THREADS)
+ln_bwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx, const float* __restrict__ mean_in,
+              const uint8_t* __restrict__ codes, int64_t ldc, float code_unit, const float* __restrict__ rstd_in,
+              const void* __restrict__ w, const void* __restrict__ b, int32_t wtype, int act, const T* __restrict__ dy,
+              int64_t lddy, T* __restrict__ dx, float* __restrict__ part) {
+  constexpr int V = VEC<T>;
+  extern __shared__ float s_mem[];             // the partial sums of the waves (not WIDE)
+  __shared__ float s_red[2 * 2 * 16];
+  int phase = 0;
+  const int l = WIDE ? threadIdx.x : (threadIdx.x & (G - 1));
+  const int groups = WIDE ? 1 : THREADS / G, grp = WIDE ? 0 : threadIdx.x / G;
+  const float inv = 1.0f / (float)C;
+  float wv[NC][V], bv[NC][V], aw[NC][V], ab[NC][V];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t c = (int64_t)(j * G + l) * V + i;
+      wv[j][i] = (w && c < C) ? load_param(w, wtype, c) : 1.f;
+      bv[j][i] = (b && c < C) ? load_param(b, wtype, c) : 0.f;
+      aw[j][i] = 0.f;
+      ab[j][i] = 0.f;
+    }
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < M; r0 += (int64_t)gridDim.x * groups) {
+    const int64_t row = r0 + grp;
+    const bool live = row < M;
+    const float mean = (!KEPT8 && live) ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
+    float xh[NC][V], g[NC][V];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int64_t c = (int64_t)(j * G + l) * V;
+      load_n(dy + row * lddy + c, live ? C - c : 0, g[j]);
+      load_xh<T, KEPT8>(x + row * ldx, codes + row * ldc, c, C, live, mean, rstd, code_unit, xh[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (act != ACT_NONE) g[j][i] *= act_grad(fmaf(xh[j][i], wv[j][i], bv[j][i]), act);
+        if (live) {
+          aw[j][i] = fmaf(g[j][i], xh[j][i], aw[j][i]);
+          ab[j][i] += g[j][i];
+        }
+        g[j][i] *= wv[j][i];
+        s[0] += g[j][i];
+        s[1] = fmaf(g[j][i], xh[j][i], s[1]);
+      }
+    }
+    row_sum<WIDE>(s, G, s_red, phase);
+    if (dx && live) {
+      const float m1 = s[0] * inv, m2 = s[1] * inv;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int64_t c = (int64_t)(j * G + l) * V;
+        if (c >= C) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[j][i] = rstd * (g[j][i] - m1 - xh[j][i] * m2);
+        store_n(dx + row * C + c, C - c, g[j]);
+      }
+    }
+  }
+  if (!part) return;
+  float* out = part + (int64_t)blockIdx.x * 2 * C;
+  if (WIDE) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int64_t c = (int64_t)(j * G + l) * V;
+      store_n(out + c, C - c, aw[j]);
+      store_n(out + C + c, C - c, ab[j]);
+    }
+    return;
+  }
+  // groups of a wave by shuffles, then the waves through LDS (one row pair each)
+  for (int off = G; off < 64; off <<= 1) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        aw[j][i] += __shfl_xor(aw[j][i], off);
+        ab[j][i] += __shfl_xor(ab[j][i], off);
+      }
+    }
+  }
+  const int wave = threadIdx.x >> 6, cols = G * NC * V;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {                // dw, then db, through the same LDS
+    if (k) __syncthreads();
+    if ((threadIdx.x & 63) < G) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) s_mem[wave * cols + (j * G + l) * V + i] = k ? ab[j][i] : aw[j][i];
+      }
+    }
+    __syncthreads();
+    for (int64_t c = threadIdx.x; c < C; c += THREADS) {
+      float t = 0.f;
+#pragma unroll
+      for (int v = 0; v < THREADS / 64; ++v) t += s_mem[v * cols + c];
+      out[k * C + c] = t;
+    }
+  }
+}
+
+// Streaming form of the input gradient (two reads of the row), and the column sums over slices of the rows.
+template <typename T, bool KEPT8>
+__global__ void __launch_bounds__(1024)
+ln_bwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx, const float* __restrict__ mean_in,
+                     const uint8_t* __restrict__ codes, int64_t ldc, float code_unit, const float* __restrict__ rstd_in,
+                     const void* __restrict__ w, const void* __restrict__ b, int32_t wtype, int act, const T* __restrict__ dy,
+                     int64_t lddy, T* __restrict__ dx) {
+  constexpr int V = VEC<T>;
+  __shared__ float s_red[2 * 2 * 16];
+  int phase = 0;
+  const float inv = (float)(1.0 / (double)C);
+  for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
+    const float mean = KEPT8 ? 0.f : mean_in[row], rstd = rstd_in[row];
+    float m1 = 0.f, m2 = 0.f;
+    for (int pass = 0; pass < 2; ++pass) {
+      float s[2] = {0.f, 0.f};
+      for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
+        float g[V], xh[V];
+        load_n(dy + row * lddy + c, C - c, g);
+        load_xh<T, KEPT8>(x + row * ldx, codes + row * ldc, c, C, true, mean, rstd, code_unit, xh);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float wi = (w && c + i < C) ? load_param(w, wtype, c + i) : 1.f;
+          const float bi = (b && c + i < C) ? load_param(b, wtype, c + i) : 0.f;
+          if (act != ACT_NONE) g[i] *= act_grad(fmaf(xh[i], wi, bi), act);
+          g[i] *= wi;
+          s[0] += g[i];
+          s[1] = fmaf(g[i], xh[i], s[1]);
+          g[i] = rstd * (g[i] - m1 - xh[i] * m2);
+        }
+        if (pass) store_n(dx + row * C + c, C - c, g);
+      }
+      if (!pass) {
+        row_sum<true>(s, 0, s_red, phase);
+        m1 = s[0] * inv;
+        m2 = s[1] * inv;
+      }
+    }
+  }
+}
+
+template <typename T, bool KEPT8>
+__global__ void __launch_bounds__(LN_WG)
+ln_bwd_columns_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx, const float* __restrict__ mean_in,
+                      const uint8_t* __restrict__ codes, int64_t ldc, float code_unit, const float* __restrict__ rstd_in,
+                      const void* __restrict__ w, const void* __restrict__ b, int32_t wtype, int act,
+                      const T* __restrict__ dy, int64_t lddy, float* __restrict__ part) {
+  constexpr int V = VEC<T>;
+  const int64_t c = ((int64_t)blockIdx.x * LN_WG + threadIdx.x) * V;
+  if (c >= C) return;
+  float aw[V] = {}, ab[V] = {};
+  for (int64_t row = blockIdx.y; row < M; row += gridDim.y) {
+    float g[V], xh[V];
+    load_n(dy + row * lddy + c, C - c, g);
+    load_xh<T, KEPT8>(x + row * ldx, codes + row * ldc, c, C, true, KEPT8 ? 0.f : mean_in[row], rstd_in[row], code_unit, xh);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (act != ACT_NONE && c + i < C)
+        g[i] *= act_grad(fmaf(xh[i], w ? load_param(w, wtype, c + i) : 1.f, b ? load_param(b, wtype, c + i) : 0.f), act);
+      aw[i] = fmaf(g[i], xh[i], aw[i]);
+      ab[i] += g[i];
+    }
+  }
+  float* out = part + (int64_t)blockIdx.y * 2 * C;
+  store_n(out + c, C - c, aw);
+  store_n(out + C + c, C - c, ab);
+}
+
+// dw / db: the workgroups' partial rows, added in order: 16 slices of the partial rows by 16 columns
+__global__ void __launch_bounds__(256)
+ln_bwd_final_kernel(int64_t C, int parts, const float* __restrict__ part, void* __restrict__ dw, void* __restrict__ db,
+                    int32_t wtype) {
+  __shared__ float s[16][17];
+  const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + cl;
+  float t = 0.f;
+  if (c < 2 * C)
+    for (int p = sl; p < parts; p += 16) t += part[(int64_t)p * 2 * C + c];
+  s[sl][cl] = t;
+  __syncthreads();
+  if (sl == 0 && c < 2 * C) {
+    t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += s[k][cl];
+    if (c < C) { if (dw) store_param(dw, wtype, c, t); }
+    else if (db) store_param(db, wtype, c - C, t);
+  }
+}
+
+struct Shape { int form; int G; int NC; int threads; };        // form 0: lanes of a wave, 1: workgroup, 2: streaming
+Shape make_shape(int64_t C, int32_t type) {
+  const int64_t n = cdiv(C, 16 / type_size(type));             // 16-byte vectors of a row
+  Shape s{0, 1, 1, LN_WG};
+  if (n <= 256) {
+    // two vectors per lane where the row gives them: half the shuffles, twice the loads in flight of one vector per lane
+    while (s.G < 64 && s.G * 2 < n) s.G *= 2;
+    s.NC = n <= s.G ? 1 : n <= 2 * s.G ? 2 : 4;
+  } else if (n <= 2048) {
+    s.form = 1;
+    s.NC = 2;
+    s.threads = n <= 512 ? 256 : n <= 1024 ? 512 : 1024;
+    s.G = s.threads;
+  } else {
+    s.form = 2;
+    s.threads = 1024;
+  }
+  return s;
+}
+
+constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024, STREAM_SLICES = 64;
+int64_t fwd_grid(const Shape& s, int64_t M) {
+  const int64_t rows = s.form ? 1 : s.threads / s.G;
+  const int64_t g = cdiv(M, rows);
+  return g < FWD_BLOCKS ? g : FWD_BLOCKS;
+}
+int64_t bwd_grid(const Shape& s, int64_t M) {
+  if (s.form == 2) return M < STREAM_SLICES ? M : STREAM_SLICES;
+  const int64_t rows = s.form ? 1 : s.threads / s.G;
+  const int64_t g = cdiv(M, rows);
+  return g < BWD_BLOCKS ? g : BWD_BLOCKS;
+}
+
+bool ln_ok(int64_t M, int64_t C, int32_t type, int32_t wtype, int32_t act) {
+  return rows_ok(M, C) && type_ok(type) && type_ok(wtype) && act >= 0 && act <= 2;
+}
+
+}  // namespace
+}  // namespace ganet
+
+using namespace ganet;
+
+extern "C" {
+
+int32_t ganet_ln_code_exponent(int64_t C) {
+  // the smallest e with sqrt(C) <= 448 2^e
+  int e = -8;
+  while (e < 16 && (double)C > 200704.0 * std::pow(4.0, e)) ++e;
+  return e;
+}
+
+int ganet_ln_fwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* x, int64_t ldx, const void* w, const void* b,
+                 float eps, int32_t act, void* y, float* mean, float* rstd, void* codes, int64_t ldc, void* stream_) {
+  if (!ln_ok(M, C, type, wtype, act)) {
+    set_error("ganet_ln_fwd: unsupported M=%lld C=%lld types=%d,%d act=%d", (long long)M, (long long)C, type, wtype, act);
+    return 4;
+  }
+  if (M == 0) return 0;
+  if (!x || !y || (ldx < C && M > 1) || (codes && (ldc % 16 || ldc < pad16(C) || (reinterpret_cast<uintptr_t>(codes) & 15)))) {
+    set_error("ganet_ln_fwd: NULL or misaligned argument, or a row stride too small");
+    return 1;
+  }
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  const Shape s = make_shape(C, type);
+  const float cs = std::ldexp(1.0f, -ganet_ln_code_exponent(C));
+  const dim3 grid((unsigned)(s.form == 2 ? (M < FWD_BLOCKS ? M : FWD_BLOCKS) : fwd_grid(s, M)));
+  uint8_t* cd = static_cast<uint8_t*>(codes);
+#define LN_FWD(NC, WIDE, TH)                                                                                            \
+  hipLaunchKernelGGL((ln_fwd_kernel<T, NC, WIDE, TH>), grid, dim3(TH), 0, stream, M, C, s.G, static_cast<const T*>(x), ldx, w, b, \
+                     wtype, eps, act, static_cast<T*>(y), mean, rstd, cd, ldc, cs)
+  GANET_BY_TYPE(type, T, {
+    if (s.form == 2)
+      hipLaunchKernelGGL(ln_fwd_stream_kernel<T>, grid, dim3(1024), 0, stream, M, C, static_cast<const T*>(x), ldx, w, b,
+                         wtype, eps, act, static_cast<T*>(y), mean, rstd, cd, ldc, cs);
+    else if (s.form == 1) {
+      if (s.threads == 256) LN_FWD(2, true, 256);
+      else if (s.threads == 512) LN_FWD(2, true, 512);
+      else LN_FWD(2, true, 1024);
+    } else {
+      if (s.NC == 1) LN_FWD(1, false, LN_WG);
+      else if (s.NC == 2) LN_FWD(2, false, LN_WG);
+      else LN_FWD(4, false, LN_WG);
+    }
+  });
+#undef LN_FWD
+  return check_hip(hipGetLastError(), "ganet_ln_fwd");
+}
+
+size_t ganet_ln_bwd_workspace(int64_t M, int64_t C, int32_t type) {
+  if (!rows_ok(M, C) || !type_ok(type)) return 0;
+  return (size_t)bwd_grid(make_shape(C, type), M < 1 ? 1 : M) * 2 * (size_t)C * sizeof(float);
+}
+
+int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* x, int64_t ldx, const float* mean,
+                 const void* codes, int64_t ldc, const float* rstd, const void* w, const void* b, int32_t act,
+                 const void* dy, int64_t lddy, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes,
+                 void* stream_) {
+  if (!ln_ok(M, C, type, wtype, act)) {
+    set_error("ganet_ln_bwd: unsupported M=%lld C=%lld types=%d,%d act=%d", (long long)M, (long long)C, type, wtype, act);
+    return 4;
+  }
+  const bool sums = dw || db;
+  if ((M > 0 && (!rstd || !dy || (!codes && (!x || !mean)) || (!codes && ldx < C && M > 1) || (lddy < C && M > 1))) ||
+      (codes && (ldc % 16 || ldc < pad16(C) || (reinterpret_cast<uintptr_t>(codes) & 15))) ||
+      (sums && (!workspace || workspace_bytes < ganet_ln_bwd_workspace(M, C, type)))) {
+    set_error("ganet_ln_bwd: NULL or misaligned argument, a row stride or the workspace too small");
+    return 1;
+  }
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  const Shape s = make_shape(C, type);
+  const float cu = std::ldexp(1.0f, ganet_ln_code_exponent(C));
+  float* part = sums ? static_cast<float*>(workspace) : nullptr;
+  const uint8_t* cd = static_cast<const uint8_t*>(codes);
+  const int64_t parts = M ? bwd_grid(s, M) : 0;
+#define LN_BWD(NC, WIDE, TH, K8)                                                                                              \
+  hipLaunchKernelGGL((ln_bwd_kernel<T, NC, WIDE, TH, K8>), dim3((unsigned)parts), dim3(TH),                                        \
+                     WIDE ? 0 : (size_t)(TH / 64) * s.G * NC * VEC<T> * sizeof(float), stream, M, C, s.G,                 \
+                     static_cast<const T*>(x), ldx, mean, cd, ldc, cu, rstd, w, b, wtype, act, static_cast<const T*>(dy), lddy, \
+                     static_cast<T*>(dx), part)
+#define LN_BWD_FORMS(K8)                                                                                                      \
+  do {                                                                                                                        \
+    if (s.form == 2) {                                                                                                        \
+      if (dx)                                                                                                                 \
+        hipLaunchKernelGGL((ln_bwd_stream_kernel<T, K8>), dim3((unsigned)(M < BWD_BLOCKS ? M : BWD_BLOCKS)), dim3(1024), 0, stream, \
+                           M, C, static_cast<const T*>(x), ldx, mean, cd, ldc, cu, rstd, w, b, wtype, act,                     \
+                           static_cast<const T*>(dy), lddy, static_cast<T*>(dx));                                             \
+      if (part)                                                                                                               \
+        hipLaunchKernelGGL((ln_bwd_columns_kernel<T, K8>), dim3((unsigned)cdiv(C, LN_WG * VEC<T>), (unsigned)parts), dim3(LN_WG), \
+                           0, stream, M, C, static_cast<const T*>(x), ldx, mean, cd, ldc, cu, rstd, w, b, wtype, act,          \
+                           static_cast<const T*>(dy), lddy, part);                                                            \
+    } else if (s.form == 1) {                                                                                                 \
+      if (s.threads == 256) LN_BWD(2, true, 256, K8);                                                                         \
+      else if (s.threads == 512) LN_BWD(2, true, 512, K8);                                                                    \
+      else LN_BWD(2, true, 1024, K8);                                                                                         \
+    } else {                                                                                                                  \
+      if (s.NC == 1) LN_BWD(1, false, LN_WG, K8);                                                                             \
+      else if (s.NC == 2) LN_BWD(2, false, LN_WG, K8);                                                                        \
+      else LN_BWD(4, false, LN_WG, K8);                                                                                       \
+    }                                                                                                                         \
+  } while (0)
+  if (M > 0) {
+    GANET_BY_TYPE(type, T, {
+      if (codes) LN_BWD_FORMS(true);
+      else LN_BWD_FORMS(false);
+    });
+  }
+#undef LN_BWD_FORMS
+#undef LN_BWD
+  if (sums)       // (also for M = 0: the gradients of no rows are zero)
+    hipLaunchKernelGGL(ln_bwd_final_kernel, dim3((unsigned)cdiv(2 * C, 16)), dim3(256), 0, stream, C, (int)parts, part, dw, db, wtype);
+  return check_hip(hipGetLastError(), "ganet_ln_bwd");
+}
+
+}  // extern "C"

@@ -14,7 +14,7 @@ import threading
 import torch
 import torch.nn.functional as F
 
-from . import _dev, _native, parallel
+from . import _dev, _native, parallel, rows8
 
 
 def _ptr(t):
@@ -110,7 +110,34 @@ class _LinearFn(torch.autograd.Function):
         return dx, dW, db
 
 
-def linear(x, weight, bias):
+class _LinearKept8Fn(torch.autograd.Function):
+    """y = x @ W^T + b in the operands' own type; of x the backward pass keeps 8 bits per value (rows8.quantize8), and
+    the weight gradient reads them as they are kept (rows8.wgrad8)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        rows = rows8.quantize8(x)
+        ctx.save_for_backward(rows.codes, rows.exps, weight)
+        ctx.lead, ctx.cols, ctx.btype = rows.lead, rows.cols, None if bias is None else bias.dtype
+        return F.linear(x, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        codes, exps, weight = ctx.saved_tensors
+        dx = g @ weight if ctx.needs_input_grad[0] else None
+        dW = db = None
+        if ctx.needs_input_grad[1] or (ctx.btype is not None and ctx.needs_input_grad[2]):
+            dW, db = rows8.wgrad8(g, rows8.Rows8(codes, exps, ctx.cols, ctx.lead), weight.dtype)
+            db = None if ctx.btype is None else db.to(ctx.btype)
+        return dx, dW, db
+
+
+def linear(x, weight, bias, checkpoint8=False):
+    """x [..., K] -> x @ weight^T + bias. checkpoint8: what the backward pass keeps of x is its 8-bit rows (a quarter of fp32), so
+    dW is that of the rounded x (2^-4 of a value at most); y and dx are unchanged."""
+    if checkpoint8:
+        return _LinearKept8Fn.apply(x, weight, bias)
     if x.is_cuda and x.dtype == torch.float32 and x.dim() == 2:
         return _LinearFn.apply(x, weight, bias)
     return F.linear(x, weight, bias)
@@ -178,6 +205,112 @@ def batchnorm_act(x, bn: torch.nn.BatchNorm1d, act: str = "softplus"):
             bn.running_mean.mul_(1 - mom).add_(mean, alpha=mom)
             bn.running_var.mul_(1 - mom).add_(var_unbiased, alpha=mom)
     return y
+
+
+_ACTS = {"identity": 0, "softplus": 1, "relu": 2}
+
+
+def _act_plain(u, act):
+    return F.softplus(u) if act == "softplus" else (F.relu(u) if act == "relu" else u)
+
+
+class _LayerNormActFn(torch.autograd.Function):
+    """act(layer_norm(x)) over the last dimension and its gradients. The backward pass keeps x and the rows' mean and rstd, or
+    (kept8) the normalised rows in 8 bits and rstd."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, act, kept8):
+        lib = _native.ganet()
+        x2 = rows8._rows2d(x)
+        M, C = x2.shape
+        grad = any(ctx.needs_input_grad[:3])
+        y = torch.empty((M, C), dtype=x.dtype, device=x.device)
+        f32 = lambda: torch.empty(M, dtype=torch.float32, device=x.device)
+        mean = f32() if grad and not kept8 else None
+        rstd = f32() if grad else None
+        ldc = (C + 15) // 16 * 16
+        codes = torch.empty((M, ldc), dtype=torch.uint8, device=x.device) if grad and kept8 else None
+        wtype = 0 if weight is None else rows8._TYPE_CODE[weight.dtype]
+        rows8._call(x.device, lib.ganet_ln_fwd, M, C, rows8._TYPE_CODE[x.dtype], wtype, _ptr(x2), rows8._ld(x2), _ptr(weight), _ptr(bias),
+                    float(eps), _ACTS[act], _ptr(y), _ptr(mean), _ptr(rstd), _ptr(codes), ldc)
+        ctx.save_for_backward(None if kept8 else x2, weight, bias, mean, rstd, codes)
+        ctx.act, ctx.shape, ctx.dtype = act, x.shape, x.dtype
+        return y.reshape(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        lib = _native.ganet()
+        x2, weight, bias, mean, rstd, codes = ctx.saved_tensors
+        g2 = rows8._rows2d(dy)
+        M, C = g2.shape
+        code = rows8._TYPE_CODE[ctx.dtype]
+        need_x = ctx.needs_input_grad[0]
+        dx = torch.empty((M, C), dtype=ctx.dtype, device=dy.device) if need_x else None
+        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
+        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
+        nbytes = lib.ganet_ln_bwd_workspace(M, C, code) if (dw is not None or db is not None) else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
+        wtype = 0 if weight is None else rows8._TYPE_CODE[weight.dtype]
+        rows8._call(dy.device, lib.ganet_ln_bwd, M, C, code, wtype, _ptr(x2), 0 if x2 is None else rows8._ld(x2), _ptr(mean), _ptr(codes),
+                    0 if codes is None else codes.stride(0), _ptr(rstd), _ptr(weight), _ptr(bias), _ACTS[ctx.act], _ptr(g2),
+                    rows8._ld(g2), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+        return (None if dx is None else dx.reshape(ctx.shape)), dw, db, None, None, None
+
+
+class _LayerNormKept8Plain(torch.autograd.Function):
+    """The same with the normalised rows kept in 8 bits, in torch operations (CPU)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, act):
+        xf = x.float()
+        d = xf - xf.mean(-1, keepdim=True)
+        rstd = torch.rsqrt((d * d).mean(-1, keepdim=True) + eps)
+        xh = d * rstd
+        e = _native.ganet().ganet_ln_code_exponent(x.shape[-1])
+        codes = (xh * 2.0 ** -e).to(torch.float8_e4m3fn)
+        ctx.save_for_backward(codes, rstd, weight, bias)
+        ctx.e, ctx.act = e, act
+        u = xh if weight is None else xh * weight.float()
+        return _act_plain(u if bias is None else u + bias.float(), act).to(x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        codes, rstd, weight, bias = ctx.saved_tensors
+        xh = codes.float() * 2.0 ** ctx.e
+        u = xh if weight is None else xh * weight.float()
+        u = u if bias is None else u + bias.float()
+        g = dy.float()
+        if ctx.act != "identity":
+            g = g * (torch.sigmoid(u) if ctx.act == "softplus" else (u > 0).float())
+        rows = tuple(range(dy.dim() - 1))
+        dw = (g * xh).sum(rows).to(weight.dtype) if weight is not None else None
+        db = g.sum(rows).to(bias.dtype) if bias is not None else None
+        gw = g if weight is None else g * weight.float()
+        dx = rstd * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
+        return dx.to(dy.dtype), dw, db, None, None
+
+
+def layernorm_act(x, ln: torch.nn.LayerNorm, act: str = "softplus", checkpoint8: bool = False):
+    """act(ln(x)) for x [..., C] and a LayerNorm over its last dimension; act: "softplus", "identity" or "relu". Unlike BatchNorm it
+    couples no rows: a rank's share of the rows needs no exchange. fp32 / bf16 / fp16 on a HIP device run one kernel forward and two
+    backward, parameters in any of these types. checkpoint8: the backward pass keeps the normalised rows in 8 bits (C bytes and one
+    float per row) in place of x; y is unchanged, the gradients are those of the rounded rows (2^-4 of a value at most)."""
+    if act not in _ACTS:
+        raise ValueError(f"layernorm_act: act {act!r} (known: {', '.join(_ACTS)})")
+    if len(ln.normalized_shape) != 1 or x.dim() < 1 or x.shape[-1] != ln.normalized_shape[0]:
+        raise ValueError(f"layernorm_act: LayerNorm over {tuple(ln.normalized_shape)} for {tuple(x.shape)}")
+    params = [p for p in (ln.weight, ln.bias) if p is not None]
+    rows8._same_device("layernorm_act", x, *params)
+    known = x.dtype in rows8._TYPE_CODE and all(p.dtype in rows8._TYPE_CODE for p in params) and len({p.dtype for p in params}) < 2
+    if x.is_cuda and known:
+        return _LayerNormActFn.apply(x, ln.weight, ln.bias, ln.eps, act, checkpoint8)
+    if checkpoint8:
+        if x.is_cuda or not known:
+            raise TypeError(f"layernorm_act: checkpoint8 with {x.dtype} rows and {[p.dtype for p in params]} parameters")
+        return _LayerNormKept8Plain.apply(x, ln.weight, ln.bias, ln.eps, act)
+    return _act_plain(ln(x), act)
 
 
 class _SsimL1Fn(torch.autograd.Function):

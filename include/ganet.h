@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define GANET_ABI_VERSION 9
+#define GANET_ABI_VERSION 10
 #define GANET_MAX_TERMS 8
 
 /* ---- dW[N,K] = sum_m g[m,n] x[m,k] ; db[N] = sum_m g[m,n] (db may be NULL).
@@ -369,6 +369,60 @@ int ganet_unet_fwd(const GanetUnetParams* params, int32_t B, const float* x, int
 size_t ganet_unet_bwd_workspace(const GanetUnetParams* params, int32_t B);
 int ganet_unet_bwd(const GanetUnetParams* params, int32_t B, const float* x, const float* saved, const float* d_out,
                    const GanetUnetGrads* grads, void* workspace, size_t workspace_bytes, void* stream, void* side_stream);
+
+/* ---- Row-wise operators in several element types: layer norm, activations kept in 8-bit floating point, and matrix
+ * products of them (csrc/ganet_norm.hip, ganet_rows8.hip, ganet_gemm8.hip, ganet_wgrad8.hip) ----------------------
+ *
+ * Element types of tensors and parameters; formats of codes. Matrices are row-major with a row stride (ld*) in
+ * elements of their own type; a row's elements are adjacent. No alignment beyond the element's own is needed for typed
+ * tensors; codes start on 16 bytes and their row stride is a multiple of 16. */
+#define GANET_F32 0
+#define GANET_BF16 1
+#define GANET_F16 2
+#define GANET_E4M3 0      /* OCP e4m3fn: largest value 448, no infinity */
+#define GANET_E5M2 1      /* OCP e5m2: largest value 57344 */
+
+/* Layer norm over the C columns of each of M rows + activation: xh = (x - mean) rstd, u = w xh + b, y = act(u); act: 0 =
+ * identity, 1 = softplus (beta 1, threshold 20), 2 = relu. w and b (wtype, [C]) may be NULL: 1 and 0. Statistics are taken in
+ * fp32, about the mean. rstd [M] is written for the backward pass, with ONE of: mean [M] (the backward pass reads x again) or
+ * codes [M, ldc] (xh as e4m3 codes of xh 2^-e, e = ganet_ln_code_exponent(C): |xh| <= sqrt(C) <= 448 2^e for every input).
+ * mean, rstd and codes may all be NULL (inference). y is contiguous [M, C]. */
+int32_t ganet_ln_code_exponent(int64_t C);
+int ganet_ln_fwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* x, int64_t ldx, const void* w, const void* b,
+                 float eps, int32_t act, void* y, float* mean, float* rstd, void* codes, int64_t ldc, void* stream);
+/* Backward: dx [M, C] contiguous (NULL: not needed), dw and db [C] in wtype (both NULL: not needed). Either x + mean or
+ * codes. The column sums are added in a fixed order: the same inputs give the same bits. */
+size_t ganet_ln_bwd_workspace(int64_t M, int64_t C, int32_t type);
+int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* x, int64_t ldx, const float* mean,
+                 const void* codes, int64_t ldc, const float* rstd, const void* w, const void* b, int32_t act,
+                 const void* dy, int64_t lddy, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* Rows in 8 bits: every 128 consecutive columns of a row share a power of two. With a the block's largest finite magnitude and
+ * F the format's largest value, e = the smallest integer with a <= F 2^e, at least -126 (a = 0: e = 0); code = x 2^-e rounded to the
+ * nearest value of the format (ties to even); value = code 2^e. A NaN stays NaN; an infinity becomes NaN in e4m3 and stays infinite
+ * in e5m2. codes [M, ldc], columns C .. ldc are zero up to the next multiple of 16; exps [M, lde] hold e + 127, lde a multiple of 4. */
+int ganet_rows8_pack(int64_t M, int64_t C, int32_t type, int32_t fmt, const void* x, int64_t ldx, void* codes, int64_t ldc,
+                     uint8_t* exps, int64_t lde, void* stream);
+/* y [M, C] contiguous = the values; one beyond the type's range becomes its largest number. */
+int ganet_rows8_unpack(int64_t M, int64_t C, int32_t type, int32_t fmt, const void* codes, int64_t ldc, const uint8_t* exps,
+                       int64_t lde, void* y, void* stream);
+/* A weight [N, K] as e4m3 codes, one exponent for each 128 x 128 block (exps [ceil(N / 128), lde]), and, unless NULL, the same codes and
+ * exponents transposed (tcodes [K, ldtc], texps [ceil(K / 128), ldte]) for products with the other side. */
+int ganet_weight8_pack(int64_t N, int64_t K, int32_t type, const void* w, int64_t ldw, void* codes, int64_t ldc, uint8_t* exps,
+                       int64_t lde, void* tcodes, int64_t ldtc, uint8_t* texps, int64_t ldte, void* stream);
+/* y [M, N] = rows [M, K] weight [N, K]^T + bias (btype, NULL: none): e4m3 or e5m2 rows, e4m3 weight; the matrix cores apply the
+ * powers of two and accumulate in fp32; one rounding to ytype. */
+size_t ganet_gemm8_workspace(int64_t M, int64_t N, int64_t K);
+int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes, int64_t ldc, const uint8_t* exps, int64_t lde,
+                const void* wcodes, int64_t ldwc, const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y,
+                int64_t ldy, int32_t ytype, void* workspace, size_t workspace_bytes, void* stream);
+/* dW [N, K] = g^T rows, db [N] = column sums of g (NULL: not needed), both contiguous in otype: the weight gradient of a layer
+ * whose input is kept as rows in 8 bits. g [M, N] in gtype enters with all its bits. */
+size_t ganet_wgrad8_workspace(int64_t M, int64_t N, int64_t K, int32_t gtype);
+int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, const void* g, int64_t ldg, const void* codes,
+                 int64_t ldc, const uint8_t* exps, int64_t lde, void* dW, void* db, int32_t otype, void* workspace,
+                 size_t workspace_bytes, void* stream);
 
 /* Optional per-kernel timing (bench/profiling only). The caller owns a GanetProfile object and binds it to the
  * calling thread; from then on every instrumented launch this thread makes whose kernel id is in `mask` is bracketed by
