@@ -15,6 +15,7 @@ namespace {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 __device__ uint4 g_zeros[1];        // what lanes past the end of a row read
 
@@ -34,115 +35,238 @@ struct Operands {
 
 // ------------------------------------------------------------------------------------------------ tiles through LDS
 // A workgroup of four waves computes 64 MT x 64 NT of y, a wave 32 MT x 32 NT. One step is one block of 128 codes: its rows go
-// from global memory straight into LDS (16 bytes per lane, no registers), the next step's while this one is multiplied. A row is
-// 128 bytes = 8 chunks of 16; chunk c of row r lies at position c ^ ((r >> 1) & 7), so that the 16 rows that a quarter of a wave
-// reads at once lie in 16 different 16-byte columns of LDS. The instruction writes lanes in order, so the swizzle is
-// in the global address that a lane fetches.
+// from global memory straight into LDS (16 bytes per lane, no registers). A row is 128 bytes = 8 chunks of 16; chunk c of row r lies at
+// position c ^ ((r >> 1) & 7), so that the 16 rows that a quarter of a wave reads at once lie in 16 different 16-byte columns of LDS.
+// The instruction writes lanes in order, so the swizzle is in the global address that a lane fetches.
+//
+// Two LDS buffers and two register sets of fragments, half a block (64 codes) each:
+//     read half 1 of step k          | multiply half 0 of step k
+//     step k + 1 landed? barrier     |
+//     fetch step k + 2, read half 0 of step k + 1 | multiply half 1 of step k
+// so that neither LDS nor memory latency stands between two multiplications, and a fetch has a whole step to arrive.
+//
+// The fetches are issued from inline assembly: they have no register result, and the compiler, which cannot tell the two buffers
+// apart, would otherwise wait for the step in flight before it reads the one that has landed. Every wait for them is the explicit one
+// below; nothing else of this loop may leave a vector load pending across it (the scale bytes are taken before the fetches).
+__device__ __forceinline__ void fetch16(const uint8_t* p, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void fetch16(const uint8_t* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+}
+
+// Rows of one operand's tile. Instruction i of a wave fetches rows 32 i + 8 wave + lane / 8; the swizzle does not depend on i, so
+// inside the matrix one lane offset serves all of them.
 template <int ROWS>
-__device__ __forceinline__ void stage(const uint8_t* __restrict__ src, int64_t ld, int64_t r0, int64_t rows, int64_t k0,
-                                      int chunks, uint8_t* lds) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+__device__ __forceinline__ void stage(const uint8_t* tile, int64_t ld, int64_t rows, int64_t k0, int chunks, unsigned lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r = wave * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+  const uint8_t* src = tile + k0;
+  lds += wave * 1024;
+  if (rows >= ROWS && chunks == 8) {
+    const unsigned off = (unsigned)(r * (unsigned)ld + c * 16);
 #pragma unroll
-  for (int i = 0; i < ROWS / 32; ++i) {
-    const int rb = (i * 4 + wave) * 8;                       // this instruction's eight rows
-    const int r = rb + (lane >> 3);
-    const int c = (lane & 7) ^ ((r >> 1) & 7);
-    const int64_t row = r0 + r < rows ? r0 + r : rows - 1;   // rows past the end: results nobody stores
-    const uint8_t* p = c < chunks ? src + row * ld + k0 + c * 16 : reinterpret_cast<const uint8_t*>(g_zeros);
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)p,
-                                     (__attribute__((address_space(3))) unsigned*)(lds + rb * 128), 16, 0, 0);
+    for (int i = 0; i < ROWS / 32; ++i) fetch16(src + i * 32 * ld, off, lds + i * 4096);
+  } else {
+    // the matrix ends in this tile: rows past its end give results that nobody stores, chunks past a row's end are zero
+#pragma unroll 1
+    for (int i = 0; i < ROWS / 32; ++i) {
+      const int64_t row = min((int64_t)(r + i * 32), rows - 1);
+      fetch16(c < chunks ? src + row * ld + c * 16 : reinterpret_cast<const uint8_t*>(g_zeros), lds + i * 4096);
+    }
   }
 }
 
-__device__ __forceinline__ i32x8 fragment(const uint8_t* lds, int row0, int lane, int half) {
-  const int r = row0 + (lane & 31), c = half * 4 + (lane >> 5) * 2, sw = (r >> 1) & 7;
-  const uint4 a = *reinterpret_cast<const uint4*>(lds + r * 128 + ((c ^ sw) * 16));
-  const uint4 b = *reinterpret_cast<const uint4*>(lds + r * 128 + (((c + 1) ^ sw) * 16));
-  return join(a, b);
+// One half block of a wave's rows, 32 codes per lane and 32 rows: chunks 2 (lane / 32) and the next of the half's four.
+template <int TILES>
+__device__ __forceinline__ void read_half(const uint8_t* lds, int lane, int half, i32x8 (&f)[TILES]) {
+  const int r = lane & 31, c = half * 4 + (lane >> 5) * 2, sw = (r >> 1) & 7;
+  const uint8_t* p0 = lds + r * 128 + (c ^ sw) * 16;
+  const uint8_t* p1 = lds + r * 128 + ((c + 1) ^ sw) * 16;
+#pragma unroll
+  for (int i = 0; i < TILES; ++i)
+    f[i] = join(*reinterpret_cast<const uint4*>(p0 + i * 32 * 128), *reinterpret_cast<const uint4*>(p1 + i * 32 * 128));
+}
+
+// Eight codes (dwords d, d + 1) times 2^e as bf16: exact.
+template <int FMT>
+__device__ __forceinline__ bf16x8 decode8(const i32x8& f, int d, float scale) {
+  union { bf16x2 h[4]; bf16x8 v; } r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (FMT == GANET_E4M3) {
+      r.h[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[d + i], scale, false);
+      r.h[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[d + i], scale, true);
+    } else {
+      r.h[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(f[d + i], scale, false);
+      r.h[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(f[d + i], scale, true);
+    }
+  }
+  return r.v;
+}
+
+// acc += b a^T over one half block. The 8-bit instructions align the 64 products of a step before they add them and drop what falls
+// below: 1.2e-5 to 2.5e-5 of a result's norm (measured against 64 bits; the same for the older 16-deep form). That is below the
+// rounding of a 16-bit result and above that of fp32, so an fp32 result (EXACT) takes the bf16 instructions on decoded codes, at half
+// the rate: error 4e-8 on the same inputs.
+template <int FMT, int MT, int NT, bool EXACT>
+__device__ __forceinline__ void multiply(const i32x8 (&a)[MT], const i32x8 (&b)[NT], const int (&sx)[MT], int sw,
+                                         f32x16 (&acc)[NT][MT]) {
+  if (!EXACT) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[j][i], GANET_E4M3, FMT, 0, sw, 0, sx[i]);
+    return;
+  }
+#pragma unroll
+  for (int d = 0; d < 8; d += 2) {                           // 16 products per instruction: eight codes of a lane
+    bf16x8 x[MT], w[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = decode8<FMT>(a[i], d, pow2(sx[i] - 127));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w[j] = decode8<GANET_E4M3>(b[j], d, pow2(sw - 127));
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[j][i], 0, 0, 0);
+  }
 }
 
 template <int FMT, int MT, int NT, typename Y>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 1)
 gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
+  constexpr bool EXACT = sizeof(Y) == 4;
   constexpr int TM = 64 * MT, TN = 64 * NT, BYTES = (TM + TN) * 128;
   extern __shared__ __align__(16) uint8_t s_tiles[];
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s_tiles;
   // Workgroups go round the 8 XCDs in turn: give each XCD one run of tiles (its own L2 sees neighbouring rows and columns), and
   // inside a run walk 8 tiles down before the next column.
   const int T = tiles_m * tiles_n, q = T / 8, rem = T % 8, xcd = blockIdx.x % 8;
   const int t = xcd * q + (xcd < rem ? xcd : rem) + blockIdx.x / 8;
   const int group = t / (8 * tiles_n), gm = min(8, tiles_m - group * 8), in = t - group * 8 * tiles_n;
   const int64_t m0 = (int64_t)(group * 8 + in % gm) * TM, n0 = (int64_t)(in / gm) * TN;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = (wave & 1) * 32 * MT, wn = (wave >> 1) * 32 * NT;
   const int64_t kend = (o.K + 15) / 16 * 16;
   const int KB = (int)((o.K + BLOCK - 1) / BLOCK);
 
+  auto fetch = [&](int kb) {
+    const unsigned lds = lds0 + (kb & 1) * BYTES;
+    const int64_t k0 = (int64_t)kb * BLOCK;
+    const int chunks = (int)min((int64_t)8, (kend - k0) / 16);
+    stage<TM>(o.x + m0 * o.ldx, o.ldx, o.M - m0, k0, chunks, lds);
+    stage<TN>(o.w + n0 * o.ldw, o.ldw, o.N - n0, k0, chunks, lds + TM * 128);
+  };
+  const uint8_t* ex = o.ex + m0 * o.ldex;
+  unsigned exo[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) exo[i] = (unsigned)(min((int64_t)(wm + i * 32 + (lane & 31)), o.M - 1 - m0) * o.ldex);
+  const uint8_t* ew = o.ew + min(n0 + wn, o.N - 1) / BLOCK * o.ldew;         // a wave's 32 NT columns lie in one block
+
+  i32x8 a0[MT], b0[NT], a1[MT], b1[NT];
+  int sx[MT], sw, sx_next[MT], sw_next;
+  // (whole dwords, four blocks at a time, the byte picked when it is taken: a byte's zero extension would wait for its load, and so
+  // for the fetches behind it, where the load stands)
+  auto scales = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sx_next[i] = *reinterpret_cast<const int*>(ex + (kb & ~3) + exo[i]);
+    sw_next = *reinterpret_cast<const int*>(ew + (kb & ~3));
+  };
+  auto take_scales = [&](int kb) {           // the scales are in registers from here on: no wait for them further down
+    const int shift = (kb & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) { asm volatile("" : "+v"(sx_next[i])); sx[i] = (int)((unsigned)sx_next[i] >> shift & 0xffu); }
+    asm volatile("" : "+v"(sw_next));
+    sw = (int)((unsigned)sw_next >> shift & 0xffu);
+  };
+  auto landed = [&]() {                      // this wave's fetches have arrived; after the barrier, every wave's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+
+  scales(0);
+  fetch(0);
+  // the sums start at the bias (its loads run beside the first fetch)
   f32x16 acc[NT][MT];
+  auto start = [&](auto bias) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float v = bias(min(n0 + wn + j * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3), o.N - 1));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i][r] = v;
+      }
+  };
+  if (!o.bias) start([](int64_t) { return 0.f; });
+  else GANET_BY_TYPE(o.btype, B, start([&](int64_t n) { return (float)static_cast<const B*>(o.bias)[n]; }));
+  landed();
+  take_scales(0);
+  if (KB > 1) { scales(1); fetch(1); }
+  read_half<MT>(s_tiles + wm * 128, lane, 0, a0);
+  read_half<NT>(s_tiles + (TM + wn) * 128, lane, 0, b0);
+  for (int kb = 0; kb + 1 < KB; ++kb) {
+    const uint8_t* lds = s_tiles + (kb & 1) * BYTES;
+    read_half<MT>(lds + wm * 128, lane, 1, a1);
+    read_half<NT>(lds + (TM + wn) * 128, lane, 1, b1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply<FMT, MT, NT, EXACT>(a0, b0, sx, sw, acc);
+    __builtin_amdgcn_sched_barrier(0);
+    landed();                                // step kb + 1 is there, and nobody reads this step's buffer any more
+    int px[MT];
+    const int pw = sw;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) px[i] = sx[i];
+    take_scales(kb + 1);
+    if (kb + 2 < KB) { scales(kb + 2); fetch(kb + 2); }
+    const uint8_t* next = s_tiles + ((kb + 1) & 1) * BYTES;
+    read_half<MT>(next + wm * 128, lane, 0, a0);
+    read_half<NT>(next + (TM + wn) * 128, lane, 0, b0);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply<FMT, MT, NT, EXACT>(a1, b1, px, pw, acc);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  {
+    const uint8_t* lds = s_tiles + ((KB - 1) & 1) * BYTES;
+    read_half<MT>(lds + wm * 128, lane, 1, a1);
+    read_half<NT>(lds + (TM + wn) * 128, lane, 1, b1);
+    multiply<FMT, MT, NT, EXACT>(a0, b0, sx, sw, acc);
+    multiply<FMT, MT, NT, EXACT>(a1, b1, sx, sw, acc);
+  }
+  // A lane holds one row m and, four at a time, consecutive columns n. Stored from there, an instruction would touch 32 rows with 16
+  // or 32 bytes each; through LDS (rows of 16 bytes more than the tile's: the 32 rows of a write fall into different banks) every
+  // row leaves in full 16-byte pieces: 57 -> 8 us per 256 x 256 tile.
+  constexpr int V = 16 / (int)sizeof(Y), PITCH = TN + V;
+  Y* s_y = reinterpret_cast<Y*>(s_tiles);
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.f;
-
-  auto fetch = [&](int kb) {
-    uint8_t* lds = s_tiles + (kb & 1) * BYTES;
-    const int64_t k0 = (int64_t)kb * BLOCK;
-    const int chunks = (int)min((int64_t)8, (kend - k0) / 16);
-    stage<TM>(o.x, o.ldx, m0, o.M, k0, chunks, lds);
-    stage<TN>(o.w, o.ldw, n0, o.N, k0, chunks, lds + TM * 128);
-  };
-  const uint8_t* exr[MT];
+      for (int g = 0; g < 4; ++g) {
+        Y v[4];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) exr[i] = o.ex + min(m0 + wm + i * 32 + (lane & 31), o.M - 1) * o.ldex;
-  const uint8_t* ewr[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) ewr[j] = o.ew + min(n0 + wn + j * 32, o.N - 1) / BLOCK * o.ldew;
-
-  fetch(0);
-  for (int kb = 0; kb < KB; ++kb) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                       // step kb has landed for every wave, and nobody reads the other buffer any more
-    if (kb + 1 < KB) fetch(kb + 1);
-    const uint8_t* lds = s_tiles + (kb & 1) * BYTES;
-    int sx[MT], sw[NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sx[i] = exr[i][kb];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) sw[j] = ewr[j][kb];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      i32x8 a[MT], b[NT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[i] = fragment(lds, wm + i * 32, lane, half);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) b[j] = fragment(lds + TM * 128, wn + j * 32, lane, half);
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[j][i], GANET_E4M3, FMT, 0, sw[j], 0, sx[i]);
-    }
-  }
-  // a lane holds one row m and, four at a time, consecutive columns n
-  Y* y = static_cast<Y*>(o.y);
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int64_t n = n0 + wn + j * 32 + g * 8 + (lane >> 5) * 4;
-      float bias[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) bias[r] = (o.bias && n + r < o.N) ? load_param(o.bias, o.btype, n + r) : 0.f;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int64_t m = m0 + wm + i * 32 + (lane & 31);
-        float v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = acc[j][i][g * 4 + r] + bias[r];
-        if (m < o.M) store_n(y + m * o.ldy + n, o.N - n, v);
+        for (int r = 0; r < 4; ++r) v[r] = (Y)acc[j][i][g * 4 + r];
+        Y* d = s_y + (wm + i * 32 + (lane & 31)) * PITCH + wn + j * 32 + g * 8 + (lane >> 5) * 4;
+        __builtin_memcpy(__builtin_assume_aligned(d, 4 * sizeof(Y)), v, sizeof(v));
       }
+  __syncthreads();
+  constexpr int PER_ROW = TN / V, ROWS = 256 / PER_ROW;
+  const int c = threadIdx.x % PER_ROW * V, r0 = threadIdx.x / PER_ROW;
+  Y* y = static_cast<Y*>(o.y) + m0 * o.ldy + n0 + c;
+  const int64_t left = o.N - n0 - c;
+  const int rows = (int)min((int64_t)TM, o.M - m0);
+  if (left >= V) {
+#pragma unroll 8
+    for (int r = r0; r < rows; r += ROWS) {
+      const uint4 v = *reinterpret_cast<const uint4*>(s_y + r * PITCH + c);
+      __builtin_memcpy(y + r * o.ldy, &v, 16);
     }
+  } else {
+    for (int r = r0; r < rows; r += ROWS)
+      for (int e = 0; e < left; ++e) y[r * o.ldy + e] = s_y[r * PITCH + c + e];
   }
 }
 
@@ -216,7 +340,7 @@ gemm8_few_kernel(Operands o) {
 template <int FMT, int MT, int NT, typename Y>
 int launch_tile(const Operands& o, hipStream_t stream) {
   static PerDeviceFlag ready;
-  constexpr int lds = 2 * 64 * (MT + NT) * 128;
+  constexpr int steps = 2 * 64 * (MT + NT) * 128, out = 64 * MT * (64 * NT * (int)sizeof(Y) + 16), lds = steps > out ? steps : out;
   auto k = gemm8_tile_kernel<FMT, MT, NT, Y>;
   if (!ready) {
     const int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
@@ -238,7 +362,8 @@ int launch(const Operands& o, hipStream_t stream) {
     else hipLaunchKernelGGL((gemm8_few_kernel<FMT, 2, Y>), grid, dim3(64 * FEW_WAVES), 0, stream, o);
     return check_hip(hipGetLastError(), "ganet_gemm8");
   }
-  if (cdiv(o.M, 256) * cdiv(o.N, 256) >= 256) return launch_tile<FMT, 4, 4, Y>(o, stream);
+  if constexpr (sizeof(Y) == 2)
+    if (cdiv(o.M, 256) * cdiv(o.N, 256) >= 256) return launch_tile<FMT, 4, 4, Y>(o, stream);
   return launch_tile<FMT, 2, 2, Y>(o, stream);
 }
 

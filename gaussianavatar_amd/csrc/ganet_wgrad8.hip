@@ -19,10 +19,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int WG = 256, TN = 128, TK = 128, STEP = 32;
-// LDS row: 128 columns and 64 bytes more, so that the four rows that a 16-lane group reads start in four different 64-byte columns
-constexpr int PITCH = TK + 32;
-constexpr int PLANE = STEP * PITCH;
+constexpr int WG = 256, STEP = 32;
+// LDS row of a plane: its columns and 64 bytes more, so that the four rows that a 16-lane group reads start in four different
+// 64-byte columns
+constexpr int pitch(int cols) { return cols + 32; }
 
 template <typename G> constexpr int PIECES = 3;
 template <> constexpr int PIECES<__bf16> = 1;
@@ -46,6 +46,7 @@ __device__ __forceinline__ unsigned decode2(unsigned codes, float scale, bool hi
 }
 
 // eight rows (8 (lane / 32) + 0..7 of the 16 that start at m0) of column c0 + lane % 32
+template <int PITCH>
 __device__ __forceinline__ bf16x8 column8(const unsigned short* plane, int m0, int c0, int lane) {
   const int grp = lane >> 4, li = lane & 15;
   const unsigned short* p = plane + (m0 + (grp >> 1) * 8 + (li >> 2)) * PITCH + c0 + (grp & 1) * 16 + (li & 3) * 4;
@@ -61,145 +62,239 @@ struct Job {
   void* dW; void* db; int32_t otype; float* part; int splits; int64_t rows; int tiles_n, tiles_k;
 };
 
-template <int FMT, typename G>
-__global__ void __launch_bounds__(WG)
+// A workgroup of four waves computes 64 T x 64 T of dW over its range of rows, a wave 32 T x 32 T. A step is 32 rows: thread t brings row
+// t / 8, 8 T columns of g and of x, from global memory into registers two steps ahead, and as bf16 into one of two LDS buffers one
+// step ahead, so that one barrier per step is enough and a load has two steps to arrive.
+template <int FMT, typename G, int T>
+__global__ void __launch_bounds__(WG, T == 4 ? 1 : 2)
 wgrad8_kernel(Job o) {
-  constexpr int P = PIECES<G>;
-  extern __shared__ __align__(16) unsigned short s_mem[];      // P planes of g, one of x
-  unsigned short* const s_x = s_mem + P * PLANE;
+  constexpr int P = PIECES<G>, COLS = 64 * T, PITCH = pitch(COLS), PLANE = STEP * PITCH, BUF = (P + 1) * PLANE;
+  constexpr int GV = 8, GC = COLS / 64;                        // g: GC vectors of 8 elements, 64 columns apart
+  constexpr int XC = COLS / 128;                               // x: XC vectors of 16 codes, one per 128 columns
+  extern __shared__ __align__(16) unsigned short s_mem[];      // two buffers: P planes of g, one of x
   const int tiles = o.tiles_n * o.tiles_k;
   const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
-  const int64_t n0 = (int64_t)(tile / o.tiles_k) * TN, kb = tile % o.tiles_k, k0 = kb * TK;
+  const int64_t n0 = (int64_t)(tile / o.tiles_k) * COLS, k0 = (int64_t)(tile % o.tiles_k) * COLS;
   const int64_t m_lo = split * o.rows, m_hi = min(m_lo + o.rows, o.M);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int wn = (wave & 1) * 64, wk = (wave >> 1) * 64;
-  const int sr = threadIdx.x >> 3, sc = (threadIdx.x & 7) * 16;        // this thread's 16 columns of a staged row
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wn = (wave & 1) * 32 * T, wk = (wave >> 1) * 32 * T;
+  const int sr = threadIdx.x >> 3, st = threadIdx.x & 7;
   const int64_t kend = (o.K + 15) / 16 * 16;
   const G* g = static_cast<const G*>(o.g);
 
-  f32x16 acc[2][2];
+  f32x16 acc[T][T];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < T; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < T; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
   const bool sums = k0 == 0 && o.db;
-  float bias[16] = {};
+  float bias[GC][GV] = {};
 
-  float gv[16];
-  uint4 xv;
-  float scale;
-  auto load = [&](int64_t m) {
-    const int64_t row = m + sr;
-    const bool live = row < m_hi;
-    load_n(g + row * o.ldg + n0 + sc, live ? o.N - (n0 + sc) : 0, gv);
-    const bool in = live && k0 + sc < kend;
-    xv = in ? *reinterpret_cast<const uint4*>(o.codes + row * o.ldc + k0 + sc) : make_uint4(0, 0, 0, 0);
-    scale = in ? pow2((int)o.exps[row * o.lde + kb] - 127) : 1.f;
+  constexpr int GW = GV * (int)sizeof(G) / 16;                 // 16-byte words of a vector of g
+  struct Raw { uint4 g[GC][GW]; uint4 x[XC]; int e[XC]; bool live; };
+  const bool inside = n0 + COLS <= o.N;                        // (uniform: no column of g is missing)
+  auto load = [&](Raw& v, int64_t m) {
+    // rows past the range and columns past the codes load the last ones instead and become zero when they are put
+    v.live = m + sr < m_hi;
+    const int64_t row = min(m + sr, m_hi - 1);
+    const G* gr = g + row * o.ldg + n0 + st * GV;
+    if (inside) {
+#pragma unroll
+      for (int i = 0; i < GC; ++i) __builtin_memcpy(v.g[i], gr + i * 64, 16 * GW);
+    } else {
+#pragma unroll
+      for (int i = 0; i < GC; ++i) {
+        asm("" : "+v"(gr));                                    // (left alone, the compiler merges these loads with the ones above)
+        G t[GV];
+#pragma unroll
+        for (int j = 0; j < GV; ++j) t[j] = n0 + st * GV + i * 64 + j < o.N ? gr[i * 64 + j] : (G)0.f;
+        __builtin_memcpy(v.g[i], t, 16 * GW);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < XC; ++i) {
+      const int64_t k = min(k0 + i * 128 + st * 16, kend - 16);
+      v.x[i] = *reinterpret_cast<const uint4*>(o.codes + row * o.ldc + k);
+      v.e[i] = o.exps[row * o.lde + k / BLOCK];
+    }
   };
-  if (m_lo < m_hi) load(m_lo);
-  for (int64_t m = m_lo; m < m_hi; m += STEP) {
-    __syncthreads();                                   // the tiles of the step before have been read
-    {
-      unsigned* d = reinterpret_cast<unsigned*>(s_x + sr * PITCH + sc);
-      const unsigned c[4] = {xv.x, xv.y, xv.z, xv.w};
+  auto put = [&](const Raw& v, int buf) {
+    unsigned short* base = s_mem + buf * BUF;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        d[2 * i] = decode2<FMT>(c[i], scale, false);
-        d[2 * i + 1] = decode2<FMT>(c[i], scale, true);
+    for (int i = 0; i < XC; ++i) {
+      const unsigned in = v.live && k0 + i * 128 + st * 16 < kend ? ~0u : 0u;
+      const float scale = pow2(v.e[i] - 127);
+      const unsigned c[4] = {v.x[i].x & in, v.x[i].y & in, v.x[i].z & in, v.x[i].w & in};
+      uint4* d = reinterpret_cast<uint4*>(base + P * PLANE + sr * PITCH + i * 128 + st * 16);
+      d[0] = make_uint4(decode2<FMT>(c[0], scale, false), decode2<FMT>(c[0], scale, true), decode2<FMT>(c[1], scale, false),
+                        decode2<FMT>(c[1], scale, true));
+      d[1] = make_uint4(decode2<FMT>(c[2], scale, false), decode2<FMT>(c[2], scale, true), decode2<FMT>(c[3], scale, false),
+                        decode2<FMT>(c[3], scale, true));
+    }
+    const unsigned in = v.live ? ~0u : 0u;
+#pragma unroll
+    for (int i = 0; i < GC; ++i) {
+      uint4 w[GW];
+#pragma unroll
+      for (int q = 0; q < GW; ++q) w[q] = make_uint4(v.g[i][q].x & in, v.g[i][q].y & in, v.g[i][q].z & in, v.g[i][q].w & in);
+      uint4* d = reinterpret_cast<uint4*>(base + sr * PITCH + i * 64 + st * GV);
+      G e[GV];
+      __builtin_memcpy(e, w, sizeof(e));
+      float f[GV];
+#pragma unroll
+      for (int j = 0; j < GV; ++j) f[j] = (float)e[j];
+      if (sums) {
+#pragma unroll
+        for (int j = 0; j < GV; ++j) bias[i][j] += f[j];
+      }
+      if constexpr (P == 1) *d = w[0];
+      else {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          *reinterpret_cast<uint4*>(reinterpret_cast<unsigned short*>(d) + p * PLANE) =
+              make_uint4(pack_hi(f[0], f[1]), pack_hi(f[2], f[3]), pack_hi(f[4], f[5]), pack_hi(f[6], f[7]));
+          if (p + 1 < P) {
+#pragma unroll
+            for (int j = 0; j < GV; ++j) f[j] -= head(f[j]);
+          }
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bias[i] += gv[i];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      unsigned* d = reinterpret_cast<unsigned*>(s_mem + p * PLANE + sr * PITCH + sc);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] = pack_hi(gv[2 * i], gv[2 * i + 1]);
-      if (p + 1 < P) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) gv[i] -= head(gv[i]);
-      }
-    }
-    __syncthreads();
-    if (m + STEP < m_hi) load(m + STEP);
+  };
+  auto compute = [&](int buf) {
+    const unsigned short* base = s_mem + buf * BUF;
 #pragma unroll
     for (int h = 0; h < STEP; h += 16) {
-      bf16x8 x[2];
+      bf16x8 x[T];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) x[j] = column8(s_x, h, wk + j * 32, lane);
+      for (int j = 0; j < T; ++j) x[j] = column8<PITCH>(base + P * PLANE, h, wk + j * 32, lane);
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p)                 // small pieces first
+      for (int p = P - 1; p >= 0; --p)                         // small pieces first
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bf16x8 a = column8(s_mem + p * PLANE, h, wn + i * 32, lane);
+        for (int i = 0; i < T; ++i) {
+          const bf16x8 a = column8<PITCH>(base + p * PLANE, h, wn + i * 32, lane);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[j], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < T; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[j], acc[i][j], 0, 0, 0);
         }
     }
+  };
+  if (m_lo < m_hi) {
+    Raw va, vb;
+    load(va, m_lo);
+    put(va, 0);
+    load(vb, m_lo + STEP);
+    __syncthreads();
+    for (int64_t m = m_lo; m < m_hi; m += 2 * STEP) {          // (an odd last step multiplies zeros)
+      load(va, m + 2 * STEP);
+      compute(0);
+      put(vb, 1);
+      __syncthreads();
+      load(vb, m + 3 * STEP);
+      compute(1);
+      put(va, 0);
+      __syncthreads();
+    }
   }
-  // a lane holds one column k of 16 rows n of each 32 x 32 tile
+  // A lane holds one column k of 16 rows n of each 32 x 32 tile: an instruction stores 32 adjacent columns of two rows. Offsets
+  // inside the tile fit 32 bits (K < 2^22).
   float* part = o.splits > 1 ? o.part + (int64_t)split * (o.N * o.K + o.N) : nullptr;
+  auto store = [&](auto* out) {
+    out += n0 * o.K + k0;
+    const unsigned K = (unsigned)o.K, rows = (unsigned)min((int64_t)COLS, o.N - n0), cols = (unsigned)min((int64_t)COLS, o.K - k0);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t k = k0 + wk + j * 32 + (lane & 31);
-    if (k >= o.K) continue;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < T; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int64_t n = n0 + wn + i * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
-        if (n >= o.N) continue;
-        if (part) part[n * o.K + k] = acc[i][j][r];
-        else store_param(o.dW, o.otype, n * o.K + k, acc[i][j][r]);
-      }
-  }
-  if (!sums) return;
-  __syncthreads();
-  float* s_b = reinterpret_cast<float*>(s_mem);        // [32][128]: 16 KiB of the planes' 20 or more
+        const unsigned n = wn + i * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
+        const unsigned at = n * K + wk + (lane & 31);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s_b[sr * TN + sc + i] = bias[i];
+        for (int j = 0; j < T; ++j)
+          if (n < rows && wk + j * 32 + (lane & 31) < cols) out[at + j * 32] = acc[i][j][r];
+        __builtin_amdgcn_sched_barrier(0);                     // one row's results in registers at a time
+      }
+  };
+  if (part) store(part);
+  else GANET_BY_TYPE(o.otype, O, store(static_cast<O*>(o.dW)));
+  if (!sums) return;
+  float* s_b = reinterpret_cast<float*>(s_mem);                // [32][COLS]: the buffers are free behind the last barrier
+#pragma unroll
+  for (int i = 0; i < GC; ++i)
+#pragma unroll
+    for (int j = 0; j < GV; ++j) s_b[sr * COLS + i * 64 + st * GV + j] = bias[i][j];
   __syncthreads();
-  if (threadIdx.x >= TN || n0 + threadIdx.x >= o.N) return;
+  if (threadIdx.x >= COLS || n0 + threadIdx.x >= o.N) return;
   float t = 0.f;
-  for (int i = 0; i < STEP; ++i) t += s_b[i * TN + threadIdx.x];
+  for (int i = 0; i < STEP; ++i) t += s_b[i * COLS + threadIdx.x];
   if (part) part[o.N * o.K + n0 + threadIdx.x] = t;
   else store_param(o.db, o.otype, n0 + threadIdx.x, t);
 }
 
+// The ranges' partial sums, added in a fixed order: a workgroup takes 64 adjacent results, its four waves a quarter of the ranges each.
 __global__ void __launch_bounds__(WG)
 wgrad8_reduce_kernel(int64_t NK, int64_t N, int splits, const float* __restrict__ part, void* __restrict__ dW,
                      void* __restrict__ db, int32_t otype) {
-  const int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x, total = NK + (db ? N : 0);
-  if (i >= total) return;
+  __shared__ float s_t[WG];
+  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63), total = NK + (db ? N : 0);
+  const int wave = threadIdx.x >> 6;
   float t = 0.f;
-  for (int s = 0; s < splits; ++s) t += part[(int64_t)s * (NK + N) + i];
+  if (i < total) {
+    const float* p = part + i;
+#pragma unroll 8
+    for (int s = wave; s < splits; s += 4) t += p[(int64_t)s * (NK + N)];
+  }
+  s_t[threadIdx.x] = t;
+  __syncthreads();
+  if (wave || i >= total) return;
+  t = (s_t[threadIdx.x] + s_t[threadIdx.x + 64]) + (s_t[threadIdx.x + 128] + s_t[threadIdx.x + 192]);
   if (i < NK) store_param(dW, otype, i, t);
   else store_param(db, otype, i - NK, t);
 }
 
-// Row ranges: as many as give every CU two workgroups, none shorter than 128 rows
-int split_count(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = cdiv(N, TN) * cdiv(K, TK);
-  int64_t s = cdiv(512, tiles);
+// The tile: 256 x 256 (one workgroup per CU) where that still gives every CU a tile and a range of at least 256 rows, else 128 x 128.
+// The ranges: as many as give every CU a workgroup (two of the small ones), none shorter than 128 rows.
+struct Plan { int T; int64_t tiles_n, tiles_k; int splits; int64_t rows; };
+Plan make_plan(int64_t M, int64_t N, int64_t K) {
+  Plan p;
+  const int64_t big = cdiv(N, 256) * cdiv(K, 256);
+  p.T = (N > 128 && K > 128 && big * cdiv(M, 256) >= 256) ? 4 : 2;
+  p.tiles_n = cdiv(N, 64 * p.T);
+  p.tiles_k = cdiv(K, 64 * p.T);
+  const int64_t tiles = p.tiles_n * p.tiles_k, want = p.T == 4 ? 256 : 512;
+  int64_t s = tiles >= want ? 1 : want / tiles;
   if (s > cdiv(M, 128)) s = cdiv(M, 128);
-  return (int)(s < 1 ? 1 : s);
+  p.splits = (int)(s < 1 ? 1 : s);
+  p.rows = cdiv(cdiv(M, p.splits), STEP) * STEP;
+  return p;
 }
 
-bool wgrad_ok(int64_t M, int64_t N, int64_t K) { return rows_ok(M, K) && N >= 1 && N < (1ll << 24); }
+bool wgrad_ok(int64_t M, int64_t N, int64_t K) { return rows_ok(M, K) && K < (1ll << 22) && N >= 1 && N < (1ll << 24); }
 
-template <int FMT, typename G>
-int launch(Job& o, hipStream_t stream) {
-  constexpr int lds = (PIECES<G> + 1) * PLANE * 2;
+template <int FMT, typename G, int T>
+int launch_tile(const Job& o, hipStream_t stream) {
+  static PerDeviceFlag ready;
+  constexpr int lds = 2 * (PIECES<G> + 1) * STEP * pitch(64 * T) * 2;
+  auto k = wgrad8_kernel<FMT, G, T>;
+  if (!ready) {
+    const int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+                             "ganet_wgrad8");
+    if (rc) return rc;
+    ready = true;
+  }
   const int64_t grid = (int64_t)o.tiles_n * o.tiles_k * o.splits;
   if (grid >= (1ll << 31)) { set_error("ganet_wgrad8: too many tiles"); return 4; }
-  hipLaunchKernelGGL((wgrad8_kernel<FMT, G>), dim3((unsigned)grid), dim3(WG), lds, stream, o);
-  if (o.splits > 1) {
-    const int64_t total = o.N * o.K + (o.db ? o.N : 0);
-    hipLaunchKernelGGL(wgrad8_reduce_kernel, dim3((unsigned)cdiv(total, WG)), dim3(WG), 0, stream, o.N * o.K, o.N, o.splits, o.part,
-                       o.dW, o.db, o.otype);
-  }
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(WG), lds, stream, o);
+  return check_hip(hipGetLastError(), "ganet_wgrad8");
+}
+
+template <int FMT, typename G>
+int launch(const Job& o, int T, hipStream_t stream) {
+  const int rc = T == 4 ? launch_tile<FMT, G, 4>(o, stream) : launch_tile<FMT, G, 2>(o, stream);
+  if (rc || o.splits == 1) return rc;
+  const int64_t total = o.N * o.K + (o.db ? o.N : 0);
+  hipLaunchKernelGGL(wgrad8_reduce_kernel, dim3((unsigned)cdiv(total, 64)), dim3(WG), 0, stream, o.N * o.K, o.N, o.splits, o.part,
+                     o.dW, o.db, o.otype);
   return check_hip(hipGetLastError(), "ganet_wgrad8");
 }
 
@@ -212,7 +307,7 @@ extern "C" {
 
 size_t ganet_wgrad8_workspace(int64_t M, int64_t N, int64_t K, int32_t gtype) {
   if (!wgrad_ok(M, N, K) || !type_ok(gtype)) return 0;
-  const int s = split_count(M, N, K);
+  const int s = make_plan(M, N, K).splits;
   return s > 1 ? (size_t)s * (size_t)(N * K + N) * sizeof(float) : 0;
 }
 
@@ -231,10 +326,10 @@ int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, co
     return 1;
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  Job o{M, N, K, g, ldg, static_cast<const uint8_t*>(codes), ldc, exps, lde, dW, db, otype, static_cast<float*>(workspace),
-        split_count(M, N, K), 0, (int)cdiv(N, TN), (int)cdiv(K, TK)};
-  o.rows = cdiv(cdiv(M, o.splits), STEP) * STEP;
-  GANET_BY_TYPE(gtype, T, return fmt == GANET_E4M3 ? launch<GANET_E4M3, T>(o, stream) : launch<GANET_E5M2, T>(o, stream));
+  const Plan p = make_plan(M, N, K);
+  const Job o{M, N, K, g, ldg, static_cast<const uint8_t*>(codes), ldc, exps, lde, dW, db, otype, static_cast<float*>(workspace),
+              p.splits, p.rows, (int)p.tiles_n, (int)p.tiles_k};
+  GANET_BY_TYPE(gtype, T, return fmt == GANET_E4M3 ? launch<GANET_E4M3, T>(o, p.T, stream) : launch<GANET_E5M2, T>(o, p.T, stream));
 }
 
 }  // extern "C"
