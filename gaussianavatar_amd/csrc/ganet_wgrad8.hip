@@ -64,14 +64,15 @@ struct Job {
 
 // A workgroup of four waves computes 64 T x 64 T of dW over its range of rows, a wave 32 T x 32 T. A step is 32 rows: thread t brings row
 // t / 8, 8 T columns of g and of x, from global memory into registers two steps ahead, and as bf16 into one of two LDS buffers one
-// step ahead, so that one barrier per step is enough and a load has two steps to arrive.
-template <int FMT, typename G, int T>
-__global__ void __launch_bounds__(WG, T == 4 ? 1 : 2)
-wgrad8_kernel(Job o) {
+// step ahead. A step is multiplied in 2 P parts (16 rows, one piece of g); the fragments of the next part are read before a
+// part is multiplied, those of the next step's first part behind the step's one barrier, which stands before its last part: neither
+// memory nor LDS latency stands between two multiplications.
+// INSIDE: the tile ends before column N of g (vectors of 8; else element by element).
+template <int FMT, typename G, int T, bool INSIDE>
+__device__ __forceinline__ void wgrad8_tile(const Job& o, unsigned short* s_mem) {
   constexpr int P = PIECES<G>, COLS = 64 * T, PITCH = pitch(COLS), PLANE = STEP * PITCH, BUF = (P + 1) * PLANE;
   constexpr int GV = 8, GC = COLS / 64;                        // g: GC vectors of 8 elements, 64 columns apart
   constexpr int XC = COLS / 128;                               // x: XC vectors of 16 codes, one per 128 columns
-  extern __shared__ __align__(16) unsigned short s_mem[];      // two buffers: P planes of g, one of x
   const int tiles = o.tiles_n * o.tiles_k;
   const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
   const int64_t n0 = (int64_t)(tile / o.tiles_k) * COLS, k0 = (int64_t)(tile % o.tiles_k) * COLS;
@@ -92,32 +93,34 @@ wgrad8_kernel(Job o) {
   const bool sums = k0 == 0 && o.db;
   float bias[GC][GV] = {};
 
-  constexpr int GW = GV * (int)sizeof(G) / 16;                 // 16-byte words of a vector of g
-  struct Raw { uint4 g[GC][GW]; uint4 x[XC]; int e[XC]; bool live; };
-  const bool inside = n0 + COLS <= o.N;                        // (uniform: no column of g is missing)
+  struct Raw { G g[GC][GV]; uint4 x[XC]; int e[XC]; bool live; };
   auto load = [&](Raw& v, int64_t m) {
-    // rows past the range and columns past the codes load the last ones instead and become zero when they are put
-    v.live = m + sr < m_hi;
-    const int64_t row = min(m + sr, m_hi - 1);
-    const G* gr = g + row * o.ldg + n0 + st * GV;
-    if (inside) {
+    // rows past the range and columns past the matrix load the last ones instead and become zero when they are put (no branch: a
+    // value that two paths may have loaded is waited for where they meet)
+    const int left = (int)min(m_hi - m, (int64_t)STEP);
+    v.live = sr < left;
+    // a uniform base and 32-bit offsets (a step's rows span less than 2^31 bytes)
+    const int64_t m_in = left > 0 ? m : m_hi - 1;
+    const unsigned row = left > 0 ? min(sr, left - 1) : 0;
+    const char* gb = reinterpret_cast<const char*>(g + m_in * o.ldg + n0);
+    const unsigned go = (row * (unsigned)o.ldg + st * GV) * (unsigned)sizeof(G);
 #pragma unroll
-      for (int i = 0; i < GC; ++i) __builtin_memcpy(v.g[i], gr + i * 64, 16 * GW);
-    } else {
+    for (int i = 0; i < GC; ++i) {
+      if constexpr (INSIDE) __builtin_memcpy(v.g[i], gb + i * 64 * sizeof(G) + go, sizeof(v.g[i]));
+      else {
+        const int last = (int)(o.N - 1 - n0), n = st * GV + i * 64;
 #pragma unroll
-      for (int i = 0; i < GC; ++i) {
-        asm("" : "+v"(gr));                                    // (left alone, the compiler merges these loads with the ones above)
-        G t[GV];
-#pragma unroll
-        for (int j = 0; j < GV; ++j) t[j] = n0 + st * GV + i * 64 + j < o.N ? gr[i * 64 + j] : (G)0.f;
-        __builtin_memcpy(v.g[i], t, 16 * GW);
+        for (int j = 0; j < GV; ++j)
+          v.g[i][j] = *reinterpret_cast<const G*>(gb + (row * (unsigned)o.ldg + min(n + j, last)) * (unsigned)sizeof(G));
       }
     }
+    const uint8_t *xb = o.codes + m_in * o.ldc + k0, *eb = o.exps + m_in * o.lde + k0 / BLOCK;
+    const int kleft = (int)min(kend - k0, (int64_t)COLS);
 #pragma unroll
     for (int i = 0; i < XC; ++i) {
-      const int64_t k = min(k0 + i * 128 + st * 16, kend - 16);
-      v.x[i] = *reinterpret_cast<const uint4*>(o.codes + row * o.ldc + k);
-      v.e[i] = o.exps[row * o.lde + k / BLOCK];
+      const int k = min(i * 128 + st * 16, kleft - 16);
+      v.x[i] = *reinterpret_cast<const uint4*>(xb + (row * (unsigned)o.ldc + k));
+      v.e[i] = eb[row * (unsigned)o.lde + k / BLOCK];
     }
   };
   auto put = [&](const Raw& v, int buf) {
@@ -133,69 +136,80 @@ wgrad8_kernel(Job o) {
       d[1] = make_uint4(decode2<FMT>(c[2], scale, false), decode2<FMT>(c[2], scale, true), decode2<FMT>(c[3], scale, false),
                         decode2<FMT>(c[3], scale, true));
     }
-    const unsigned in = v.live ? ~0u : 0u;
 #pragma unroll
     for (int i = 0; i < GC; ++i) {
-      uint4 w[GW];
-#pragma unroll
-      for (int q = 0; q < GW; ++q) w[q] = make_uint4(v.g[i][q].x & in, v.g[i][q].y & in, v.g[i][q].z & in, v.g[i][q].w & in);
       uint4* d = reinterpret_cast<uint4*>(base + sr * PITCH + i * 64 + st * GV);
-      G e[GV];
-      __builtin_memcpy(e, w, sizeof(e));
       float f[GV];
 #pragma unroll
-      for (int j = 0; j < GV; ++j) f[j] = (float)e[j];
-      if (sums) {
+      for (int j = 0; j < GV; ++j)
+        f[j] = v.live && (INSIDE || n0 + st * GV + i * 64 + j < o.N) ? (float)v.g[i][j] : 0.f;
 #pragma unroll
-        for (int j = 0; j < GV; ++j) bias[i][j] += f[j];
-      }
-      if constexpr (P == 1) *d = w[0];
-      else {
+      for (int j = 0; j < GV; ++j) bias[i][j] += f[j];         // (used by the first column of tiles; a branch here costs more)
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          *reinterpret_cast<uint4*>(reinterpret_cast<unsigned short*>(d) + p * PLANE) =
-              make_uint4(pack_hi(f[0], f[1]), pack_hi(f[2], f[3]), pack_hi(f[4], f[5]), pack_hi(f[6], f[7]));
-          if (p + 1 < P) {
+      for (int p = 0; p < P; ++p) {
+        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned short*>(d) + p * PLANE) =
+            make_uint4(pack_hi(f[0], f[1]), pack_hi(f[2], f[3]), pack_hi(f[4], f[5]), pack_hi(f[6], f[7]));
+        if (p + 1 < P) {
 #pragma unroll
-            for (int j = 0; j < GV; ++j) f[j] -= head(f[j]);
-          }
+          for (int j = 0; j < GV; ++j) f[j] -= head(f[j]);
         }
       }
     }
   };
-  auto compute = [&](int buf) {
+  // part q of a step: rows 16 (q / P) .., piece P - 1 - q % P of g (small pieces first)
+  bf16x8 a[2][T], x[2][T];
+  auto read = [&](int buf, int q) {
     const unsigned short* base = s_mem + buf * BUF;
+    const int h = q / P * 16, p = P - 1 - q % P;
 #pragma unroll
-    for (int h = 0; h < STEP; h += 16) {
-      bf16x8 x[T];
+    for (int i = 0; i < T; ++i) a[q & 1][i] = column8<PITCH>(base + p * PLANE, h, wn + i * 32, lane);
+    if (q % P == 0) {
 #pragma unroll
-      for (int j = 0; j < T; ++j) x[j] = column8<PITCH>(base + P * PLANE, h, wk + j * 32, lane);
+      for (int j = 0; j < T; ++j) x[q / P][j] = column8<PITCH>(base + P * PLANE, h, wk + j * 32, lane);
+    }
+  };
+  auto multiply = [&](int q) {
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p)                         // small pieces first
+    for (int i = 0; i < T; ++i)
 #pragma unroll
-        for (int i = 0; i < T; ++i) {
-          const bf16x8 a = column8<PITCH>(base + p * PLANE, h, wn + i * 32, lane);
+      for (int j = 0; j < T; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[q & 1][i], x[q / P][j], acc[i][j], 0, 0, 0);
+  };
+  auto step = [&](Raw& there, Raw& far, int buf, int64_t m) {
+    load(far, m + 2 * STEP);
 #pragma unroll
-          for (int j = 0; j < T; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, x[j], acc[i][j], 0, 0, 0);
+    for (int q = 0; q < 2 * P; ++q) {
+      if (q + 1 < 2 * P) read(buf, q + 1);
+      else {
+        __syncthreads();                     // the next step's tiles stand, and this step's have been read
+        read(buf ^ 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(q);
+      if (q == 0) {                          // (between the multiplications)
+        put(there, buf ^ 1);
+#pragma unroll
+        for (int i = 0; i < T * T; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // a matrix instruction
+          __builtin_amdgcn_sched_group_barrier(0x002, 48 * P / T, 0);    // vector instructions
+          __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);             // an LDS write
         }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   if (m_lo < m_hi) {
     Raw va, vb;
     load(va, m_lo);
-    put(va, 0);
     load(vb, m_lo + STEP);
+    put(va, 0);
     __syncthreads();
+    read(0, 0);
     for (int64_t m = m_lo; m < m_hi; m += 2 * STEP) {          // (an odd last step multiplies zeros)
-      load(va, m + 2 * STEP);
-      compute(0);
-      put(vb, 1);
-      __syncthreads();
-      load(vb, m + 3 * STEP);
-      compute(1);
-      put(va, 0);
-      __syncthreads();
+      step(vb, va, 0, m);
+      step(va, vb, 1, m + STEP);
     }
+    __syncthreads();
   }
   // A lane holds one column k of 16 rows n of each 32 x 32 tile: an instruction stores 32 adjacent columns of two rows. Offsets
   // inside the tile fit 32 bits (K < 2^22).
@@ -229,6 +243,14 @@ wgrad8_kernel(Job o) {
   for (int i = 0; i < STEP; ++i) t += s_b[i * COLS + threadIdx.x];
   if (part) part[o.N * o.K + n0 + threadIdx.x] = t;
   else store_param(o.db, o.otype, n0 + threadIdx.x, t);
+}
+
+template <int FMT, typename G, int T>
+__global__ void __launch_bounds__(WG, T == 4 ? 1 : 2)
+wgrad8_kernel(Job o) {
+  extern __shared__ __align__(16) unsigned short s_mem[];      // two buffers: the planes of g, one of x
+  if ((int64_t)(blockIdx.x % (o.tiles_n * o.tiles_k) / o.tiles_k + 1) * 64 * T <= o.N) wgrad8_tile<FMT, G, T, true>(o, s_mem);
+  else wgrad8_tile<FMT, G, T, false>(o, s_mem);
 }
 
 // The ranges' partial sums, added in a fixed order: a workgroup takes 64 adjacent results, its four waves a quarter of the ranges each.
