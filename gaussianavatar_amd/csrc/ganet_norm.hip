@@ -25,40 +25,52 @@ constexpr int ACT_NONE = 0, ACT_RELU = 2;      // (1: softplus)
 constexpr int LN_WG = 256;
 
 // softplus = max(u, 0) + log1p(exp(-|u|)): relative accuracy on both sides (torch's threshold of 20 differs by 2e-9 of the value).
-// log1p by the series where exp(-|u|) is small: the hardware logarithm of 1 + e keeps 1e-7 absolute only.
+// log1p by its series where exp(-|u|) < 1/32, where it leaves out e^4 / 5 = 2e-7: the hardware logarithm of 1 + e is good to 1e-7
+// absolute only. A NaN goes through exp and log.
 __device__ __forceinline__ float act_fwd(float u, int act) {
   if (act == ACT_NONE) return u;
   if (act == ACT_RELU) return u > 0.f || u != u ? u : 0.f;
   const float e = __expf(-fabsf(u));
-  const float l = e < 0.0625f ? e * (1.f - e * (0.5f - e * (0.333333333f - e * (0.25f - e * 0.2f)))) : __logf(1.f + e);
-  return fmaxf(u, 0.f) + l + (u != u ? u : 0.f);
+  const float l = e < 0.03125f ? e * fmaf(e, fmaf(e, fmaf(e, -0.25f, 0.333333333f), -0.5f), 1.f) : __logf(1.f + e);
+  return fmaxf(u, 0.f) + l;
 }
+// sigmoid(u) = 1 / (1 + exp(-u)); exp(-u) = infinity gives 0. The hardware reciprocal: 1 ulp.
 __device__ __forceinline__ float act_grad(float u, int act) {
   if (act == ACT_NONE) return 1.f;
   if (act == ACT_RELU) return u > 0.f ? 1.f : (u != u ? u : 0.f);
-  const float e = __expf(-fabsf(u));
-  const float r = 1.f / (1.f + e);
-  return u > 0.f ? r : (u != u ? u : e * r);
+  return __builtin_amdgcn_rcpf(1.f + __expf(-u));
 }
 
 template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
 
-// Sum over the lanes that hold a row; every lane gets it. WIDE: over the workgroup, through LDS (two buffers in turn: a
-// buffer is written again only after a barrier that every reader of its last content has passed).
+// Sum over 2^k <= 64 adjacent lanes; every lane gets it. Up to 16 lanes by register permutations: once all lanes of a group of 4
+// (8) hold their sum, the mirrored lane of the 8 (16) holds the other group's.
+template <int CTRL>
+__device__ __forceinline__ float permuted(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int N>
+__device__ __forceinline__ void lane_sum(float (&v)[N], int lanes) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (lanes > 1) v[i] += permuted<0xB1>(v[i]);       // quad_perm [1,0,3,2]
+    if (lanes > 2) v[i] += permuted<0x4E>(v[i]);       // quad_perm [2,3,0,1]
+    if (lanes > 4) v[i] += permuted<0x141>(v[i]);      // row_half_mirror
+    if (lanes > 8) v[i] += permuted<0x140>(v[i]);      // row_mirror
+    if (lanes > 16) v[i] += __shfl_xor(v[i], 16);
+    if (lanes > 32) v[i] += __shfl_xor(v[i], 32);
+  }
+}
+
+// Sum over the lanes that hold a row. WIDE: over the workgroup, through LDS (two buffers in turn: a buffer is written again only
+// after a barrier that every reader of its last content has passed).
 template <bool WIDE, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], int G, float* s_red, int& phase) {
   if (!WIDE) {
-    for (int off = 1; off < G; off <<= 1) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off);
-    }
+    lane_sum(v, G);
     return;
   }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off);
-  }
+  lane_sum(v, 64);
   const int nw = blockDim.x >> 6, wave = threadIdx.x >> 6;
   float* s = s_red + phase * 2 * 16;
   if ((threadIdx.x & 63) == 0) {
@@ -75,9 +87,23 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int G, float* s_red, int&
   phase ^= 1;
 }
 
+// A vector of a row as it was loaded: elements past the row's end, and all of a row that does not exist, are zero.
+template <typename T>
+struct Vec { T e[VEC<T>]; };
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* __restrict__ p, int n) {
+  Vec<T> v;
+  if (n >= VEC<T>) __builtin_memcpy(&v, p, sizeof(v));
+  else {
+#pragma unroll
+    for (int i = 0; i < VEC<T>; ++i) v.e[i] = i < n ? p[i] : (T)0.f;
+  }
+  return v;
+}
+
 template <typename T, int NC, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS)
-ln_fwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
+ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
               const void* __restrict__ b, int32_t wtype, float eps, int act, T* __restrict__ y, float* __restrict__ mean_out,
               float* __restrict__ rstd_out, uint8_t* __restrict__ codes, int64_t ldc, float code_scale) {
   constexpr int V = VEC<T>;
@@ -86,43 +112,58 @@ ln_fwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx,
   const int l = WIDE ? threadIdx.x : (threadIdx.x & (G - 1));
   const int groups = WIDE ? 1 : THREADS / G, grp = WIDE ? 0 : threadIdx.x / G;
   const float inv = 1.0f / (float)C;
+  const bool full = C % V == 0;              // no vector ends past the row
   float wv[NC][V], bv[NC][V];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int64_t c = (int64_t)(j * G + l) * V + i;
+      const int c = (j * G + l) * V + i;
       wv[j][i] = (w && c < C) ? load_param(w, wtype, c) : 1.f;
       bv[j][i] = (b && c < C) ? load_param(b, wtype, c) : 0.f;
     }
   }
-  // every lane of a wave takes the same number of turns: the shuffles need whole groups, a turn without a row reads nothing
-  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < M; r0 += (int64_t)gridDim.x * groups) {
-    const int64_t row = r0 + grp;
+  // every lane of a wave takes the same number of turns: the sums need whole groups, a turn without a row reads nothing. The next
+  // turn's row is loaded before this one's sums.
+  const int64_t turn = (int64_t)gridDim.x * groups;
+  int64_t row = (int64_t)blockIdx.x * groups + grp;
+  const int64_t turns = (M - (int64_t)blockIdx.x * groups + turn - 1) / turn;
+  Vec<T> next[NC];
+  auto fetch = [&](int64_t r) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = (j * G + l) * V;
+      next[j] = load_vec(x + r * ldx + c, r < M ? C - c : 0);
+    }
+  };
+  fetch(row);
+  for (int64_t t = 0; t < turns; ++t, row += turn) {
     const bool live = row < M;
     float v[NC][V];
     float s[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int64_t c = (int64_t)(j * G + l) * V;
-      load_n(x + row * ldx + c, live ? C - c : 0, v[j]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[0] += v[j][i];
+      for (int i = 0; i < V; ++i) { v[j][i] = (float)next[j].e[i]; s[0] += v[j][i]; }
     }
+    if (t + 1 < turns) fetch(row + turn);
     row_sum<WIDE>(s, G, s_red, phase);
     const float mean = s[0] * inv;
     s[0] = 0.f;
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int64_t c = (int64_t)(j * G + l) * V;
+      const int left = C - (j * G + l) * V;
+      if (full) {
+        const float m = left > 0 ? mean : 0.f;             // (a vector past the row is zero: it stays so)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[j][i] = c + i < C ? v[j][i] - mean : 0.f;
-        s[0] = fmaf(v[j][i], v[j][i], s[0]);
+        for (int i = 0; i < V; ++i) { v[j][i] -= m; s[0] = fmaf(v[j][i], v[j][i], s[0]); }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) { v[j][i] = i < left ? v[j][i] - mean : 0.f; s[0] = fmaf(v[j][i], v[j][i], s[0]); }
       }
     }
     row_sum<WIDE>(s, G, s_red, phase);
-    const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+    const float rstd = rsqrtf(fmaf(s[0], inv, eps));
     if (live && l == 0) {
       if (mean_out) mean_out[row] = mean;
       if (rstd_out) rstd_out[row] = rstd;
@@ -130,7 +171,7 @@ ln_fwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx,
     if (!live) continue;
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int64_t c = (int64_t)(j * G + l) * V;
+      const int c = (j * G + l) * V;
       if (c >= C) continue;
 #pragma unroll
       for (int i = 0; i < V; ++i) v[j][i] *= rstd;
@@ -143,7 +184,11 @@ ln_fwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx,
                                 v[j][4 * q + 3] * code_scale);
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[j][i] = act_fwd(fmaf(v[j][i], wv[j][i], bv[j][i]), act);
+      for (int i = 0; i < V; ++i) v[j][i] = fmaf(v[j][i], wv[j][i], bv[j][i]);
+      if (act != ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = act_fwd(v[j][i], act);
+      }
       store_n(y + row * C + c, C - c, v[j]);
     }
   }
@@ -181,7 +226,7 @@ ln_fwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx,
       }
     }
     row_sum<true>(s, 0, s_red, phase);
-    const float rstd = 1.0f / sqrtf((float)(s[0] * inv) + eps);
+    const float rstd = rsqrtf((float)(s[0] * inv) + eps);
     if (threadIdx.x == 0) {
       if (mean_out) mean_out[row] = mean;
       if (rstd_out) rstd_out[row] = rstd;
@@ -208,30 +253,37 @@ ln_fwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx,
   }
 }
 
-// xh of one vector: from x, or from its codes. Columns beyond C read as zero.
+// What the backward pass loads of a vector, and xh from it. Columns past the row give -mean rstd or zero: their gradient is zero.
 template <typename T, bool KEPT8>
-__device__ __forceinline__ void load_xh(const T* xr, const uint8_t* cr, int64_t c, int64_t C, bool live, float mean, float rstd,
-                                        float code_unit, float (&xh)[VEC<T>]) {
-  constexpr int V = VEC<T>;
-  if (KEPT8) {
-    const bool in = live && c < C;
+struct Kept {
+  Vec<T> x;
+  unsigned c[VEC<T> / 4];
+  __device__ __forceinline__ void load(const T* xr, const uint8_t* cr, int c0, int n) {
+    if (KEPT8) {
 #pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      float t[4];
-      unpack4<GANET_E4M3>(in ? reinterpret_cast<const unsigned*>(cr + c)[q] : 0u, t);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xh[4 * q + i] = c + 4 * q + i < C ? t[i] * code_unit : 0.f;
-    }
-  } else {
-    load_n(xr + c, live ? C - c : 0, xh);
-#pragma unroll
-    for (int i = 0; i < V; ++i) xh[i] = (live && c + i < C) ? (xh[i] - mean) * rstd : 0.f;
+      for (int q = 0; q < VEC<T> / 4; ++q) c[q] = 0u;
+      if (n > 0) __builtin_memcpy(c, __builtin_assume_aligned(cr + c0, VEC<T>), VEC<T>);
+    } else x = load_vec(xr + c0, n);
   }
-}
+  __device__ __forceinline__ void values(float mean, float rstd, float code_unit, float (&xh)[VEC<T>]) const {
+    if (KEPT8) {
+#pragma unroll
+      for (int q = 0; q < VEC<T> / 4; ++q) {
+        float t[4];
+        unpack4<GANET_E4M3>(c[q], t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xh[4 * q + i] = t[i] * code_unit;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC<T>; ++i) xh[i] = ((float)x.e[i] - mean) * rstd;
+    }
+  }
+};
 
 template <typename T, int NC, bool WIDE, int THREADS, bool KEPT8>
 __global__ void __launch_bounds__(THREADS)
-ln_bwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx, const float* __restrict__ mean_in,
+ln_bwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, const float* __restrict__ mean_in,
               const uint8_t* __restrict__ codes, int64_t ldc, float code_unit, const float* __restrict__ rstd_in,
               const void* __restrict__ w, const void* __restrict__ b, int32_t wtype, int act, const T* __restrict__ dy,
               int64_t lddy, T* __restrict__ dx, float* __restrict__ part) {
@@ -247,48 +299,66 @@ ln_bwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx,
   for (int j = 0; j < NC; ++j) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int64_t c = (int64_t)(j * G + l) * V + i;
+      const int c = (j * G + l) * V + i;
       wv[j][i] = (w && c < C) ? load_param(w, wtype, c) : 1.f;
       bv[j][i] = (b && c < C) ? load_param(b, wtype, c) : 0.f;
       aw[j][i] = 0.f;
       ab[j][i] = 0.f;
     }
   }
-  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < M; r0 += (int64_t)gridDim.x * groups) {
-    const int64_t row = r0 + grp;
-    const bool live = row < M;
-    const float mean = (!KEPT8 && live) ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
+  const int64_t turn = (int64_t)gridDim.x * groups;
+  int64_t row = (int64_t)blockIdx.x * groups + grp;
+  const int64_t turns = (M - (int64_t)blockIdx.x * groups + turn - 1) / turn;
+  Vec<T> gn[NC];
+  Kept<T, KEPT8> xn[NC];
+  float mean_n = 0.f, rstd_n = 0.f;
+  auto fetch = [&](int64_t r) {                // (a row that does not exist: zeros, and rstd = 0)
+    const bool live = r < M;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = (j * G + l) * V, n = live ? C - c : 0;
+      gn[j] = load_vec(dy + r * lddy + c, n);
+      xn[j].load(x + r * ldx, codes + r * ldc, c, n);
+    }
+    if (!KEPT8) mean_n = live ? mean_in[r] : 0.f;
+    rstd_n = live ? rstd_in[r] : 0.f;
+  };
+  fetch(row);
+  for (int64_t t = 0; t < turns; ++t, row += turn) {
+    const float mean = mean_n, rstd = rstd_n;
     float xh[NC][V], g[NC][V];
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int64_t c = (int64_t)(j * G + l) * V;
-      load_n(dy + row * lddy + c, live ? C - c : 0, g[j]);
-      load_xh<T, KEPT8>(x + row * ldx, codes + row * ldc, c, C, live, mean, rstd, code_unit, xh[j]);
+      xn[j].values(mean, rstd, code_unit, xh[j]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) g[j][i] = (float)gn[j].e[i];
     }
+    if (t + 1 < turns) fetch(row + turn);
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
+      if (act != ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[j][i] *= act_grad(fmaf(xh[j][i], wv[j][i], bv[j][i]), act);
+      }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        if (act != ACT_NONE) g[j][i] *= act_grad(fmaf(xh[j][i], wv[j][i], bv[j][i]), act);
-        if (live) {
-          aw[j][i] = fmaf(g[j][i], xh[j][i], aw[j][i]);
-          ab[j][i] += g[j][i];
-        }
+        aw[j][i] = fmaf(g[j][i], xh[j][i], aw[j][i]);
+        ab[j][i] += g[j][i];
         g[j][i] *= wv[j][i];
         s[0] += g[j][i];
         s[1] = fmaf(g[j][i], xh[j][i], s[1]);
       }
     }
     row_sum<WIDE>(s, G, s_red, phase);
-    if (dx && live) {
+    if (dx && row < M) {
       const float m1 = s[0] * inv, m2 = s[1] * inv;
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        const int64_t c = (int64_t)(j * G + l) * V;
+        const int c = (j * G + l) * V;
         if (c >= C) continue;
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[j][i] = rstd * (g[j][i] - m1 - xh[j][i] * m2);
+        for (int i = 0; i < V; ++i) g[j][i] = rstd * (g[j][i] - fmaf(xh[j][i], m2, m1));
         store_n(dx + row * C + c, C - c, g[j]);
       }
     }
@@ -298,13 +368,13 @@ ln_bwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx,
   if (WIDE) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int64_t c = (int64_t)(j * G + l) * V;
+      const int c = (j * G + l) * V;
       store_n(out + c, C - c, aw[j]);
       store_n(out + C + c, C - c, ab[j]);
     }
     return;
   }
-  // groups of a wave by shuffles, then the waves through LDS (one row pair each)
+  // groups of a wave by shuffles, then the waves through LDS (dw, then db, through the same)
   for (int off = G; off < 64; off <<= 1) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
@@ -317,7 +387,7 @@ ln_bwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx,
   }
   const int wave = threadIdx.x >> 6, cols = G * NC * V;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {                // dw, then db, through the same LDS
+  for (int k = 0; k < 2; ++k) {
     if (k) __syncthreads();
     if ((threadIdx.x & 63) < G) {
 #pragma unroll
@@ -327,7 +397,7 @@ ln_bwd_kernel(int64_t M, int64_t C, int G, const T* __restrict__ x, int64_t ldx,
       }
     }
     __syncthreads();
-    for (int64_t c = threadIdx.x; c < C; c += THREADS) {
+    for (int c = threadIdx.x; c < C; c += THREADS) {
       float t = 0.f;
 #pragma unroll
       for (int v = 0; v < THREADS / 64; ++v) t += s_mem[v * cols + c];
@@ -355,7 +425,9 @@ ln_bwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx,
       for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
         float g[V], xh[V];
         load_n(dy + row * lddy + c, C - c, g);
-        load_xh<T, KEPT8>(x + row * ldx, codes + row * ldc, c, C, true, mean, rstd, code_unit, xh);
+        Kept<T, KEPT8> kept;
+        kept.load(x + row * ldx, codes + row * ldc, (int)c, (int)(C - c));
+        kept.values(mean, rstd, code_unit, xh);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float wi = (w && c + i < C) ? load_param(w, wtype, c + i) : 1.f;
@@ -390,7 +462,9 @@ ln_bwd_columns_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx
   for (int64_t row = blockIdx.y; row < M; row += gridDim.y) {
     float g[V], xh[V];
     load_n(dy + row * lddy + c, C - c, g);
-    load_xh<T, KEPT8>(x + row * ldx, codes + row * ldc, c, C, true, KEPT8 ? 0.f : mean_in[row], rstd_in[row], code_unit, xh);
+    Kept<T, KEPT8> kept;
+    kept.load(x + row * ldx, codes + row * ldc, (int)c, (int)(C - c));
+    kept.values(KEPT8 ? 0.f : mean_in[row], rstd_in[row], code_unit, xh);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       if (act != ACT_NONE && c + i < C)
@@ -404,22 +478,24 @@ ln_bwd_columns_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx
   store_n(out + C + c, C - c, ab);
 }
 
-// dw / db: the workgroups' partial rows, added in order: 16 slices of the partial rows by 16 columns
-__global__ void __launch_bounds__(256)
+// dw / db: the workgroups' partial rows, added in a fixed order: a workgroup takes 16 adjacent columns, 64 slices of the rows
+__global__ void __launch_bounds__(1024)
 ln_bwd_final_kernel(int64_t C, int parts, const float* __restrict__ part, void* __restrict__ dw, void* __restrict__ db,
                     int32_t wtype) {
-  __shared__ float s[16][17];
+  __shared__ float s[64][17];
   const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4;
   const int64_t c = (int64_t)blockIdx.x * 16 + cl;
   float t = 0.f;
-  if (c < 2 * C)
-    for (int p = sl; p < parts; p += 16) t += part[(int64_t)p * 2 * C + c];
+  if (c < 2 * C) {
+#pragma unroll 8
+    for (int p = sl; p < parts; p += 64) t += part[(int64_t)p * 2 * C + c];
+  }
   s[sl][cl] = t;
   __syncthreads();
   if (sl == 0 && c < 2 * C) {
     t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) t += s[k][cl];
+    for (int k = 0; k < 64; ++k) t += s[k][cl];
     if (c < C) { if (dw) store_param(dw, wtype, c, t); }
     else if (db) store_param(db, wtype, c - C, t);
   }
@@ -493,7 +569,7 @@ int ganet_ln_fwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
   const dim3 grid((unsigned)(s.form == 2 ? (M < FWD_BLOCKS ? M : FWD_BLOCKS) : fwd_grid(s, M)));
   uint8_t* cd = static_cast<uint8_t*>(codes);
 #define LN_FWD(NC, WIDE, TH)                                                                                            \
-  hipLaunchKernelGGL((ln_fwd_kernel<T, NC, WIDE, TH>), grid, dim3(TH), 0, stream, M, C, s.G, static_cast<const T*>(x), ldx, w, b, \
+  hipLaunchKernelGGL((ln_fwd_kernel<T, NC, WIDE, TH>), grid, dim3(TH), 0, stream, M, (int)C, s.G, static_cast<const T*>(x), ldx, w, b, \
                      wtype, eps, act, static_cast<T*>(y), mean, rstd, cd, ldc, cs)
   GANET_BY_TYPE(type, T, {
     if (s.form == 2)
@@ -541,7 +617,7 @@ int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
   const int64_t parts = M ? bwd_grid(s, M) : 0;
 #define LN_BWD(NC, WIDE, TH, K8)                                                                                              \
   hipLaunchKernelGGL((ln_bwd_kernel<T, NC, WIDE, TH, K8>), dim3((unsigned)parts), dim3(TH),                                        \
-                     WIDE ? 0 : (size_t)(TH / 64) * s.G * NC * VEC<T> * sizeof(float), stream, M, C, s.G,                 \
+                     WIDE ? 0 : (size_t)(TH / 64) * s.G * NC * VEC<T> * sizeof(float), stream, M, (int)C, s.G,                 \
                      static_cast<const T*>(x), ldx, mean, cd, ldc, cu, rstd, w, b, wtype, act, static_cast<const T*>(dy), lddy, \
                      static_cast<T*>(dx), part)
 #define LN_BWD_FORMS(K8)                                                                                                      \
@@ -574,7 +650,7 @@ int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
 #undef LN_BWD_FORMS
 #undef LN_BWD
   if (sums)       // (also for M = 0: the gradients of no rows are zero)
-    hipLaunchKernelGGL(ln_bwd_final_kernel, dim3((unsigned)cdiv(2 * C, 16)), dim3(256), 0, stream, C, (int)parts, part, dw, db, wtype);
+    hipLaunchKernelGGL(ln_bwd_final_kernel, dim3((unsigned)cdiv(2 * C, 16)), dim3(1024), 0, stream, C, (int)parts, part, dw, db, wtype);
   return check_hip(hipGetLastError(), "ganet_ln_bwd");
 }
 

@@ -62,6 +62,8 @@ struct Job {
   void* dW; void* db; int32_t otype; float* part; int splits; int64_t rows; int tiles_n, tiles_k;
 };
 
+struct Where { int tn, tk, split; };
+
 // A workgroup of four waves computes 64 T x 64 T of dW over its range of rows, a wave 32 T x 32 T. A step is 32 rows: thread t brings row
 // t / 8, 8 T columns of g and of x, from global memory into registers two steps ahead, and as bf16 into one of two LDS buffers one
 // step ahead. A step is multiplied in 2 P parts (16 rows, one piece of g); the fragments of the next part are read before a
@@ -69,13 +71,12 @@ struct Job {
 // memory nor LDS latency stands between two multiplications.
 // INSIDE: the tile ends before column N of g (vectors of 8; else element by element).
 template <int FMT, typename G, int T, bool INSIDE>
-__device__ __forceinline__ void wgrad8_tile(const Job& o, unsigned short* s_mem) {
+__device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsigned short* s_mem) {
   constexpr int P = PIECES<G>, COLS = 64 * T, PITCH = pitch(COLS), PLANE = STEP * PITCH, BUF = (P + 1) * PLANE;
   constexpr int GV = 8, GC = COLS / 64;                        // g: GC vectors of 8 elements, 64 columns apart
   constexpr int XC = COLS / 128;                               // x: XC vectors of 16 codes, one per 128 columns
-  const int tiles = o.tiles_n * o.tiles_k;
-  const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
-  const int64_t n0 = (int64_t)(tile / o.tiles_k) * COLS, k0 = (int64_t)(tile % o.tiles_k) * COLS;
+  const int64_t n0 = (int64_t)w.tn * COLS, k0 = (int64_t)w.tk * COLS;
+  const int split = w.split;
   const int64_t m_lo = split * o.rows, m_hi = min(m_lo + o.rows, o.M);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wn = (wave & 1) * 32 * T, wk = (wave >> 1) * 32 * T;
@@ -249,8 +250,14 @@ template <int FMT, typename G, int T>
 __global__ void __launch_bounds__(WG, T == 4 ? 1 : 2)
 wgrad8_kernel(Job o) {
   extern __shared__ __align__(16) unsigned short s_mem[];      // two buffers: the planes of g, one of x
-  if ((int64_t)(blockIdx.x % (o.tiles_n * o.tiles_k) / o.tiles_k + 1) * 64 * T <= o.N) wgrad8_tile<FMT, G, T, true>(o, s_mem);
-  else wgrad8_tile<FMT, G, T, false>(o, s_mem);
+  // Workgroups go round the 8 XCDs in turn: give each XCD one run of tiles, walked 4 tiles of n before the next tile of k, so that its 32
+  // CUs read 4 strips of g and 8 of x through their L2 (where workgroup i takes tile i: 16 strips of g and 2 of x).
+  const int tiles = o.tiles_n * o.tiles_k, T0 = tiles * o.splits, q = T0 / 8, rem = T0 % 8, xcd = blockIdx.x % 8;
+  const int t = xcd * q + (xcd < rem ? xcd : rem) + blockIdx.x / 8, in_split = t % tiles;
+  const int group = in_split / (4 * o.tiles_k), gn = min(4, o.tiles_n - group * 4), in = in_split - group * 4 * o.tiles_k;
+  const Where w{group * 4 + in % gn, in / gn, t / tiles};
+  if ((int64_t)(w.tn + 1) * 64 * T <= o.N) wgrad8_tile<FMT, G, T, true>(o, w, s_mem);
+  else wgrad8_tile<FMT, G, T, false>(o, w, s_mem);
 }
 
 // The ranges' partial sums, added in a fixed order: a workgroup takes 64 adjacent results, its four waves a quarter of the ranges each.
@@ -305,7 +312,7 @@ int launch_tile(const Job& o, hipStream_t stream) {
     ready = true;
   }
   const int64_t grid = (int64_t)o.tiles_n * o.tiles_k * o.splits;
-  if (grid >= (1ll << 31)) { set_error("ganet_wgrad8: too many tiles"); return 4; }
+  if (grid >= (1ll << 30)) { set_error("ganet_wgrad8: too many tiles"); return 4; }
   hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(WG), lds, stream, o);
   return check_hip(hipGetLastError(), "ganet_wgrad8");
 }
