@@ -116,12 +116,9 @@ ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
   float wv[NC][V], bv[NC][V];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (j * G + l) * V + i;
-      wv[j][i] = (w && c < C) ? load_param(w, wtype, c) : 1.f;
-      bv[j][i] = (b && c < C) ? load_param(b, wtype, c) : 0.f;
-    }
+    const int c = (j * G + l) * V;
+    load_params(w, wtype, c, C - c, 1.f, wv[j]);
+    load_params(b, wtype, c, C - c, 0.f, bv[j]);
   }
   // every lane of a wave takes the same number of turns: the sums need whole groups, a turn without a row reads nothing. The next
   // turn's row is loaded before this one's sums.
@@ -294,17 +291,19 @@ ln_bwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
   const int l = WIDE ? threadIdx.x : (threadIdx.x & (G - 1));
   const int groups = WIDE ? 1 : THREADS / G, grp = WIDE ? 0 : threadIdx.x / G;
   const float inv = 1.0f / (float)C;
+  // 1024 threads have 128 registers each: the parameters are read again (from cache) with every row
+  constexpr bool HOLD = THREADS < 1024;
   float wv[NC][V], bv[NC][V], aw[NC][V], ab[NC][V];
+  auto params = [&](int j) {
+    const int c = (j * G + l) * V;
+    load_params(w, wtype, c, C - c, 1.f, wv[j]);
+    if (act != ACT_NONE) load_params(b, wtype, c, C - c, 0.f, bv[j]);
+  };
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
+    if (HOLD) params(j);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (j * G + l) * V + i;
-      wv[j][i] = (w && c < C) ? load_param(w, wtype, c) : 1.f;
-      bv[j][i] = (b && c < C) ? load_param(b, wtype, c) : 0.f;
-      aw[j][i] = 0.f;
-      ab[j][i] = 0.f;
-    }
+    for (int i = 0; i < V; ++i) aw[j][i] = ab[j][i] = 0.f;
   }
   const int64_t turn = (int64_t)gridDim.x * groups;
   int64_t row = (int64_t)blockIdx.x * groups + grp;
@@ -337,6 +336,7 @@ ln_bwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
     if (t + 1 < turns) fetch(row + turn);
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
+      if (!HOLD) params(j);
       if (act != ACT_NONE) {
 #pragma unroll
         for (int i = 0; i < V; ++i) g[j][i] *= act_grad(fmaf(xh[j][i], wv[j][i], bv[j][i]), act);
@@ -521,17 +521,19 @@ Shape make_shape(int64_t C, int32_t type) {
   return s;
 }
 
-constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024, STREAM_SLICES = 64;
-int64_t fwd_grid(const Shape& s, int64_t M) {
-  const int64_t rows = s.form ? 1 : s.threads / s.G;
-  const int64_t g = cdiv(M, rows);
-  return g < FWD_BLOCKS ? g : FWD_BLOCKS;
+// Workgroups that are resident at a time (256 CUs; by the kernels' registers): one round of them strides over the rows, so that none is left to
+// run on its own at the end, in equal numbers of turns. (2,048 workgroups where 1,792 fit cost 25 % at 262,144 x 128 fp32.)
+constexpr int CUS = 256, STREAM_SLICES = 64;
+int64_t even_grid(int64_t turns, int64_t resident) { return turns <= resident ? turns : cdiv(turns, cdiv(turns, resident)); }
+int64_t fwd_grid(const Shape& s, int32_t type, int64_t M) {
+  if (s.form == 2) return M < 2 * CUS ? M : 2 * CUS;
+  const int per_cu = s.threads == 1024 ? 1 : s.threads == 512 ? 2 : type == GANET_F32 ? 6 : 4;
+  return even_grid(cdiv(M, s.form ? 1 : s.threads / s.G), (int64_t)CUS * per_cu);
 }
-int64_t bwd_grid(const Shape& s, int64_t M) {
+int64_t bwd_grid(const Shape& s, int32_t type, int64_t M) {
   if (s.form == 2) return M < STREAM_SLICES ? M : STREAM_SLICES;
-  const int64_t rows = s.form ? 1 : s.threads / s.G;
-  const int64_t g = cdiv(M, rows);
-  return g < BWD_BLOCKS ? g : BWD_BLOCKS;
+  const int per_cu = s.threads >= 512 ? (type == GANET_F32 && s.threads == 512 ? 2 : 1) : type == GANET_F32 ? (s.NC > 2 ? 2 : 4) : s.NC > 2 ? 1 : s.form ? 3 : 2;
+  return even_grid(cdiv(M, s.form ? 1 : s.threads / s.G), (int64_t)CUS * per_cu);
 }
 
 bool ln_ok(int64_t M, int64_t C, int32_t type, int32_t wtype, int32_t act) {
@@ -566,7 +568,7 @@ int ganet_ln_fwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   const Shape s = make_shape(C, type);
   const float cs = std::ldexp(1.0f, -ganet_ln_code_exponent(C));
-  const dim3 grid((unsigned)(s.form == 2 ? (M < FWD_BLOCKS ? M : FWD_BLOCKS) : fwd_grid(s, M)));
+  const dim3 grid((unsigned)fwd_grid(s, type, M));
   uint8_t* cd = static_cast<uint8_t*>(codes);
 #define LN_FWD(NC, WIDE, TH)                                                                                            \
   hipLaunchKernelGGL((ln_fwd_kernel<T, NC, WIDE, TH>), grid, dim3(TH), 0, stream, M, (int)C, s.G, static_cast<const T*>(x), ldx, w, b, \
@@ -591,7 +593,7 @@ int ganet_ln_fwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
 
 size_t ganet_ln_bwd_workspace(int64_t M, int64_t C, int32_t type) {
   if (!rows_ok(M, C) || !type_ok(type)) return 0;
-  return (size_t)bwd_grid(make_shape(C, type), M < 1 ? 1 : M) * 2 * (size_t)C * sizeof(float);
+  return (size_t)bwd_grid(make_shape(C, type), type, M < 1 ? 1 : M) * 2 * (size_t)C * sizeof(float);
 }
 
 int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* x, int64_t ldx, const float* mean,
@@ -614,7 +616,7 @@ int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
   const float cu = std::ldexp(1.0f, ganet_ln_code_exponent(C));
   float* part = sums ? static_cast<float*>(workspace) : nullptr;
   const uint8_t* cd = static_cast<const uint8_t*>(codes);
-  const int64_t parts = M ? bwd_grid(s, M) : 0;
+  const int64_t parts = M ? bwd_grid(s, type, M) : 0;
 #define LN_BWD(NC, WIDE, TH, K8)                                                                                              \
   hipLaunchKernelGGL((ln_bwd_kernel<T, NC, WIDE, TH, K8>), dim3((unsigned)parts), dim3(TH),                                        \
                      WIDE ? 0 : (size_t)(TH / 64) * s.G * NC * VEC<T> * sizeof(float), stream, M, (int)C, s.G,                 \
@@ -624,7 +626,7 @@ int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
   do {                                                                                                                        \
     if (s.form == 2) {                                                                                                        \
       if (dx)                                                                                                                 \
-        hipLaunchKernelGGL((ln_bwd_stream_kernel<T, K8>), dim3((unsigned)(M < BWD_BLOCKS ? M : BWD_BLOCKS)), dim3(1024), 0, stream, \
+        hipLaunchKernelGGL((ln_bwd_stream_kernel<T, K8>), dim3((unsigned)(M < 2 * CUS ? M : 2 * CUS)), dim3(1024), 0, stream, \
                            M, C, static_cast<const T*>(x), ldx, mean, cd, ldc, cu, rstd, w, b, wtype, act,                     \
                            static_cast<const T*>(dy), lddy, static_cast<T*>(dx));                                             \
       if (part)                                                                                                               \

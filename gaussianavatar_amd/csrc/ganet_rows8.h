@@ -62,6 +62,23 @@ __device__ __forceinline__ void store_param(void* p, int32_t type, int64_t i, fl
   else static_cast<_Float16*>(p)[i] = (_Float16)v;
 }
 
+// N consecutive parameters from element c on, `fill` where there are none (no tensor, or past its n elements)
+template <int N>
+__device__ __forceinline__ void load_params(const void* p, int32_t type, int c, int n, float fill, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = fill;
+  if (!p || n <= 0) return;
+  if (n >= N) {
+    if (type == GANET_F32) load_n(static_cast<const float*>(p) + c, n, v);
+    else if (type == GANET_BF16) load_n(static_cast<const __bf16*>(p) + c, n, v);
+    else load_n(static_cast<const _Float16*>(p) + c, n, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) v[i] = load_param(p, type, c + i);
+  }
+}
+
 // four values -> four codes, round to nearest, ties to even
 template <int FMT>
 __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
