@@ -21,24 +21,45 @@ using namespace rows8;
 
 namespace {
 
-constexpr int ACT_NONE = 0, ACT_RELU = 2;      // (1: softplus)
+constexpr int ACT_NONE = 0, ACT_SOFTPLUS = 1, ACT_RELU = 2;
 constexpr int LN_WG = 256;
 
 // softplus = max(u, 0) + log1p(exp(-|u|)): relative accuracy on both sides (torch's threshold of 20 differs by 2e-9 of the value).
 // log1p by its series where exp(-|u|) < 1/32, where it leaves out e^4 / 5 = 2e-7: the hardware logarithm of 1 + e is good to 1e-7
-// absolute only. A NaN goes through exp and log.
-__device__ __forceinline__ float act_fwd(float u, int act) {
-  if (act == ACT_NONE) return u;
-  if (act == ACT_RELU) return u > 0.f || u != u ? u : 0.f;
-  const float e = __expf(-fabsf(u));
-  const float l = e < 0.03125f ? e * fmaf(e, fmaf(e, fmaf(e, -0.25f, 0.333333333f), -0.5f), 1.f) : __logf(1.f + e);
-  return fmaxf(u, 0.f) + l;
+// absolute only. Both are computed and one is taken (a branch per element costs more); a NaN goes through exp and log.
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+__device__ __forceinline__ float softplus(float u) {
+  const float e = __builtin_amdgcn_exp2f(-LOG2E * fabsf(u));
+  const float series = e * fmaf(e, fmaf(e, fmaf(e, -0.25f, 0.333333333f), -0.5f), 1.f);
+  const float log = LN2 * __builtin_amdgcn_logf(1.f + e);
+  return fmaxf(u, 0.f) + (e < 0.03125f ? series : log);
 }
 // sigmoid(u) = 1 / (1 + exp(-u)); exp(-u) = infinity gives 0. The hardware reciprocal: 1 ulp.
-__device__ __forceinline__ float act_grad(float u, int act) {
-  if (act == ACT_NONE) return 1.f;
-  if (act == ACT_RELU) return u > 0.f ? 1.f : (u != u ? u : 0.f);
-  return __builtin_amdgcn_rcpf(1.f + __expf(-u));
+__device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * u)); }
+
+// act of N values, and g times its derivative (the kind is uniform: one branch per vector)
+template <int N>
+__device__ __forceinline__ void act_fwd(float (&v)[N], int act) {
+  if (act == ACT_SOFTPLUS) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = softplus(v[i]);
+  } else if (act == ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];
+  }
+}
+template <int N>
+__device__ __forceinline__ void act_bwd(float (&g)[N], const float (&xh)[N], const float (&w)[N], const float (&b)[N], int act) {
+  if (act == ACT_SOFTPLUS) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] *= sigmoid(fmaf(xh[i], w[i], b[i]));
+  } else if (act == ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float u = fmaf(xh[i], w[i], b[i]);
+      g[i] = u > 0.f ? g[i] : (u != u ? u : 0.f);
+    }
+  }
 }
 
 template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
@@ -182,10 +203,7 @@ ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) v[j][i] = fmaf(v[j][i], wv[j][i], bv[j][i]);
-      if (act != ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[j][i] = act_fwd(v[j][i], act);
-      }
+      act_fwd(v[j], act);
       store_n(y + row * C + c, C - c, v[j]);
     }
   }
@@ -239,12 +257,12 @@ ln_fwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx,
           reinterpret_cast<unsigned*>(p)[q] = pack4<GANET_E4M3>(v[4 * q] * code_scale, v[4 * q + 1] * code_scale,
                                                                 v[4 * q + 2] * code_scale, v[4 * q + 3] * code_scale);
       }
+      float wv[V], bv[V];
+      load_params(w, wtype, (int)c, (int)(C - c), 1.f, wv);
+      load_params(b, wtype, (int)c, (int)(C - c), 0.f, bv);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float wi = (w && c + i < C) ? load_param(w, wtype, c + i) : 1.f;
-        const float bi = (b && c + i < C) ? load_param(b, wtype, c + i) : 0.f;
-        v[i] = act_fwd(fmaf(v[i], wi, bi), act);
-      }
+      for (int i = 0; i < V; ++i) v[i] = fmaf(v[i], wv[i], bv[i]);
+      act_fwd(v, act);
       store_n(y + row * C + c, C - c, v);
     }
   }
@@ -337,10 +355,7 @@ ln_bwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       if (!HOLD) params(j);
-      if (act != ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) g[j][i] *= act_grad(fmaf(xh[j][i], wv[j][i], bv[j][i]), act);
-      }
+      act_bwd(g[j], xh[j], wv[j], bv[j], act);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         aw[j][i] = fmaf(g[j][i], xh[j][i], aw[j][i]);
@@ -428,12 +443,13 @@ ln_bwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx,
         Kept<T, KEPT8> kept;
         kept.load(x + row * ldx, codes + row * ldc, (int)c, (int)(C - c));
         kept.values(mean, rstd, code_unit, xh);
+        float wv[V], bv[V];
+        load_params(w, wtype, (int)c, (int)(C - c), 1.f, wv);
+        load_params(b, wtype, (int)c, (int)(C - c), 0.f, bv);
+        act_bwd(g, xh, wv, bv, act);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float wi = (w && c + i < C) ? load_param(w, wtype, c + i) : 1.f;
-          const float bi = (b && c + i < C) ? load_param(b, wtype, c + i) : 0.f;
-          if (act != ACT_NONE) g[i] *= act_grad(fmaf(xh[i], wi, bi), act);
-          g[i] *= wi;
+          g[i] *= wv[i];
           s[0] += g[i];
           s[1] = fmaf(g[i], xh[i], s[1]);
           g[i] = rstd * (g[i] - m1 - xh[i] * m2);
@@ -458,17 +474,18 @@ ln_bwd_columns_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx
   constexpr int V = VEC<T>;
   const int64_t c = ((int64_t)blockIdx.x * LN_WG + threadIdx.x) * V;
   if (c >= C) return;
-  float aw[V] = {}, ab[V] = {};
+  float aw[V] = {}, ab[V] = {}, wv[V], bv[V];
+  load_params(w, wtype, (int)c, (int)(C - c), 1.f, wv);
+  load_params(b, wtype, (int)c, (int)(C - c), 0.f, bv);
   for (int64_t row = blockIdx.y; row < M; row += gridDim.y) {
     float g[V], xh[V];
     load_n(dy + row * lddy + c, C - c, g);
     Kept<T, KEPT8> kept;
     kept.load(x + row * ldx, codes + row * ldc, (int)c, (int)(C - c));
     kept.values(KEPT8 ? 0.f : mean_in[row], rstd_in[row], code_unit, xh);
+    act_bwd(g, xh, wv, bv, act);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (act != ACT_NONE && c + i < C)
-        g[i] *= act_grad(fmaf(xh[i], w ? load_param(w, wtype, c + i) : 1.f, b ? load_param(b, wtype, c + i) : 0.f), act);
       aw[i] = fmaf(g[i], xh[i], aw[i]);
       ab[i] += g[i];
     }
