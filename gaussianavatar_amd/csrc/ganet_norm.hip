@@ -538,19 +538,25 @@ Shape make_shape(int64_t C, int32_t type) {
   return s;
 }
 
-// Workgroups that are resident at a time (256 CUs; by the kernels' registers): one round of them strides over the rows, so that none is left to
-// run on its own at the end, in equal numbers of turns. (2,048 workgroups where 1,792 fit cost 25 % at 262,144 x 128 fp32.)
+// One round of workgroups strides over the rows: as many as are resident at a time (256 CUs; by the kernels' registers), the same number on
+// every CU, and among those numbers the one that leaves the fewest idle in the last turn.
 constexpr int CUS = 256, STREAM_SLICES = 64;
-int64_t even_grid(int64_t turns, int64_t resident) { return turns <= resident ? turns : cdiv(turns, cdiv(turns, resident)); }
+int64_t even_grid(int64_t turns, int per_cu) {
+  if (turns <= (int64_t)CUS * per_cu) return turns;
+  int best = per_cu;
+  for (int k = per_cu; k > per_cu / 2; --k)
+    if (cdiv(turns, (int64_t)CUS * k) * k < cdiv(turns, (int64_t)CUS * best) * best) best = k;
+  return (int64_t)CUS * best;
+}
 int64_t fwd_grid(const Shape& s, int32_t type, int64_t M) {
   if (s.form == 2) return M < 2 * CUS ? M : 2 * CUS;
   const int per_cu = s.threads == 1024 ? 1 : s.threads == 512 ? 2 : type == GANET_F32 ? 6 : 4;
-  return even_grid(cdiv(M, s.form ? 1 : s.threads / s.G), (int64_t)CUS * per_cu);
+  return even_grid(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu);
 }
 int64_t bwd_grid(const Shape& s, int32_t type, int64_t M) {
   if (s.form == 2) return M < STREAM_SLICES ? M : STREAM_SLICES;
   const int per_cu = s.threads >= 512 ? (type == GANET_F32 && s.threads == 512 ? 2 : 1) : type == GANET_F32 ? (s.NC > 2 ? 2 : 4) : s.NC > 2 ? 1 : s.form ? 3 : 2;
-  return even_grid(cdiv(M, s.form ? 1 : s.threads / s.G), (int64_t)CUS * per_cu);
+  return even_grid(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu);
 }
 
 bool ln_ok(int64_t M, int64_t C, int32_t type, int32_t wtype, int32_t act) {
