@@ -171,7 +171,8 @@ GANET_SYMBOLS = ["ganet_linear_wgrad_workspace", "ganet_linear_wgrad", "ganet_bn
                  "ganet_conv5_packed_bytes", "ganet_conv5_pack", "ganet_conv5_apply",
                  "ganet_conv5_wgrad_workspace", "ganet_conv5_wgrad",
                  "ganet_ln_code_exponent", "ganet_ln_fwd", "ganet_ln_bwd_workspace", "ganet_ln_bwd", "ganet_rows8_pack", "ganet_rows8_unpack",
-                 "ganet_weight8_pack", "ganet_gemm8_workspace", "ganet_gemm8", "ganet_wgrad8_workspace", "ganet_wgrad8",
+                 "ganet_weight8_pack", "ganet_gemm8", "ganet_rows8_bytes", "ganet_weight8_bytes", "ganet_linear8_held_workspace", "ganet_linear8_held",
+                 "ganet_linear8_fwd", "ganet_linear8_bwd_workspace", "ganet_linear8_bwd", "ganet_wgrad8_workspace", "ganet_wgrad8",
                  "ganet_last_error", "ganet_abi_version"]
 
 
@@ -350,10 +351,18 @@ def ganet() -> ctypes.CDLL:
         lib.ganet_rows8_unpack.argtypes = [L, L, I, I, P, L, P, L, P, P]
         lib.ganet_weight8_pack.restype = c_int
         lib.ganet_weight8_pack.argtypes = [L, L, I, P, L, P, L, P, L, P, L, P, L, P]
-        lib.ganet_gemm8_workspace.restype = c_size_t
-        lib.ganet_gemm8_workspace.argtypes = [L, L, L]
         lib.ganet_gemm8.restype = c_int
-        lib.ganet_gemm8.argtypes = [L, L, L, I, P, L, P, L, P, L, P, L, P, I, P, L, I, P, c_size_t, P]
+        lib.ganet_gemm8.argtypes = [L, L, L, I, P, L, P, L, P, L, P, L, P, I, P, L, I, P]
+        for name, args in (("ganet_rows8_bytes", [L, L]), ("ganet_weight8_bytes", [L, L]), ("ganet_linear8_held_workspace", [L, L]),
+                           ("ganet_linear8_bwd_workspace", [L, L, L, I])):
+            getattr(lib, name).restype = c_size_t
+            getattr(lib, name).argtypes = args
+        lib.ganet_linear8_held.restype = c_int
+        lib.ganet_linear8_held.argtypes = [L, L, L, I, P, L, P, L, P, L, P, I, P, P, c_size_t, P]
+        lib.ganet_linear8_fwd.restype = c_int
+        lib.ganet_linear8_fwd.argtypes = [L, L, L, I, P, L, I, P, L, P, I, P, P, P, P, P]
+        lib.ganet_linear8_bwd.restype = c_int
+        lib.ganet_linear8_bwd.argtypes = [L, L, L, I, P, L, P, P, P, P, P, I, P, c_size_t, P]
         lib.ganet_wgrad8_workspace.restype = c_size_t
         lib.ganet_wgrad8_workspace.argtypes = [L, L, L, I]
         lib.ganet_wgrad8.restype = c_int

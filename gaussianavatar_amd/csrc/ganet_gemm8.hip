@@ -271,13 +271,32 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// The weight's codes are the traffic: every wave streams its share of the blocks of 16 weight rows straight from global memory
-// into matrix operands (a lane: 32 codes of one row), the eight waves' sums meet in LDS.
+// The weight's codes are the traffic: every wave streams its share of the blocks of 16 weight rows straight from global memory into matrix
+// operands (a lane: 32 codes of one row), the eight waves' sums meet in LDS. X: the rows' type. Rows that come as they are (not as
+// codes) are packed in registers, by the rule of ganet_rows8_pack: the four lanes that hold a row's block take its maximum and
+// convert; every workgroup repeats that, which costs less than a launch for up to 32 rows.
 constexpr int FEW_WAVES = 8, FEW_UNROLL = 4;
+struct Codes;        // the rows' type where they are codes already
 
-template <int FMT, int MT, typename Y>
+// 32 values of a row's block, held by the four lanes l, l ^ 16, l ^ 32, l ^ 48 -> operand and biased exponent
+__device__ __forceinline__ void pack_block(const float (&v)[32], i32x8& f, int& e) {
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) a = fmaxf(a, finite_abs(v[i]));
+  a = fmaxf(a, __shfl_xor(a, 16));
+  a = fmaxf(a, __shfl_xor(a, 32));
+  const int x = block_exponent<GANET_E4M3>(a);
+  const float s = pow2(-x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (int)pack4<GANET_E4M3>(v[4 * i] * s, v[4 * i + 1] * s, v[4 * i + 2] * s, v[4 * i + 3] * s);
+  e = x + 127;
+}
+
+template <int FMT, int MT, typename X, typename Y>
 __global__ void __launch_bounds__(64 * FEW_WAVES)
 gemm8_few_kernel(Operands o) {
+  constexpr bool CODES = __is_same(X, Codes), EXACT = sizeof(Y) == 4;
+  constexpr int UNROLL = CODES ? FEW_UNROLL : 2;
   __shared__ f32x4 s_acc[FEW_WAVES][MT][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
@@ -285,22 +304,16 @@ gemm8_few_kernel(Operands o) {
   const int KB = (int)((o.K + BLOCK - 1) / BLOCK);
   const uint8_t* wr = o.w + min(n0 + r, o.N - 1) * o.ldw + q * 32;
   const uint8_t* ew = o.ew + n0 / BLOCK * o.ldew;
-  const uint8_t *xr[MT], *ex[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int64_t m = min((int64_t)(i * 16 + r), o.M - 1);
-    xr[i] = o.x + m * o.ldx + q * 32;
-    ex[i] = o.ex + m * o.ldex;
-  }
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int kb0 = wave; kb0 < KB; kb0 += FEW_WAVES * FEW_UNROLL) {
-    uint4 w[FEW_UNROLL][2], x[FEW_UNROLL][MT][2];
-    int sw[FEW_UNROLL], sx[FEW_UNROLL][MT];
+  for (int kb0 = wave; kb0 < KB; kb0 += FEW_WAVES * UNROLL) {
+    uint4 w[UNROLL][2];
+    i32x8 x[UNROLL][MT];
+    int sw[UNROLL], sx[UNROLL][MT];
 #pragma unroll
-    for (int u = 0; u < FEW_UNROLL; ++u) {
+    for (int u = 0; u < UNROLL; ++u) {
       const int kb = kb0 + u * FEW_WAVES;
       const int64_t k = (int64_t)kb * BLOCK;
       const bool lo = kb < KB && k + q * 32 < kend, hi = kb < KB && k + q * 32 + 16 < kend;
@@ -309,17 +322,37 @@ gemm8_few_kernel(Operands o) {
       sw[u] = kb < KB ? ew[kb] : 127;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        x[u][i][0] = lo ? *reinterpret_cast<const uint4*>(xr[i] + k) : zero;
-        x[u][i][1] = hi ? *reinterpret_cast<const uint4*>(xr[i] + k + 16) : zero;
-        sx[u][i] = kb < KB ? ex[i][kb] : 127;
+        const int64_t m = min((int64_t)(i * 16 + r), o.M - 1);
+        if constexpr (CODES) {
+          const uint8_t* xr = o.x + m * o.ldx + k + q * 32;
+          x[u][i] = join(lo ? *reinterpret_cast<const uint4*>(xr) : zero, hi ? *reinterpret_cast<const uint4*>(xr + 16) : zero);
+          sx[u][i] = kb < KB ? o.ex[m * o.ldex + kb] : 127;
+        } else {
+          float v[32];
+          const X* xr = reinterpret_cast<const X*>(o.x) + m * o.ldx + k + q * 32;
+          load_n(xr, i * 16 + r < o.M && kb < KB ? o.K - (k + q * 32) : 0, v);
+          pack_block(v, x[u][i], sx[u][i]);
+        }
       }
     }
 #pragma unroll
-    for (int u = 0; u < FEW_UNROLL; ++u)
+    for (int u = 0; u < UNROLL; ++u) {
+      const i32x8 b = join(w[u][0], w[u][1]);
+      if constexpr (!EXACT) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w[u][0], w[u][1]), join(x[u][i][0], x[u][i][1]), acc[i],
-                                                                  GANET_E4M3, FMT, 0, sw[u], 0, sx[u][i]);
+        for (int i = 0; i < MT; ++i)
+          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, x[u][i], acc[i], GANET_E4M3, FMT, 0, sw[u], 0, sx[u][i]);
+      } else {
+        // fp32 results: bf16 instructions on decoded codes (see multiply() above)
+#pragma unroll
+        for (int d = 0; d < 8; d += 2) {
+          const bf16x8 wd = decode8<GANET_E4M3>(b, d, pow2(sw[u] - 127));
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd, decode8<FMT>(x[u][i], d, pow2(sx[u][i] - 127)), acc[i], 0, 0, 0);
+        }
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) s_acc[wave][i][lane] = acc[i];
@@ -335,6 +368,15 @@ gemm8_few_kernel(Operands o) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) v[c] = t[c] + ((o.bias && n + c < o.N) ? load_param(o.bias, o.btype, n + c) : 0.f);
   store_n(static_cast<Y*>(o.y) + m * o.ldy + n, o.N - n, v);
+}
+
+constexpr int FEW_ROWS = 32;
+template <int FMT, typename X, typename Y>
+int launch_few(const Operands& o, hipStream_t stream) {
+  const dim3 grid((unsigned)cdiv(o.N, 16));
+  if (o.M <= 16) hipLaunchKernelGGL((gemm8_few_kernel<FMT, 1, X, Y>), grid, dim3(64 * FEW_WAVES), 0, stream, o);
+  else hipLaunchKernelGGL((gemm8_few_kernel<FMT, 2, X, Y>), grid, dim3(64 * FEW_WAVES), 0, stream, o);
+  return check_hip(hipGetLastError(), "ganet_gemm8");
 }
 
 template <int FMT, int MT, int NT, typename Y>
@@ -356,15 +398,23 @@ int launch_tile(const Operands& o, hipStream_t stream) {
 
 template <int FMT, typename Y>
 int launch(const Operands& o, hipStream_t stream) {
-  if (o.M <= 32) {
-    const dim3 grid((unsigned)cdiv(o.N, 16));
-    if (o.M <= 16) hipLaunchKernelGGL((gemm8_few_kernel<FMT, 1, Y>), grid, dim3(64 * FEW_WAVES), 0, stream, o);
-    else hipLaunchKernelGGL((gemm8_few_kernel<FMT, 2, Y>), grid, dim3(64 * FEW_WAVES), 0, stream, o);
-    return check_hip(hipGetLastError(), "ganet_gemm8");
-  }
+  if (o.M <= FEW_ROWS) return launch_few<FMT, Codes, Y>(o, stream);
   if constexpr (sizeof(Y) == 2)
     if (cdiv(o.M, 256) * cdiv(o.N, 256) >= 256) return launch_tile<FMT, 4, 4, Y>(o, stream);
   return launch_tile<FMT, 2, 2, Y>(o, stream);
+}
+
+bool held_ok(int64_t N, int64_t K, const void* c, int64_t ld, const uint8_t* e, int64_t le) {
+  return c && e && ld % 16 == 0 && ld >= pad16(K) && (reinterpret_cast<uintptr_t>(c) & 15) == 0 && le % 4 == 0 &&
+         le >= cdiv(K, BLOCK) && (reinterpret_cast<uintptr_t>(e) & 3) == 0;
+}
+
+// Where a buffer of ganet_rows8_bytes / ganet_weight8_bytes keeps its codes and exponents
+struct Packed { uint8_t* codes; int64_t ldc; uint8_t* exps; int64_t lde; };
+Packed packed(void* buffer, int64_t rows, int64_t cols) {
+  const int64_t ldc = pad16(cols);
+  uint8_t* b = static_cast<uint8_t*>(buffer);
+  return {b, ldc, b + rows * ldc, (cdiv(cols, BLOCK) + 3) / 4 * 4};
 }
 
 }  // namespace
@@ -374,22 +424,16 @@ using namespace ganet;
 
 extern "C" {
 
-size_t ganet_gemm8_workspace(int64_t M, int64_t N, int64_t K) { return 0; }
-
 int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes, int64_t ldc, const uint8_t* exps, int64_t lde,
                 const void* wcodes, int64_t ldwc, const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y,
-                int64_t ldy, int32_t ytype, void* workspace, size_t workspace_bytes, void* stream_) {
+                int64_t ldy, int32_t ytype, void* stream_) {
   if (!rows_ok(M, K) || N < 1 || N >= (1ll << 24) || (fmt != GANET_E4M3 && fmt != GANET_E5M2) || !type_ok(ytype) || !type_ok(btype)) {
     set_error("ganet_gemm8: unsupported M=%lld N=%lld K=%lld format=%d types=%d,%d", (long long)M, (long long)N, (long long)K, fmt,
               ytype, btype);
     return 4;
   }
   if (M == 0) return 0;
-  const auto ok = [&](const void* c, int64_t ld, const uint8_t* e, int64_t le) {
-    return c && e && ld % 16 == 0 && ld >= pad16(K) && (reinterpret_cast<uintptr_t>(c) & 15) == 0 && le % 4 == 0 &&
-           le >= cdiv(K, BLOCK) && (reinterpret_cast<uintptr_t>(e) & 3) == 0;
-  };
-  if (!y || (ldy < N && M > 1) || !ok(codes, ldc, exps, lde) || !ok(wcodes, ldwc, wexps, ldwe)) {
+  if (!y || (ldy < N && M > 1) || !held_ok(M, K, codes, ldc, exps, lde) || !held_ok(N, K, wcodes, ldwc, wexps, ldwe)) {
     set_error("ganet_gemm8: NULL or misaligned argument, or a row stride too small");
     return 1;
   }
@@ -397,6 +441,84 @@ int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes,
   const Operands o{M, N, K, static_cast<const uint8_t*>(codes), ldc, exps, lde, static_cast<const uint8_t*>(wcodes), ldwc, wexps,
                    ldwe, bias, btype, y, ldy};
   GANET_BY_TYPE(ytype, T, return fmt == GANET_E4M3 ? launch<GANET_E4M3, T>(o, stream) : launch<GANET_E5M2, T>(o, stream));
+}
+
+size_t ganet_rows8_bytes(int64_t M, int64_t C) {
+  return rows_ok(M, C) ? (size_t)(M * pad16(C) + M * ((cdiv(C, BLOCK) + 3) / 4 * 4)) : 0;
+}
+
+size_t ganet_weight8_bytes(int64_t N, int64_t K) {
+  return rows_ok(N, K) ? (size_t)(N * pad16(K) + cdiv(N, BLOCK) * ((cdiv(K, BLOCK) + 3) / 4 * 4)) : 0;
+}
+
+size_t ganet_linear8_held_workspace(int64_t M, int64_t K) { return M <= FEW_ROWS ? 0 : ganet_rows8_bytes(M, K); }
+
+int ganet_linear8_held(int64_t M, int64_t N, int64_t K, int32_t type, const void* x, int64_t ldx, const void* wcodes, int64_t ldwc,
+                       const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y, void* workspace,
+                       size_t workspace_bytes, void* stream_) {
+  if (!rows_ok(M, K) || N < 1 || N >= (1ll << 24) || !type_ok(type) || !type_ok(btype)) {
+    set_error("ganet_linear8_held: unsupported M=%lld N=%lld K=%lld types=%d,%d", (long long)M, (long long)N, (long long)K, type, btype);
+    return 4;
+  }
+  if (M == 0) return 0;
+  if (!x || !y || (ldx < K && M > 1) || !held_ok(N, K, wcodes, ldwc, wexps, ldwe) ||
+      workspace_bytes < ganet_linear8_held_workspace(M, K) || (M > FEW_ROWS && !workspace)) {
+    set_error("ganet_linear8_held: NULL or misaligned argument, a row stride or the workspace too small");
+    return 1;
+  }
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  if (M <= FEW_ROWS) {
+    const Operands o{M, N, K, static_cast<const uint8_t*>(x), ldx, nullptr, 0, static_cast<const uint8_t*>(wcodes), ldwc, wexps, ldwe,
+                     bias, btype, y, N};
+    GANET_BY_TYPE(type, T, return (launch_few<GANET_E4M3, T, T>(o, stream)));
+  }
+  const Packed r = packed(workspace, M, K);
+  const int rc = ganet_rows8_pack(M, K, type, GANET_E4M3, x, ldx, r.codes, r.ldc, r.exps, r.lde, stream_);
+  return rc ? rc : ganet_gemm8(M, N, K, GANET_E4M3, r.codes, r.ldc, r.exps, r.lde, wcodes, ldwc, wexps, ldwe, bias, btype, y, N, type,
+                               stream_);
+}
+
+int ganet_linear8_fwd(int64_t M, int64_t N, int64_t K, int32_t type, const void* x, int64_t ldx, int32_t wtype, const void* w,
+                      int64_t ldw, const void* bias, int32_t btype, void* y, void* rows8, void* weight8, void* tweight8,
+                      void* stream_) {
+  if (!rows_ok(M, K) || !rows_ok(N, K) || N < 1 || !rows8 || !weight8) {
+    set_error("ganet_linear8_fwd: unsupported M=%lld N=%lld K=%lld, or a NULL buffer", (long long)M, (long long)N, (long long)K);
+    return 4;
+  }
+  const Packed r = packed(rows8, M, K), p = packed(weight8, N, K), t = tweight8 ? packed(tweight8, K, N) : Packed{};
+  int rc = ganet_rows8_pack(M, K, type, GANET_E4M3, x, ldx, r.codes, r.ldc, r.exps, r.lde, stream_);
+  if (!rc) rc = ganet_weight8_pack(N, K, wtype, w, ldw, p.codes, p.ldc, p.exps, p.lde, t.codes, t.ldc, t.exps, t.lde, stream_);
+  return rc ? rc : ganet_gemm8(M, N, K, GANET_E4M3, r.codes, r.ldc, r.exps, r.lde, p.codes, p.ldc, p.exps, p.lde, bias, btype, y, N,
+                               type, stream_);
+}
+
+size_t ganet_linear8_bwd_workspace(int64_t M, int64_t N, int64_t K, int32_t type) {
+  const size_t rows = (ganet_rows8_bytes(M, N) + 255) / 256 * 256;
+  return rows + ganet_wgrad8_workspace(M, N, K, type);
+}
+
+int ganet_linear8_bwd(int64_t M, int64_t N, int64_t K, int32_t type, const void* g, int64_t ldg, const void* rows8,
+                      const void* tweight8, void* dx, void* dW, void* db, int32_t wtype, void* workspace, size_t workspace_bytes,
+                      void* stream_) {
+  if (!rows_ok(M, K) || !rows_ok(M, N) || N < 1 || workspace_bytes < ganet_linear8_bwd_workspace(M, N, K, type) || !workspace ||
+      !rows8 || (dx && !tweight8)) {
+    set_error("ganet_linear8_bwd: unsupported M=%lld N=%lld K=%lld, a NULL buffer, or the workspace too small", (long long)M,
+              (long long)N, (long long)K);
+    return 4;
+  }
+  int rc = 0;
+  if (dx) {
+    const Packed q = packed(workspace, M, N), t = packed(const_cast<void*>(tweight8), K, N);
+    rc = ganet_rows8_pack(M, N, type, GANET_E4M3, g, ldg, q.codes, q.ldc, q.exps, q.lde, stream_);
+    if (!rc)
+      rc = ganet_gemm8(M, K, N, GANET_E4M3, q.codes, q.ldc, q.exps, q.lde, t.codes, t.ldc, t.exps, t.lde, nullptr, GANET_F32, dx, K, type,
+                       stream_);
+  }
+  if (rc || !dW) return rc;
+  const Packed r = packed(const_cast<void*>(rows8), M, K);
+  uint8_t* ws = static_cast<uint8_t*>(workspace) + (ganet_rows8_bytes(M, N) + 255) / 256 * 256;
+  return ganet_wgrad8(M, N, K, GANET_E4M3, type, g, ldg, r.codes, r.ldc, r.exps, r.lde, dW, db, wtype, ws,
+                      ganet_wgrad8_workspace(M, N, K, type), stream_);
 }
 
 }  // extern "C"

@@ -220,42 +220,49 @@ class _LayerNormActFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, act, kept8):
-        lib = _native.ganet()
         x2 = rows8._rows2d(x)
         M, C = x2.shape
-        grad = any(ctx.needs_input_grad[:3])
-        y = torch.empty((M, C), dtype=x.dtype, device=x.device)
-        f32 = lambda: torch.empty(M, dtype=torch.float32, device=x.device)
-        mean = f32() if grad and not kept8 else None
-        rstd = f32() if grad else None
-        ldc = (C + 15) // 16 * 16
-        codes = torch.empty((M, ldc), dtype=torch.uint8, device=x.device) if grad and kept8 else None
-        wtype = 0 if weight is None else rows8._TYPE_CODE[weight.dtype]
-        rows8._call(x.device, lib.ganet_ln_fwd, M, C, rows8._TYPE_CODE[x.dtype], wtype, _ptr(x2), rows8._ld(x2), _ptr(weight), _ptr(bias),
-                    float(eps), _ACTS[act], _ptr(y), _ptr(mean), _ptr(rstd), _ptr(codes), ldc)
-        ctx.save_for_backward(None if kept8 else x2, weight, bias, mean, rstd, codes)
+        stats = torch.empty(M if kept8 else 2 * M, dtype=torch.float32, device=x.device)          # rstd, then the mean
+        codes = torch.empty((M, (C + 15) // 16 * 16), dtype=torch.uint8, device=x.device) if kept8 else None
+        y = _ln_fwd(x2, weight, bias, eps, act, stats, codes)
+        ctx.save_for_backward(None if kept8 else x2, weight, bias, stats, codes)
         ctx.act, ctx.shape, ctx.dtype = act, x.shape, x.dtype
-        return y.reshape(x.shape)
+        return y if x.dim() == 2 else y.reshape(x.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        lib = _native.ganet()
-        x2, weight, bias, mean, rstd, codes = ctx.saved_tensors
+        x2, weight, bias, stats, codes = ctx.saved_tensors
         g2 = rows8._rows2d(dy)
         M, C = g2.shape
         code = rows8._TYPE_CODE[ctx.dtype]
-        need_x = ctx.needs_input_grad[0]
-        dx = torch.empty((M, C), dtype=ctx.dtype, device=dy.device) if need_x else None
-        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
-        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
+        lib, dev = _native.ganet(), dy.device
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty((M, C), dtype=ctx.dtype, device=dev) if need_x else None
+        dw = torch.empty_like(weight) if weight is not None and need_w else None
+        db = torch.empty_like(bias) if bias is not None and need_b else None
         nbytes = lib.ganet_ln_bwd_workspace(M, C, code) if (dw is not None or db is not None) else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
-        wtype = 0 if weight is None else rows8._TYPE_CODE[weight.dtype]
-        rows8._call(dy.device, lib.ganet_ln_bwd, M, C, code, wtype, _ptr(x2), 0 if x2 is None else rows8._ld(x2), _ptr(mean), _ptr(codes),
-                    0 if codes is None else codes.stride(0), _ptr(rstd), _ptr(weight), _ptr(bias), _ACTS[ctx.act], _ptr(g2),
-                    rows8._ld(g2), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
-        return (None if dx is None else dx.reshape(ctx.shape)), dw, db, None, None, None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        ptr = rows8._ptr
+        at = stats.data_ptr()
+        rows8._call(dev, lib.ganet_ln_bwd, M, C, code, 0 if weight is None else rows8._TYPE_CODE[weight.dtype], ptr(x2),
+                    0 if x2 is None else rows8._ld(x2), at + 4 * M, ptr(codes), 0 if codes is None else codes.shape[1], at, ptr(weight),
+                    ptr(bias), _ACTS[ctx.act], g2.data_ptr(), rows8._ld(g2), ptr(dx), ptr(dw), ptr(db), ptr(ws), nbytes)
+        if dx is not None and len(ctx.shape) != 2:
+            dx = dx.reshape(ctx.shape)
+        return dx, dw, db, None, None, None
+
+
+def _ln_fwd(x2, weight, bias, eps, act, stats, codes):
+    M, C = x2.shape
+    y = torch.empty((M, C), dtype=x2.dtype, device=x2.device)
+    ptr = rows8._ptr
+    at = ptr(stats)
+    rows8._call(x2.device, _native.ganet().ganet_ln_fwd, M, C, rows8._TYPE_CODE[x2.dtype],
+                0 if weight is None else rows8._TYPE_CODE[weight.dtype], x2.data_ptr(), rows8._ld(x2), ptr(weight), ptr(bias), eps,
+                _ACTS[act], y.data_ptr(), at + 4 * M if at and codes is None else None, at, ptr(codes),
+                0 if codes is None else codes.shape[1])
+    return y
 
 
 class _LayerNormKept8Plain(torch.autograd.Function):
@@ -301,15 +308,19 @@ def layernorm_act(x, ln: torch.nn.LayerNorm, act: str = "softplus", checkpoint8:
         raise ValueError(f"layernorm_act: act {act!r} (known: {', '.join(_ACTS)})")
     if len(ln.normalized_shape) != 1 or x.dim() < 1 or x.shape[-1] != ln.normalized_shape[0]:
         raise ValueError(f"layernorm_act: LayerNorm over {tuple(ln.normalized_shape)} for {tuple(x.shape)}")
-    params = [p for p in (ln.weight, ln.bias) if p is not None]
+    weight, bias = ln.weight, ln.bias
+    params = [p for p in (weight, bias) if p is not None]
     rows8._same_device("layernorm_act", x, *params)
-    known = x.dtype in rows8._TYPE_CODE and all(p.dtype in rows8._TYPE_CODE for p in params) and len({p.dtype for p in params}) < 2
+    known = x.dtype in rows8._TYPE_CODE and all(p.dtype in rows8._TYPE_CODE and p.dtype == params[0].dtype for p in params)
     if x.is_cuda and known:
-        return _LayerNormActFn.apply(x, ln.weight, ln.bias, ln.eps, act, checkpoint8)
+        if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)):
+            return _LayerNormActFn.apply(x, weight, bias, ln.eps, act, checkpoint8)
+        y = _ln_fwd(rows8._rows2d(x.detach()), weight, bias, ln.eps, act, None, None)
+        return y if x.dim() == 2 else y.reshape(x.shape)
     if checkpoint8:
         if x.is_cuda or not known:
             raise TypeError(f"layernorm_act: checkpoint8 with {x.dtype} rows and {[p.dtype for p in params]} parameters")
-        return _LayerNormKept8Plain.apply(x, ln.weight, ln.bias, ln.eps, act)
+        return _LayerNormKept8Plain.apply(x, weight, bias, ln.eps, act)
     return _act_plain(ln(x), act)
 
 

@@ -16,8 +16,6 @@ fp32, bf16 and fp16 tensors on a HIP device run on the kernels; on the CPU the s
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _native
@@ -29,16 +27,19 @@ BLOCK = 128
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _call(device, fn, *args):
     """fn(*args, stream) on `device`'s current stream; the launch happens with that device current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        _native.ganet_check(fn(*args, ctypes.c_void_p(_native.raw_stream(device))))
-        return
-    with torch.cuda.device(device):
-        _native.ganet_check(fn(*args, ctypes.c_void_p(_native.raw_stream(device))))
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if index is None else index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _native.ganet_check(rc)
 
 
 def _type_code(t, what):
@@ -240,14 +241,11 @@ def matmul8(rows, w8, bias=None, dtype=torch.float32):
     if not rows.codes.is_cuda:
         y = _plain_values(rows.codes, rows.exps, K) @ w8.dequantize().t()
         return (y if bias is None else y + bias.float()).to(dtype).reshape(*rows.lead, N)
-    lib = _native.ganet()
     y = torch.empty((M, N), dtype=dtype, device=rows.codes.device)
     bias = None if bias is None else bias.detach().contiguous()
-    nbytes = lib.ganet_gemm8_workspace(M, N, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=y.device) if nbytes else None
-    _call(y.device, lib.ganet_gemm8, M, N, K, _FMT_CODE[rows.codes.dtype], _ptr(rows.codes), rows.codes.stride(0), _ptr(rows.exps),
-          rows.exps.stride(0), _ptr(w8.codes), w8.codes.stride(0), _ptr(w8.exps), w8.exps.stride(0), _ptr(bias), btype, _ptr(y), N,
-          _TYPE_CODE[dtype], _ptr(ws), nbytes)
+    _call(y.device, _native.ganet().ganet_gemm8, M, N, K, _FMT_CODE[rows.codes.dtype], _ptr(rows.codes), rows.codes.stride(0),
+          _ptr(rows.exps), rows.exps.stride(0), _ptr(w8.codes), w8.codes.stride(0), _ptr(w8.exps), w8.exps.stride(0), _ptr(bias), btype,
+          _ptr(y), N, _TYPE_CODE[dtype])
     return y.reshape(*rows.lead, N)
 
 
@@ -279,30 +277,75 @@ def wgrad8(g, rows, dtype=None):
     return dW, db
 
 
+def _bytes(n, like):
+    return torch.empty(n, dtype=torch.uint8, device=like.device)
+
+
 class _Linear8Fn(torch.autograd.Function):
     """y = Q(x) Q(W)^T + b; dx = Q(g) Q(W); dW = g^T Q(x); db = sum g. The packed input of the product is what the backward pass keeps of x."""
 
     @staticmethod
     def forward(ctx, x, weight, bias):
-        rows = quantize8(x)
-        w8 = quantize8_weight(weight, transposed=ctx.needs_input_grad[0])
-        ctx.save_for_backward(rows.codes, rows.exps, w8.t_codes, w8.t_exps)
+        x2, w2 = _rows2d(x), _rows2d(weight)
+        M, K = x2.shape
+        N = w2.shape[0]
+        lib = _native.ganet()
+        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        rows, held = _bytes(max(16, lib.ganet_rows8_bytes(M, K)), x), _bytes(lib.ganet_weight8_bytes(N, K), x)
+        back = _bytes(lib.ganet_weight8_bytes(K, N), x) if ctx.needs_input_grad[0] else None
+        b = None if bias is None else bias.contiguous()
+        _call(x.device, lib.ganet_linear8_fwd, M, N, K, _TYPE_CODE[x.dtype], x2.data_ptr(), _ld(x2), _TYPE_CODE[weight.dtype],
+              w2.data_ptr(), _ld(w2), _ptr(b), 0 if b is None else _TYPE_CODE[b.dtype], y.data_ptr(), rows.data_ptr(),
+              held.data_ptr(), _ptr(back))
+        ctx.save_for_backward(rows, back)
+        ctx.dims, ctx.shape = (M, N, K), x.shape
         ctx.types = (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        ctx.lead, ctx.dims = rows.lead, w8.shape
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        rows, back = ctx.saved_tensors
+        M, N, K = ctx.dims
+        xt, wt, bt = ctx.types
+        need_x, need_w, need_b = ctx.needs_input_grad
+        need_b = need_b and bt is not None
+        lib = _native.ganet()
+        g2 = _rows2d(g)
+        new = lambda shape, t: torch.empty(shape, dtype=t, device=g.device)
+        dx = new((M, K), xt) if need_x else None
+        dW = new((N, K), wt) if need_w or need_b else None
+        db = new(N, wt) if need_b else None
+        code = _TYPE_CODE[xt]
+        ws = _bytes(max(16, lib.ganet_linear8_bwd_workspace(M, N, K, code)), g)
+        _call(g.device, lib.ganet_linear8_bwd, M, N, K, code, g2.data_ptr(), _ld(g2), rows.data_ptr(), _ptr(back), _ptr(dx), _ptr(dW),
+              _ptr(db), _TYPE_CODE[wt], ws.data_ptr(), ws.numel())
+        if need_x and len(ctx.shape) != 2:
+            dx = dx.reshape(ctx.shape)
+        return dx, dW if need_w else None, db.to(bt) if need_b else None
+
+
+class _Linear8Plain(torch.autograd.Function):
+    """The same in torch operations (CPU)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        rows = quantize8(x)
+        w8 = quantize8_weight(weight)
+        ctx.save_for_backward(rows.codes, rows.exps, w8.codes, w8.exps)
+        ctx.shape, ctx.types = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
         return matmul8(rows, w8, bias, x.dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        codes, exps, t_codes, t_exps = ctx.saved_tensors
+        codes, exps, w_codes, w_exps = ctx.saved_tensors
         xt, wt, bt = ctx.types
-        dx = dW = db = None
-        if ctx.needs_input_grad[0]:
-            dx = matmul8(quantize8(g), Weight8(t_codes, t_exps, ctx.dims[0]), None, xt)
-        if ctx.needs_input_grad[1] or (bt is not None and ctx.needs_input_grad[2]):
-            dW, db = wgrad8(g, Rows8(codes, exps, ctx.dims[1], ctx.lead), wt)
-            db = None if bt is None else db.to(bt)
-        return dx, dW, db
+        w = Weight8(w_codes, w_exps, ctx.shape[-1]).dequantize()
+        q = quantize8(g)
+        dx = (q.dequantize() @ w).to(xt)
+        dW, db = wgrad8(g, Rows8(codes, exps, ctx.shape[-1], ctx.shape[:-1]), wt)
+        return dx, dW, None if bt is None else db.to(bt)
 
 
 def linear8(x, weight, bias=None):
@@ -316,12 +359,31 @@ def linear8(x, weight, bias=None):
             raise ValueError(f"linear8: {K} columns for a weight of {weight.cols}")
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise RuntimeError("linear8: a held Weight8 is for evaluation (torch.no_grad()); pass the weight itself to train")
-        return matmul8(quantize8(x), weight, bias, x.dtype)
+        if not x.is_cuda:
+            return matmul8(quantize8(x), weight, bias, x.dtype)
+        N = weight.codes.shape[0]
+        if bias is not None and tuple(bias.shape) != (N,):
+            raise ValueError(f"linear8: a bias of {tuple(bias.shape)} for {N} columns")
+        code = _type_code(x, "linear8")
+        btype = 0 if bias is None else _type_code(bias, "linear8: bias")
+        _same_device("linear8", x, weight.codes, bias)
+        x2 = _rows2d(x.detach())
+        M = x2.shape[0]
+        lib = _native.ganet()
+        y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        nbytes = lib.ganet_linear8_held_workspace(M, K)
+        ws = _bytes(nbytes, x) if nbytes else None
+        bias = None if bias is None else bias.detach().contiguous()
+        _call(x.device, lib.ganet_linear8_held, M, N, K, code, x2.data_ptr(), _ld(x2), weight.codes.data_ptr(), weight.codes.stride(0),
+              weight.exps.data_ptr(), weight.exps.stride(0), _ptr(bias), btype, y.data_ptr(), _ptr(ws), nbytes)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
     if weight.dim() != 2 or weight.shape[1] != K:
         raise ValueError(f"linear8: {K} columns for a weight of {tuple(weight.shape)}")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError(f"linear8: a bias of {tuple(bias.shape)} for {weight.shape[0]} columns")
     _type_code(x, "linear8")
     _type_code(weight, "linear8: weight")
+    if bias is not None:
+        _type_code(bias, "linear8: bias")
     _same_device("linear8", x, weight, bias)
-    return _Linear8Fn.apply(x, weight, bias)
+    return (_Linear8Fn if x.is_cuda else _Linear8Plain).apply(x, weight, bias)

@@ -413,16 +413,34 @@ int ganet_weight8_pack(int64_t N, int64_t K, int32_t type, const void* w, int64_
                        int64_t lde, void* tcodes, int64_t ldtc, uint8_t* texps, int64_t ldte, void* stream);
 /* y [M, N] = rows [M, K] weight [N, K]^T + bias (btype, NULL: none): e4m3 or e5m2 rows, e4m3 weight; the matrix cores apply the
  * powers of two and accumulate in fp32; one rounding to ytype. */
-size_t ganet_gemm8_workspace(int64_t M, int64_t N, int64_t K);
 int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes, int64_t ldc, const uint8_t* exps, int64_t lde,
                 const void* wcodes, int64_t ldwc, const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y,
-                int64_t ldy, int32_t ytype, void* workspace, size_t workspace_bytes, void* stream);
+                int64_t ldy, int32_t ytype, void* stream);
 /* dW [N, K] = g^T rows, db [N] = column sums of g (NULL: not needed), both contiguous in otype: the weight gradient of a layer
  * whose input is kept as rows in 8 bits. g [M, N] in gtype enters with all its bits. */
 size_t ganet_wgrad8_workspace(int64_t M, int64_t N, int64_t K, int32_t gtype);
 int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, const void* g, int64_t ldg, const void* codes,
                  int64_t ldc, const uint8_t* exps, int64_t lde, void* dW, void* db, int32_t otype, void* workspace,
                  size_t workspace_bytes, void* stream);
+
+/* A linear layer on these, y [M, N] = Q(x) Q(W)^T + bias in x's type (e4m3 both), as one call each way.
+ * _held: the weight is codes already; up to 32 rows are packed inside the product's kernel (no workspace).
+ * _fwd / _bwd: training. rows8 (ganet_rows8_bytes(M, K)) keeps Q(x) for the backward pass, weight8 (ganet_weight8_bytes(N, K)) holds Q(W)
+ * during the call, tweight8 (ganet_weight8_bytes(K, N); NULL: no input gradient) its transposed codes for the backward pass; each
+ * buffer: codes, row stride = columns up to a multiple of 16, then exponents, row stride = blocks of 128 up to a multiple of 4.
+ * dx = Q(g) Q(W) (NULL: not needed), dW = g^T Q(x) and db in wtype (dW NULL: neither). */
+size_t ganet_rows8_bytes(int64_t M, int64_t C);
+size_t ganet_weight8_bytes(int64_t N, int64_t K);
+size_t ganet_linear8_held_workspace(int64_t M, int64_t K);
+int ganet_linear8_held(int64_t M, int64_t N, int64_t K, int32_t type, const void* x, int64_t ldx, const void* wcodes, int64_t ldwc,
+                       const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int ganet_linear8_fwd(int64_t M, int64_t N, int64_t K, int32_t type, const void* x, int64_t ldx, int32_t wtype, const void* w,
+                      int64_t ldw, const void* bias, int32_t btype, void* y, void* rows8, void* weight8, void* tweight8, void* stream);
+size_t ganet_linear8_bwd_workspace(int64_t M, int64_t N, int64_t K, int32_t type);
+int ganet_linear8_bwd(int64_t M, int64_t N, int64_t K, int32_t type, const void* g, int64_t ldg, const void* rows8,
+                      const void* tweight8, void* dx, void* dW, void* db, int32_t wtype, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 /* Optional per-kernel timing (bench/profiling only). The caller owns a GanetProfile object and binds it to the
  * calling thread; from then on every instrumented launch this thread makes whose kernel id is in `mask` is bracketed by
