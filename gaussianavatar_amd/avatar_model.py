@@ -56,7 +56,7 @@ def default_params(**overrides):
         num_points=200_000, num_frames=16, image_width=1024, image_height=1024)
     net = SimpleNamespace(c_pose=64, c_geom=64, hsize=128, nf=32, up_mode="upconv", use_dropout=0,
                           pos_encoding=0, num_emb_freqs=6, posemb_incl_input=0, geom_layer_type="conv",
-                          gaussian_kernel_size=5)
+                          gaussian_kernel_size=5, decoder_norm="batch", decoder_bits8=0)
     epochs = 200
     opt = SimpleNamespace(epochs=epochs, lambda_dssim=0.2, lambda_scale=3e-2, lambda_lpips=0.2,
                           lambda_pose=10, lambda_rgl=1e1, log_iter=2000, lpips_start_iter=30,
@@ -270,7 +270,8 @@ class AvatarModel:
         np_ = self.net_parms
         self.net = POP_no_unet(c_geom=np_.c_geom, geom_layer_type=np_.geom_layer_type, nf=np_.nf,
                                hsize=np_.hsize, up_mode=np_.up_mode, use_dropout=bool(np_.use_dropout),
-                               uv_feat_dim=2).to(self.device)
+                               uv_feat_dim=2, decoder_norm=getattr(np_, "decoder_norm", "batch"),
+                               decoder_bits8=bool(getattr(np_, "decoder_bits8", 0))).to(self.device)
         S_in = self.model_parms.inp_posmap_size
         geo = torch.ones(1, np_.c_geom, S_in, S_in).normal_(mean=0.0, std=0.01).float().to(self.device)
         if geo.is_cuda and np_.c_geom == 64 and S_in % 64 == 0:

@@ -675,7 +675,7 @@ def _decoder_modules(dec):
 
 
 def decoder_supported(dec, x) -> bool:
-    if not (x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and not dec.use_relu
+    if not (x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and not dec.use_relu and dec.norm == "batch" and not dec.bits8
             and dec.hsize == 128 and dec.in_size <= _K1_PAD and x.shape[1] in (dec.in_size, _K1_PAD)):
         return False
     training = dec.training

@@ -27,7 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import fused
+from . import fused, rows8
 
 
 def uv_to_grid(uv_idx_map: torch.Tensor, resolution: int) -> torch.Tensor:
@@ -62,12 +62,20 @@ class GeomConvLayers(nn.Module):
 class ShapeDecoder(nn.Module):
     """Trunk of 5 layers with a DeepSDF-style skip into layer 5, then three 3-layer heads:
     position residual (conv6/7/8), scale (conv6N/7N/8N, sigmoid), colour (conv6SH/7SH/8SH,
-    sigmoid). BatchNorm (batch statistics) + softplus after every hidden layer."""
+    sigmoid). BatchNorm (batch statistics) + softplus after every hidden layer.
+
+    norm="layer": LayerNorm over the channels of a point instead (parameters ln1 ..): no statistics over the rows, so a rank's
+    share of them needs no exchange, and evaluation is the same function as training. bits8: the hidden layers multiply in 8-bit
+    floating point (rows8.linear8) and keep 8 bits of every activation for the backward pass; the three output layers stay in
+    the rows' own type."""
 
     HEADS = ("", "N", "SH")
 
-    def __init__(self, in_size, hsize=256, actv_fn="softplus"):
+    def __init__(self, in_size, hsize=256, actv_fn="softplus", norm="batch", bits8=False):
         super().__init__()
+        if norm not in ("batch", "layer"):
+            raise ValueError(f"ShapeDecoder: norm {norm!r} (known: batch, layer)")
+        self.norm, self.bits8 = norm, bool(bits8)
         self.hsize = hsize
         self.in_size = in_size
         h = hsize
@@ -83,7 +91,10 @@ class ShapeDecoder(nn.Module):
             ci, co = dims[name]
             setattr(self, name, nn.Conv1d(ci, co, 1))
         for name in ("bn1", "bn2", "bn3", "bn4", "bn5", "bn6", "bn7", "bn6N", "bn7N", "bn6SH", "bn7SH"):
-            setattr(self, name, nn.BatchNorm1d(h))
+            if norm == "batch":
+                setattr(self, name, nn.BatchNorm1d(h))
+            else:
+                setattr(self, name.replace("bn", "ln"), nn.LayerNorm(h))
         self.use_relu = actv_fn == "relu"
 
     def _layer(self, x, conv: str, bn: str):
@@ -91,12 +102,15 @@ class ShapeDecoder(nn.Module):
         # BatchNorm(batch statistics)+softplus kernel pair (gaussianavatar_amd/fused.py);
         # on the CPU the same calls reduce to F.linear / BatchNorm1d / softplus
         c = getattr(self, conv)
-        y = fused.linear(x, c.weight.squeeze(-1), c.bias)
-        return fused.batchnorm_act(y, getattr(self, bn), "relu" if self.use_relu else "softplus")
+        act = "relu" if self.use_relu else "softplus"
+        y = (rows8.linear8 if self.bits8 else fused.linear)(x, c.weight.squeeze(-1), c.bias)
+        if self.norm == "layer":
+            return fused.layernorm_act(y, getattr(self, bn.replace("bn", "ln")), act, checkpoint8=self.bits8)
+        return fused.batchnorm_act(y, getattr(self, bn), act)
 
     def _out(self, x, conv: str):
         c = getattr(self, conv)
-        return fused.linear(x, c.weight.squeeze(-1), c.bias)
+        return fused.linear(x, c.weight.squeeze(-1), c.bias, checkpoint8=self.bits8)
 
     def forward_points(self, x, raw_heads: bool = False, m_global=None):
         """x [M, in_size] -> (residual [M,3], scale [M,1], colour [M,3]); with raw_heads the scale and
@@ -109,7 +123,7 @@ class ShapeDecoder(nn.Module):
             # epilogue); the per-layer formulation below is the CPU / unsupported-shape path
             r, s, c = fused.decoder_mlp(self, x, m_global)
             return r, act(s), act(c)
-        if m_global is not None and int(m_global) != x.shape[0] and self.training:
+        if m_global is not None and int(m_global) != x.shape[0] and self.training and self.norm == "batch":
             # (evaluation mode normalises with the running statistics: nothing to synchronise, the per-layer
             # formulation below serves a rank's share of the rows as it is)
             raise NotImplementedError("synchronised BatchNorm statistics need the fused decoder path "
@@ -239,7 +253,7 @@ class UnetNoCond5DS(nn.Module):
 
 class POP_no_unet(nn.Module):
     def __init__(self, c_geom=64, geom_layer_type="conv", nf=64, hsize=256, up_mode="upconv",
-                 use_dropout=False, uv_feat_dim=2):
+                 use_dropout=False, uv_feat_dim=2, decoder_norm="batch", decoder_bits8=False):
         super().__init__()
         self.geom_layer_type = geom_layer_type
         if geom_layer_type == "conv":
@@ -248,7 +262,8 @@ class POP_no_unet(nn.Module):
             self.geom_proc_layers = UnetNoCond5DS(c_geom, c_geom, nf, up_mode, use_dropout)
         elif geom_layer_type is not None:
             raise NotImplementedError(f"geom_layer_type={geom_layer_type!r} (the reference default is 'conv')")
-        self.decoder = ShapeDecoder(in_size=uv_feat_dim + c_geom, hsize=hsize, actv_fn="softplus")
+        self.decoder = ShapeDecoder(in_size=uv_feat_dim + c_geom, hsize=hsize, actv_fn="softplus",
+                                    norm=decoder_norm, bits8=decoder_bits8)
 
     @staticmethod
     def _is_broadcast(t: torch.Tensor) -> bool:

@@ -1,0 +1,414 @@
+"""8-bit rows, weights, products and weight gradients on the GPU against 64-bit arithmetic (tests/rows8_oracle.py).
+
+Tolerances. u = 2^-24 is half a step of fp32. A sum of n terms in fp32, in any order, is off by at most n u sum|terms|. The 8-bit
+matrix instructions first add products in groups of eight adjacent k, each cut to a multiple of 2^-13 of the group's largest power of two
+(observed: 2^16 + 2^3 keeps the 2^3, 2^16 + 2^2 gives 2^16, if both lie in one group of eight; in different groups 2^16 + 2^-7 is exact). The
+seven others of a group lose less than one such unit each, the largest loses nothing: at most 7 2^-13 of the largest, summed over the
+groups. (The first version of this bound took 2^-14 of sum|terms| for the whole step, which a group of one large and seven small products
+exceeds.) Rounding the result adds half a step of its type."""
+import pytest
+import torch
+
+from tests import rows8_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def spread(M, K, dtype, seed, scale=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, K, generator=gen) * torch.exp(0.8 * torch.randn(1, K, generator=gen)) + 0.3 * torch.randn(1, K, generator=gen)
+    return (x * scale).to(dtype).cuda()
+
+
+def assert_same(got, want):
+    got, want = got.double().cpu(), want.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    keep = ~torch.isnan(want)
+    assert torch.equal(got[keep], want[keep])
+
+
+# ---------------------------------------------------------------------------------------------- rows and weights
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 15), (5, 16), (7, 17), (2, 127), (4, 128), (3, 129), (9, 300), (2, 2047), (3, 2049), (1, 8192), (0, 40), (4097, 66)])
+def test_rows_equal_their_definition(M, K, dtype, fmt):
+    from gaussianavatar_amd import rows8
+    x = spread(M, K, dtype, M + K)
+    r = rows8.quantize8(x, fmt)
+    v, e = oracle.rows(x.cpu(), fmt)
+    assert torch.equal(r.exps[:, :e.shape[1]].cpu().long() - 127, e)
+    most = torch.finfo(dtype).max
+    assert_same(r.dequantize(dtype), v.clamp(-most, most).to(dtype))
+    assert not r.codes[:, K:].float().any() and r.codes.shape[1] % 16 == 0
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+def test_rows_of_special_values(fmt):
+    from gaussianavatar_amd import rows8
+    from tests.test_rows8_cpu import special_rows
+    x = special_rows(fmt)
+    r = rows8.quantize8(x.cuda(), fmt)
+    v, e = oracle.rows(x, fmt)
+    assert torch.equal(r.exps[:, :2].cpu().long() - 127, e)
+    assert_same(r.dequantize(), v.clamp(-3.4028234663852886e38, 3.4028234663852886e38) if fmt == "e4m3" else v)
+    big = torch.tensor([[65504.0, 1.0, -65504.0]], device="cuda", dtype=torch.float16)
+    assert rows8.quantize8(big, fmt).dequantize(torch.float16).abs().max() == 65504
+
+
+def test_rows_of_strided_and_shaped_tensors():
+    from gaussianavatar_amd import rows8
+    base = spread(70, 400, torch.bfloat16, 3)
+    for x in (base[:, 3:260], base[::3, 1:130], base.t()[:200], base[5].expand(6, 400), base.view(7, 10, 400), base[0], base[:1, 7:]):
+        r = rows8.quantize8(x)
+        v, _ = oracle.rows(x.cpu().reshape(-1, x.shape[-1]))
+        assert r.dequantize().shape == x.shape
+        assert_same(r.dequantize().reshape(v.shape), v)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,K", [(1, 1), (3, 130), (128, 128), (129, 127), (300, 200), (17, 1000), (513, 48)])
+def test_weights_equal_their_definition(N, K, dtype):
+    from gaussianavatar_amd import rows8
+    w = spread(N, K + 5, dtype, N * K)[:, 2:2 + K]
+    w8 = rows8.quantize8_weight(w, transposed=True)
+    v, e = oracle.weight(w.cpu())
+    assert torch.equal(w8.exps[:, :e.shape[1]].cpu().long() - 127, e)
+    assert_same(w8.dequantize(), v)
+    assert_same(w8.transposed().dequantize(), v.t())
+    assert not w8.codes[:, K:].float().any() and not w8.t_codes[:, N:].float().any()
+    only = rows8.quantize8_weight(w)
+    assert torch.equal(only.codes.view(torch.uint8), w8.codes.view(torch.uint8))
+
+
+# ---------------------------------------------------------------------------------------------- products
+
+
+def assert_product(y, x, w, b, dtype):
+    """y against x w^T + b (64 bits), by the bound of the sum and the type's rounding."""
+    want, size = x @ w.t(), x.abs() @ w.abs().t()
+    if b is not None:
+        want, size = want + b, size + b.abs()
+    tol = (x.shape[1] + 2) * U * size
+    if dtype != torch.float32:
+        pad = (0, -x.shape[1] % 8)
+        groups = zip(torch.nn.functional.pad(x.abs(), pad).split(8, 1), torch.nn.functional.pad(w.abs(), pad).split(8, 1))
+        for p, q in groups:
+            tol += 7 * 2.0 ** -13 * torch.stack([p[:, k:k + 1] * q[None, :, k] for k in range(8)]).amax(0)
+    tol = tol + oracle.half_step(dtype) * want.abs() + torch.finfo(dtype).smallest_normal * 2.0 ** -8
+    off = (y.double().cpu() - want).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+SHAPES = [(1, 1, 1), (1, 17, 130), (1, 4096, 1024), (5, 33, 16), (16, 48, 129), (17, 250, 384), (31, 16, 2100), (32, 130, 640),
+          (33, 64, 127), (45, 231, 1000), (64, 3, 128), (127, 129, 255), (130, 128, 66), (300, 1, 300), (1000, 500, 260)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_products_equal_the_formula(M, N, K, dtype):
+    from gaussianavatar_amd import rows8
+    x, w = spread(M, K, dtype, M + N), spread(N, K, dtype, N + K, K ** -0.5)
+    b = spread(1, N, dtype, 5)[0]
+    w8 = rows8.quantize8_weight(w)
+    xo, wo = oracle.rows(x.cpu())[0], oracle.weight(w.cpu())[0]
+    assert_product(rows8.linear8(x, w8, b), xo, wo, b.double().cpu(), dtype)
+    y = rows8.matmul8(rows8.quantize8(x), w8, None, dtype)
+    assert_product(y, xo, wo, None, dtype)
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(4096, 4096, 300, torch.bfloat16), (4100, 4090, 640, torch.float16), (5000, 3900, 129, torch.bfloat16)])
+def test_products_on_the_large_tiles(M, N, K, dtype):
+    """256 x 256 tiles: inside the matrix, past its rows, past its columns, an odd number of blocks; a sample of rows against 64 bits."""
+    from gaussianavatar_amd import rows8
+    x, w, b = spread(M, K, dtype, 1), spread(N, K, dtype, 2, K ** -0.5), spread(1, N, dtype, 3)[0]
+    y = rows8.linear8(x, rows8.quantize8_weight(w), b)
+    at = torch.cat([torch.arange(0, M, 97), torch.arange(M - 40, M)])
+    assert_product(y[at.cuda()], oracle.rows(x.cpu()[at])[0], oracle.weight(w.cpu())[0], b.double().cpu(), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [7, 29, 150])
+def test_products_of_e5m2_rows_and_other_result_types(M, dtype):
+    from gaussianavatar_amd import rows8
+    x, w = spread(M, 333, torch.float32, 8), spread(77, 333, torch.bfloat16, 9, 0.05)
+    xo, wo = oracle.rows(x.cpu(), "e5m2")[0], oracle.weight(w.cpu())[0]
+    b = spread(1, 77, torch.float16, 4)[0]
+    y = rows8.matmul8(rows8.quantize8(x, "e5m2"), rows8.quantize8_weight(w), b, dtype)
+    assert_product(y, xo, wo, b.double().cpu(), dtype)
+
+
+def test_few_rows_are_packed_as_the_rows_kernel_packs_them():
+    """The same codes either way, so the same bits."""
+    from gaussianavatar_amd import rows8
+    for dtype in TYPES:
+        for M, K in ((1, 700), (16, 130), (20, 1029), (32, 64)):
+            x, w8 = spread(M, K, dtype, M), rows8.quantize8_weight(spread(90, K, dtype, 2))
+            assert torch.equal(rows8.linear8(x, w8), rows8.matmul8(rows8.quantize8(x), w8, None, dtype))
+
+
+def test_a_nan_stays_in_its_row_and_an_infinity_is_one():
+    from gaussianavatar_amd import rows8
+    for M in (4, 200):
+        x = spread(M, 200, torch.bfloat16, 1)
+        x[1, 7], x[3, 150] = float("nan"), float("inf")
+        y = rows8.linear8(x, rows8.quantize8_weight(spread(70, 200, torch.bfloat16, 2)))
+        bad = torch.isnan(y).all(1)
+        assert bad[1] and bad[3] and int(torch.isnan(y).any(1).sum()) == 2
+
+
+def test_an_odd_result_row_is_written_whole_and_nothing_beyond_it():
+    from gaussianavatar_amd import _native, rows8
+    M, N, K = 70, 37, 100
+    r, w8 = rows8.quantize8(spread(M, K, torch.bfloat16, 1)), rows8.quantize8_weight(spread(N, K, torch.bfloat16, 2))
+    big = torch.full((M + 2, N + 6), 7.0, dtype=torch.bfloat16, device="cuda")
+    y = big[1:M + 1, 3:N + 3]
+    rows8._call(big.device, _native.ganet().ganet_gemm8, M, N, K, 0, r.codes.data_ptr(), r.codes.stride(0), r.exps.data_ptr(), r.exps.stride(0),
+                w8.codes.data_ptr(), w8.codes.stride(0), w8.exps.data_ptr(), w8.exps.stride(0), None, 0, y.data_ptr(), big.stride(0), 1)
+    assert torch.equal(y, rows8.matmul8(r, w8, None, torch.bfloat16))
+    big[1:M + 1, 3:N + 3] = 7.0
+    assert (big == 7.0).all()
+
+
+# ---------------------------------------------------------------------------------------------- weight gradients
+
+
+def assert_wgrad(dW, db, g, v, dtype, pieces=3):
+    want, size = g.t() @ v, g.abs().t() @ v.abs()
+    n = pieces * g.shape[0] + 600                                # products of a sum, and the ranges' sums
+    off, tol = (dW.double().cpu() - want).abs(), n * U * size + oracle.half_step(dtype) * want.abs() + torch.finfo(dtype).smallest_normal
+    assert (off <= tol).all(), float((off / tol).max())
+    want, size = g.sum(0), g.abs().sum(0)
+    off, tol = (db.double().cpu() - want).abs(), n * U * size + oracle.half_step(dtype) * want.abs() + torch.finfo(dtype).smallest_normal
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (2, 17, 130), (31, 128, 128), (32, 3, 66), (33, 129, 16), (777, 17, 300), (130, 260, 257), (1500, 128, 194)])
+def test_weight_gradients_equal_the_formula(M, N, K, dtype, fmt):
+    from gaussianavatar_amd import rows8
+    x, g = spread(M, K, dtype, M), spread(M, N, dtype, N)
+    dW, db = rows8.wgrad8(g, rows8.quantize8(x, fmt))
+    assert_wgrad(dW, db, g.double().cpu(), oracle.rows(x.cpu(), fmt)[0], dtype)
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(4096, 1024, 1024, torch.bfloat16), (4099, 1030, 1100, torch.bfloat16), (4096, 1024, 1000, torch.float32),
+                                         (4133, 1022, 1024, torch.float16)])
+def test_weight_gradients_on_the_large_tiles(M, N, K, dtype):
+    from gaussianavatar_amd import rows8
+    x, g = spread(M, K, dtype, 1), spread(M, N, dtype, 2)
+    dW, db = rows8.wgrad8(g, rows8.quantize8(x))
+    assert_wgrad(dW, db, g.double().cpu(), oracle.rows(x.cpu())[0], dtype)
+
+
+def test_an_fp32_weight_gradient_over_many_rows_is_fp32_accurate():
+    """262,144 rows: the error of sums of this length in fp32 grows like its root, not like the bound: 2^-24 sqrt(n) of the norm, taken
+    four times."""
+    from gaussianavatar_amd import rows8
+    x, g = spread(262144, 72, torch.float32, 1), spread(262144, 40, torch.float32, 2)
+    dW, db = rows8.wgrad8(g, rows8.quantize8(x))
+    v, gd = oracle.rows(x.cpu())[0], g.double().cpu()
+    want = gd.t() @ v
+    assert float((dW.double().cpu() - want).norm() / want.norm()) <= 4 * U * 512
+    assert float((db.double().cpu() - gd.sum(0)).norm() / gd.sum(0).norm()) <= 4 * U * 512
+
+
+def test_weight_gradient_of_no_rows_strided_gradients_and_other_types():
+    from gaussianavatar_amd import rows8
+    r = rows8.quantize8(torch.randn(0, 70, device="cuda"))
+    dW, db = rows8.wgrad8(torch.randn(0, 9, device="cuda"), r)
+    assert dW.shape == (9, 70) and not dW.any() and not db.any()
+    x = spread(100, 90, torch.bfloat16, 1)
+    r, v = rows8.quantize8(x), oracle.rows(x.cpu())[0]
+    base = spread(100, 200, torch.float32, 2)
+    for g in (base[:, 7:60], base.t().contiguous().t()[:, :33], base[:1].expand(100, 200), base[:, 1:2]):
+        dW, db = rows8.wgrad8(g, r, torch.bfloat16)
+        assert dW.dtype == torch.bfloat16
+        assert_wgrad(dW, db, g.double().cpu(), v, torch.bfloat16)
+    g3 = spread(100, 8, torch.bfloat16, 3).view(4, 25, 8)
+    dW, _ = rows8.wgrad8(g3, rows8.quantize8(x.view(4, 25, 90)), torch.float32)
+    assert_wgrad(dW, g3.double().sum((0, 1)), g3.double().cpu().reshape(100, 8), v, torch.float32)
+
+
+def test_the_same_inputs_give_the_same_bits():
+    from gaussianavatar_amd import rows8
+    x, g = spread(20000, 100, torch.float32, 1), spread(20000, 60, torch.float32, 2)
+    first = rows8.wgrad8(g, rows8.quantize8(x))
+    for _ in range(3):
+        again = rows8.wgrad8(g, rows8.quantize8(x))
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# ---------------------------------------------------------------------------------------------- the layer
+
+
+@pytest.mark.parametrize("xt,wt", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32),
+                                   (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("lead,N,K", [((1,), 5, 40), ((3, 7), 130, 66), ((300,), 128, 200), ((0,), 4, 20)])
+def test_linear8_and_its_gradients(lead, N, K, xt, wt):
+    from gaussianavatar_amd import rows8
+    M = int(torch.tensor(lead).prod())
+    x = spread(max(M, 1), K, xt, 1)[:M].reshape(*lead, K).requires_grad_(True)
+    w = spread(N, K, wt, 2, K ** -0.5).requires_grad_(True)
+    b = spread(1, N, wt, 3)[0].requires_grad_(True)
+    g = spread(max(M, 1), N, xt, 4)[:M].reshape(*lead, N)
+    y = rows8.linear8(x, w, b)
+    assert y.shape == (*lead, N) and y.dtype == xt
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    assert (dx.dtype, dw.dtype, db.dtype) == (xt, wt, wt) and dx.shape == x.shape
+    if M == 0:
+        assert not dw.any() and not db.any()
+        return
+    xo, wo = oracle.rows(x.detach().cpu().reshape(M, K))[0], oracle.weight(w.detach().cpu())[0]
+    g2 = g.cpu().reshape(M, N)
+    assert_product(y.detach().reshape(M, N), xo, wo, b.detach().double().cpu(), xt)
+    assert_product(dx.reshape(M, K), oracle.rows(g2)[0], wo.t(), None, xt)
+    assert_wgrad(dw, db, g2.double(), xo, wt)
+
+
+def test_linear8_gradients_equal_exact_differences():
+    """Small whole numbers are their own codes and their sums exact: differences of the loss are the gradient."""
+    from gaussianavatar_amd import rows8
+    gen = torch.Generator().manual_seed(2)
+    ints = lambda *s: torch.randint(-3, 4, s, generator=gen).float().cuda()
+    x, w, b, g = ints(150, 140).requires_grad_(True), ints(9, 140).requires_grad_(True), ints(9).requires_grad_(True), ints(150, 9)
+    loss = lambda *a: (rows8.linear8(*a).double() * g).sum()
+    grads = torch.autograd.grad(loss(x, w, b), (x, w, b))
+    for k in range(3):
+        args = [a.detach() for a in (x, w, b)]
+        d = torch.randint(-1, 2, args[k].shape, generator=gen).float().cuda()
+        up, down = list(args), list(args)
+        up[k], down[k] = args[k] + d, args[k] - d
+        assert float((loss(*up) - loss(*down)) / 2) == float((grads[k].double() * d).sum())
+
+
+def test_linear8_gives_only_the_gradients_asked_for():
+    from gaussianavatar_amd import rows8
+    x, w, b = spread(40, 30, torch.float32, 1), spread(20, 30, torch.float32, 2), spread(1, 20, torch.float32, 3)[0]
+    full = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(rows8.linear8(*full).sum(), full)
+    for k in range(3):
+        args = [t.clone().requires_grad_(i == k) for i, t in enumerate((x, w, b))]
+        rows8.linear8(*args).sum().backward()
+        assert torch.equal(args[k].grad, want[k]) and all(a.grad is None for i, a in enumerate(args) if i != k)
+
+
+def test_linear_with_an_8_bit_checkpoint():
+    from gaussianavatar_amd import fused
+    x, w, b = (t.requires_grad_(True) for t in (spread(500, 66, torch.float32, 1), spread(40, 66, torch.float32, 2), spread(1, 40, torch.float32, 3)[0]))
+    g = spread(500, 40, torch.float32, 4)
+    y, full = fused.linear(x, w, b, checkpoint8=True), fused.linear(x, w, b)
+    assert torch.equal(y, full)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    fx = torch.autograd.grad(full, x, g)[0]
+    assert torch.equal(dx, fx)
+    assert_wgrad(dw, db, g.double().cpu(), oracle.rows(x.detach().cpu())[0], torch.float32)
+
+
+def test_held_weights_do_not_train():
+    from gaussianavatar_amd import rows8
+    w8 = rows8.quantize8_weight(spread(8, 32, torch.float32, 1))
+    x = spread(4, 32, torch.float32, 2).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="evaluation"):
+        rows8.linear8(x, w8)
+    with torch.no_grad():
+        assert not rows8.linear8(x, w8).requires_grad
+    with pytest.raises(ValueError):
+        rows8.linear8(x.detach().cpu(), w8)
+
+
+# ---------------------------------------------------------------------------------------------- streams and graphs
+
+
+def test_calls_on_two_streams_do_not_share_anything():
+    from gaussianavatar_amd import rows8
+    w8 = rows8.quantize8_weight(spread(300, 500, torch.bfloat16, 1))
+    xs = [spread(200, 500, torch.bfloat16, k) for k in range(6)]
+    want = [rows8.linear8(x, w8) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for k, x in enumerate(xs):
+        with torch.cuda.stream(streams[k % 2]):
+            got.append(rows8.linear8(x, w8))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_training_step_of_the_operators_together_replays_from_a_graph():
+    """linear8 -> layer norm kept in 8 bits -> linear8, forward and backward, captured once and replayed on new inputs, with eager work
+    between the replays."""
+    from gaussianavatar_amd import fused, rows8
+    M = 500
+    w1, w2 = spread(130, 66, torch.float32, 1, 0.1).requires_grad_(True), spread(40, 130, torch.float32, 2, 0.1).requires_grad_(True)
+    ln = torch.nn.LayerNorm(130, device="cuda")
+    params = (w1, ln.weight, ln.bias, w2)
+
+    def step(x, g):
+        h = fused.layernorm_act(rows8.linear8(x, w1), ln, "softplus", checkpoint8=True)
+        y = rows8.linear8(h, w2)
+        return (y.detach(), *torch.autograd.grad(y, params, g))
+
+    x, g = spread(M, 66, torch.float32, 3), spread(M, 40, torch.float32, 4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(x, g)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, g)
+    for k in range(4):
+        x.copy_(spread(M, 66, torch.float32, 10 + k))
+        g.copy_(spread(M, 40, torch.float32, 20 + k))
+        want = step(x.clone(), g.clone())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+# ---------------------------------------------------------------------------------------------- the decoder
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+def test_decoder_with_layer_norm_equals_its_cpu_form(bits8):
+    """The whole decoder, kernels against torch operations on the CPU: outputs and every parameter's gradient. fp32 differs by sums and
+    functions in another order: a few 2^-24 of the largest value a layer, through seven layers, taken as 2^-14 of each tensor's
+    largest. With 8 bits a value next to the border of two codes may go the other way, by 2^-3 of itself, and the layers behind hand it on:
+    the comparison is one of norms, at half of the format's own rounding, 2^-5."""
+    from gaussianavatar_amd.network import ShapeDecoder
+    torch.manual_seed(0)
+    cpu = ShapeDecoder(66, 64, norm="layer", bits8=bits8)
+    gpu = ShapeDecoder(66, 64, norm="layer", bits8=bits8).cuda()
+    gpu.load_state_dict(cpu.state_dict())
+    x = torch.randn(1000, 66)
+    outs = []
+    for net, dev in ((cpu, "cpu"), (gpu, "cuda")):
+        y = torch.cat(net.forward_points(x.to(dev), raw_heads=True), 1)
+        (y * torch.linspace(-1, 1, 7, device=dev)).square().mean().backward()
+        outs.append([y.detach().cpu()] + [p.grad.cpu() for p in net.parameters()])
+    for a, b in zip(*outs):
+        if bits8:
+            assert float((a - b).norm()) <= 2 ** -5 * float(a.norm()) + 1e-7
+        else:
+            assert float((a - b).abs().max()) <= 2 ** -14 * float(a.abs().max()) + 1e-7
+
+
+def test_avatar_model_trains_with_the_8_bit_layer_norm_decoder():
+    from gaussianavatar_amd.avatar_model import AvatarModel, collate_frames, default_params
+    torch.manual_seed(0)
+    mp, npar, op = default_params(batch_size=2, num_points=3000, query_posmap_size=64, inp_posmap_size=32, image_width=128, image_height=128,
+                                  num_frames=4, decoder_norm="layer", decoder_bits8=1)
+    model = AvatarModel(mp, npar, op, train=True)
+    model.training_setup()
+    batch = collate_frames([model.train_dataset[i] for i in range(2)], "cuda")
+    image, points, offset_loss, geo_loss, scale_loss = model.train_stage1(batch, 50)
+    (image.mean() + offset_loss + geo_loss + scale_loss).backward()
+    grads = [p.grad for n, p in model.net.decoder.named_parameters()]
+    assert all(g is not None and torch.isfinite(g).all() for g in grads) and any(g.abs().max() > 0 for g in grads)
+    model.step(1)
