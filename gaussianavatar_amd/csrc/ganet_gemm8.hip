@@ -146,7 +146,8 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
   const int T = tiles_m * tiles_n, q = T / 8, rem = T % 8, xcd = blockIdx.x % 8;
   const int t = xcd * q + (xcd < rem ? xcd : rem) + blockIdx.x / 8;
   const int group = t / (8 * tiles_n), gm = min(8, tiles_m - group * 8), in = t - group * 8 * tiles_n;
-  const int64_t m0 = (int64_t)(group * 8 + in % gm) * TM, n0 = (int64_t)(in / gm) * TN;
+  // (in scalar registers: the divisions are done in vector ones)
+  const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(group * 8 + in % gm) * TM, n0 = (int64_t)__builtin_amdgcn_readfirstlane(in / gm) * TN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = (wave & 1) * 32 * MT, wn = (wave >> 1) * 32 * NT;
   const int64_t kend = (o.K + 15) / 16 * 16;

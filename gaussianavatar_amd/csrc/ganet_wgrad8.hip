@@ -255,7 +255,9 @@ wgrad8_kernel(Job o) {
   const int tiles = o.tiles_n * o.tiles_k, T0 = tiles * o.splits, q = T0 / 8, rem = T0 % 8, xcd = blockIdx.x % 8;
   const int t = xcd * q + (xcd < rem ? xcd : rem) + blockIdx.x / 8, in_split = t % tiles;
   const int group = in_split / (4 * o.tiles_k), gn = min(4, o.tiles_n - group * 4), in = in_split - group * 4 * o.tiles_k;
-  const Where w{group * 4 + in % gn, in / gn, t / tiles};
+  // (in scalar registers: the divisions are done in vector ones)
+  const Where w{__builtin_amdgcn_readfirstlane(group * 4 + in % gn), __builtin_amdgcn_readfirstlane(in / gn),
+                __builtin_amdgcn_readfirstlane(t / tiles)};
   if ((int64_t)(w.tn + 1) * 64 * T <= o.N) wgrad8_tile<FMT, G, T, true>(o, w, s_mem);
   else wgrad8_tile<FMT, G, T, false>(o, w, s_mem);
 }
