@@ -17,8 +17,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-__device__ uint4 g_zeros[1];        // what lanes past the end of a row read
-
 __device__ __forceinline__ i32x8 join(const uint4& a, const uint4& b) {
   i32x8 r;
   r[0] = (int)a.x; r[1] = (int)a.y; r[2] = (int)a.z; r[3] = (int)a.w;
@@ -40,52 +38,30 @@ struct Operands {
 // The instruction writes lanes in order, so the swizzle is in the global address that a lane fetches.
 //
 // Two LDS buffers and two register sets of fragments, half a block (64 codes) each:
-//     read half 1 of step k          | multiply half 0 of step k
-//     step k + 1 landed? barrier     |
-//     fetch step k + 2, read half 0 of step k + 1 | multiply half 1 of step k
-// so that neither LDS nor memory latency stands between two multiplications, and a fetch has a whole step to arrive.
+//     multiply half 0 of step k     and, between the multiplications, read half 1 of step k
+//     step k + 1 landed? barrier
+//     multiply half 1 of step k     and, between the multiplications, read half 0 of step k + 1 and fetch step k + 2
+// so that neither LDS nor memory latency stands between two multiplications, and a fetch has a whole step to arrive. A wave issues in
+// order: what stands behind sixteen multiplications waits for fifteen of them and then runs beside the last one only. So every
+// multiplication is followed by its share of the reads and fetches, and nothing crosses it (8192 x 4096 x 8192: 2.0 PFLOP/s with the
+// reads and fetches in one go; 2.6 without the fetches).
+//
+// No branch in the loop: rows past the matrix fetch its last row (results nobody stores), chunks past a row's codes fetch its last
+// chunk and are zeroed in x's fragments, which only the last step needs.
 //
 // The fetches are issued from inline assembly: they have no register result, and the compiler, which cannot tell the two buffers
 // apart, would otherwise wait for the step in flight before it reads the one that has landed. Every wait for them is the explicit one
 // below; nothing else of this loop may leave a vector load pending across it (the scale bytes are taken before the fetches).
-__device__ __forceinline__ void fetch16(const uint8_t* p, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
-}
 __device__ __forceinline__ void fetch16(const uint8_t* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
 
-// Rows of one operand's tile. Instruction i of a wave fetches rows 32 i + 8 wave + lane / 8; the swizzle does not depend on i, so
-// inside the matrix one lane offset serves all of them.
-template <int ROWS>
-__device__ __forceinline__ void stage(const uint8_t* tile, int64_t ld, int64_t rows, int64_t k0, int chunks, unsigned lds) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int r = wave * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-  const uint8_t* src = tile + k0;
-  lds += wave * 1024;
-  if (rows >= ROWS && chunks == 8) {
-    const unsigned off = (unsigned)(r * (unsigned)ld + c * 16);
-#pragma unroll
-    for (int i = 0; i < ROWS / 32; ++i) fetch16(src + i * 32 * ld, off, lds + i * 4096);
-  } else {
-    // the matrix ends in this tile: rows past its end give results that nobody stores, chunks past a row's end are zero
-#pragma unroll 1
-    for (int i = 0; i < ROWS / 32; ++i) {
-      const int64_t row = min((int64_t)(r + i * 32), rows - 1);
-      fetch16(c < chunks ? src + row * ld + c * 16 : reinterpret_cast<const uint8_t*>(g_zeros), lds + i * 4096);
-    }
-  }
-}
-
-// One half block of a wave's rows, 32 codes per lane and 32 rows: chunks 2 (lane / 32) and the next of the half's four.
-template <int TILES>
-__device__ __forceinline__ void read_half(const uint8_t* lds, int lane, int half, i32x8 (&f)[TILES]) {
-  const int r = lane & 31, c = half * 4 + (lane >> 5) * 2, sw = (r >> 1) & 7;
-  const uint8_t* p0 = lds + r * 128 + (c ^ sw) * 16;
-  const uint8_t* p1 = lds + r * 128 + ((c + 1) ^ sw) * 16;
-#pragma unroll
-  for (int i = 0; i < TILES; ++i)
-    f[i] = join(*reinterpret_cast<const uint4*>(p0 + i * 32 * 128), *reinterpret_cast<const uint4*>(p1 + i * 32 * 128));
+// Chunk h of fragment i of a wave's rows, one half block: a lane holds 32 codes of one of 32 rows, chunks 2 (lane / 32) and the next
+// of the half's four.
+__device__ __forceinline__ void read_chunk(const uint8_t* lds, int lane, int half, int i, int h, i32x8& f) {
+  const int r = lane & 31, c = half * 4 + (lane >> 5) * 2 + h, sw = (r >> 1) & 7;
+  const uint4 v = *reinterpret_cast<const uint4*>(lds + r * 128 + i * 4096 + (c ^ sw) * 16);
+  f[4 * h] = (int)v.x; f[4 * h + 1] = (int)v.y; f[4 * h + 2] = (int)v.z; f[4 * h + 3] = (int)v.w;
 }
 
 // Eight codes (dwords d, d + 1) times 2^e as bf16: exact.
@@ -109,28 +85,35 @@ __device__ __forceinline__ bf16x8 decode8(const i32x8& f, int d, float scale) {
 // group's largest power of two, before they go on in fp32: 1.2e-5 to 2.5e-5 of a result's norm (measured against 64 bits; the older
 // 16-deep instructions are the same). That is below the rounding of a 16-bit result and above that of fp32, so an fp32 result (EXACT)
 // takes the bf16 instructions on decoded codes, at half the rate: error 4e-8 on the same inputs.
-template <int FMT, int MT, int NT, bool EXACT>
-__device__ __forceinline__ void multiply(const i32x8 (&a)[MT], const i32x8 (&b)[NT], const int (&sx)[MT], int sw,
-                                         f32x16 (&acc)[NT][MT]) {
-  if (!EXACT) {
+// between(q) is called behind multiplication q of MULTIPLICATIONS.
+template <bool EXACT, int MT, int NT> constexpr int MULTIPLICATIONS = (EXACT ? 4 : 1) * MT * NT;
+template <int FMT, int MT, int NT, bool EXACT, typename Between>
+__device__ __forceinline__ void multiply(const i32x8 (&a)[MT], const i32x8 (&b)[NT], const int (&sx)[MT], int sw, f32x16 (&acc)[NT][MT],
+                                         Between between) {
+  if constexpr (!EXACT) {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i) {
         acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[j][i], GANET_E4M3, FMT, 0, sw, 0, sx[i]);
-    return;
-  }
+        between(j * MT + i);
+      }
+  } else {
 #pragma unroll
-  for (int d = 0; d < 8; d += 2) {                           // 16 products per instruction: eight codes of a lane
-    bf16x8 x[MT], w[NT];
+    for (int d = 0; d < 4; ++d) {                            // 16 products per instruction: eight codes of a lane
+      bf16x8 x[MT], w[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) x[i] = decode8<FMT>(a[i], d, pow2(sx[i] - 127));
+      for (int i = 0; i < MT; ++i) x[i] = decode8<FMT>(a[i], 2 * d, pow2(sx[i] - 127));
 #pragma unroll
-    for (int j = 0; j < NT; ++j) w[j] = decode8<GANET_E4M3>(b[j], d, pow2(sw - 127));
+      for (int j = 0; j < NT; ++j) w[j] = decode8<GANET_E4M3>(b[j], 2 * d, pow2(sw - 127));
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[j][i], 0, 0, 0);
+        for (int i = 0; i < MT; ++i) {
+          acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[j][i], 0, 0, 0);
+          between((d * NT + j) * MT + i);
+        }
+    }
   }
 }
 
@@ -153,12 +136,22 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
   const int64_t kend = (o.K + 15) / 16 * 16;
   const int KB = (int)((o.K + BLOCK - 1) / BLOCK);
 
-  auto fetch = [&](int kb) {
-    const unsigned lds = lds0 + (kb & 1) * BYTES;
-    const int64_t k0 = (int64_t)kb * BLOCK;
-    const int chunks = (int)min((int64_t)8, (kend - k0) / 16);
-    stage<TM>(o.x + m0 * o.ldx, o.ldx, o.M - m0, k0, chunks, lds);
-    stage<TN>(o.w + n0 * o.ldw, o.ldw, o.N - n0, k0, chunks, lds + TM * 128);
+  // Instruction i of a wave's fetches of an operand: rows 32 i + 8 wave + lane / 8, the lane's chunk. (The swizzle does not depend on i.)
+  const int fr = wave * 8 + (lane >> 3), fc = (lane & 7) ^ ((fr >> 1) & 7);
+  const int last_chunks = (int)((kend - (int64_t)(KB - 1) * BLOCK) / 16);
+  const unsigned last_shift = (unsigned)(min(fc, last_chunks - 1) - fc) * 16u;       // (0, or negative)
+  unsigned offx[2 * MT], offw[2 * NT];
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) offx[i] = (unsigned)min((int64_t)(fr + i * 32), o.M - 1 - m0) * (unsigned)o.ldx + fc * 16;
+#pragma unroll
+  for (int i = 0; i < 2 * NT; ++i) offw[i] = (unsigned)min((int64_t)(fr + i * 32), o.N - 1 - n0) * (unsigned)o.ldw + fc * 16;
+  const uint8_t *xt = o.x + m0 * o.ldx, *wt = o.w + n0 * o.ldw;
+  constexpr int PARTS = 2 * (MT + NT), MULS = MULTIPLICATIONS<EXACT, MT, NT>;
+  auto fetch = [&](int kb, int p) {          // instruction p of PARTS
+    const unsigned lds = lds0 + (kb & 1) * BYTES + wave * 1024;
+    const unsigned shift = kb + 1 == KB ? last_shift : 0u;
+    if (p < 2 * MT) fetch16(xt + (int64_t)kb * BLOCK, offx[p] + shift, lds + p * 4096);
+    else fetch16(wt + (int64_t)kb * BLOCK, offw[p - 2 * MT] + shift, lds + TM * 128 + (p - 2 * MT) * 4096);
   };
   const uint8_t* ex = o.ex + m0 * o.ldex;
   unsigned exo[MT];
@@ -186,8 +179,15 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
 
+  auto read = [&](int kb, int half, i32x8 (&a)[MT], i32x8 (&b)[NT], int p) {       // instruction p of PARTS
+    const uint8_t* lds = s_tiles + (kb & 1) * BYTES;
+    if (p < 2 * MT) read_chunk(lds + wm * 128, lane, half, p >> 1, p & 1, a[p >> 1]);
+    else read_chunk(lds + (TM + wn) * 128, lane, half, (p - 2 * MT) >> 1, p & 1, b[(p - 2 * MT) >> 1]);
+  };
+
   scales(0);
-  fetch(0);
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) fetch(0, p);
   // the sums start at the bias (its loads run beside the first fetch)
   f32x16 acc[NT][MT];
   auto start = [&](auto bias) {
@@ -204,37 +204,59 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
   else GANET_BY_TYPE(o.btype, B, start([&](int64_t n) { return (float)static_cast<const B*>(o.bias)[n]; }));
   landed();
   take_scales(0);
-  if (KB > 1) { scales(1); fetch(1); }
-  read_half<MT>(s_tiles + wm * 128, lane, 0, a0);
-  read_half<NT>(s_tiles + (TM + wn) * 128, lane, 0, b0);
+  if (KB > 1) {
+    scales(1);
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) fetch(1, p);
+  }
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) read(0, 0, a0, b0, p);
   for (int kb = 0; kb + 1 < KB; ++kb) {
-    const uint8_t* lds = s_tiles + (kb & 1) * BYTES;
-    read_half<MT>(lds + wm * 128, lane, 1, a1);
-    read_half<NT>(lds + (TM + wn) * 128, lane, 1, b1);
     __builtin_amdgcn_sched_barrier(0);
-    multiply<FMT, MT, NT, EXACT>(a0, b0, sx, sw, acc);
-    __builtin_amdgcn_sched_barrier(0);
+    multiply<FMT, MT, NT, EXACT>(a0, b0, sx, sw, acc, [&](int q) {
+#pragma unroll
+      for (int p = PARTS * q / MULS; p < PARTS * (q + 1) / MULS; ++p) read(kb, 1, a1, b1, p);
+      __builtin_amdgcn_sched_barrier(0);
+    });
     landed();                                // step kb + 1 is there, and nobody reads this step's buffer any more
     int px[MT];
     const int pw = sw;
 #pragma unroll
     for (int i = 0; i < MT; ++i) px[i] = sx[i];
     take_scales(kb + 1);
-    if (kb + 2 < KB) { scales(kb + 2); fetch(kb + 2); }
-    const uint8_t* next = s_tiles + ((kb + 1) & 1) * BYTES;
-    read_half<MT>(next + wm * 128, lane, 0, a0);
-    read_half<NT>(next + (TM + wn) * 128, lane, 0, b0);
+    const int next = min(kb + 2, KB - 1);    // (behind the last step the last one is fetched again, into the buffer nobody reads)
+    scales(next);
     __builtin_amdgcn_sched_barrier(0);
-    multiply<FMT, MT, NT, EXACT>(a1, b1, px, pw, acc);
-    __builtin_amdgcn_sched_barrier(0);
+    multiply<FMT, MT, NT, EXACT>(a1, b1, px, pw, acc, [&](int q) {
+#pragma unroll
+      for (int p = PARTS * q / MULS; p < PARTS * (q + 1) / MULS; ++p) {
+        read(kb + 1, 0, a0, b0, p);
+        const unsigned lds = lds0 + (kb & 1) * BYTES + wave * 1024;
+        const unsigned shift = next + 1 == KB ? last_shift : 0u;
+        if (p < 2 * MT) fetch16(xt + (int64_t)next * BLOCK, offx[p] + shift, lds + p * 4096);
+        else fetch16(wt + (int64_t)next * BLOCK, offw[p - 2 * MT] + shift, lds + TM * 128 + (p - 2 * MT) * 4096);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
   }
-  {
-    const uint8_t* lds = s_tiles + ((KB - 1) & 1) * BYTES;
-    read_half<MT>(lds + wm * 128, lane, 1, a1);
-    read_half<NT>(lds + (TM + wn) * 128, lane, 1, b1);
-    multiply<FMT, MT, NT, EXACT>(a0, b0, sx, sw, acc);
-    multiply<FMT, MT, NT, EXACT>(a1, b1, sx, sw, acc);
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) read(KB - 1, 1, a1, b1, p);
+  if (last_chunks < 8) {                     // what was fetched past the rows' codes
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool in0 = (lane >> 5) * 2 + h < last_chunks, in1 = 4 + (lane >> 5) * 2 + h < last_chunks;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int d = 4 * h; d < 4 * h + 4; ++d) {
+          a0[i][d] = in0 ? a0[i][d] : 0;
+          a1[i][d] = in1 ? a1[i][d] : 0;
+        }
+    }
   }
+  multiply<FMT, MT, NT, EXACT>(a0, b0, sx, sw, acc, [](int) {});
+  multiply<FMT, MT, NT, EXACT>(a1, b1, sx, sw, acc, [](int) {});
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // (the fetches behind the last step)
   // A lane holds one row m and, four at a time, consecutive columns n. Stored from there, an instruction would touch 32 rows with 16
   // or 32 bytes each; through LDS (rows of 16 bytes more than the tile's: the 32 rows of a write fall into different banks) every
   // row leaves in full 16-byte pieces: 57 -> 8 us per 256 x 256 tile.
@@ -406,8 +428,9 @@ int launch(const Operands& o, hipStream_t stream) {
 }
 
 bool held_ok(int64_t N, int64_t K, const void* c, int64_t ld, const uint8_t* e, int64_t le) {
-  return c && e && ld % 16 == 0 && ld >= pad16(K) && (reinterpret_cast<uintptr_t>(c) & 15) == 0 && le % 4 == 0 &&
-         le >= cdiv(K, BLOCK) && (reinterpret_cast<uintptr_t>(e) & 3) == 0;
+  // (offsets inside a tile of 256 rows are 32 bits)
+  return c && e && ld % 16 == 0 && ld >= pad16(K) && ld <= (1 << 24) && (reinterpret_cast<uintptr_t>(c) & 15) == 0 && le % 4 == 0 &&
+         le >= cdiv(K, BLOCK) && le <= (1 << 24) && (reinterpret_cast<uintptr_t>(e) & 3) == 0;
 }
 
 // Where a buffer of ganet_rows8_bytes / ganet_weight8_bytes keeps its codes and exponents
