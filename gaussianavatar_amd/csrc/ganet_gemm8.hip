@@ -32,35 +32,33 @@ struct Operands {
 };
 
 // ------------------------------------------------------------------------------------------------ tiles through LDS
-// A workgroup of four waves computes 64 MT x 64 NT of y, a wave 32 MT x 32 NT. One step is one block of 128 codes: its rows go
-// from global memory straight into LDS (16 bytes per lane, no registers). A row is 128 bytes = 8 chunks of 16; chunk c of row r lies at
-// position c ^ ((r >> 1) & 7), so that the 16 rows that a quarter of a wave reads at once lie in 16 different 16-byte columns of LDS.
+// A workgroup of four waves computes 64 MT x 64 NT of y, a wave 32 MT x 32 NT. One phase is half a block, 64 codes: its rows go
+// from global memory straight into LDS (16 bytes per lane, no registers). A row of a phase is 64 bytes = 4 chunks of 16; chunk c of row r lies at
+// position c ^ ((r >> 2) & 3), so that the 16 rows that a quarter of a wave reads at once lie in 16 different 16-byte columns of LDS.
 // The instruction writes lanes in order, so the swizzle is in the global address that a lane fetches.
 //
-// Two LDS buffers and two register sets of fragments, half a block (64 codes) each:
-//     multiply half 0 of step k     and, between the multiplications, read half 1 of step k
-//     step k + 1 landed? barrier
-//     multiply half 1 of step k     and, between the multiplications, read half 0 of step k + 1 and fetch step k + 2
-// so that neither LDS nor memory latency stands between two multiplications, and a fetch has a whole step to arrive. A wave issues in
-// order: what stands behind sixteen multiplications waits for fifteen of them and then runs beside the last one only. So every
-// multiplication is followed by its share of the reads and fetches, and nothing crosses it (8192 x 4096 x 8192: 2.0 PFLOP/s with the
-// reads and fetches in one go; 2.6 without the fetches).
+// Four LDS buffers and two register sets of fragments. Phase h:
+//     phase h + 1 has landed; barrier (and everybody has read phase h)
+//     multiply phase h and, between the multiplications, read phase h + 1 and fetch phase h + 4 into the buffer of phase h
+// so that neither LDS nor memory latency stands between two multiplications, and a fetch has three phases to arrive (with whole blocks
+// and two buffers it had two: 8192^3 2.28 PFLOP/s). A wave issues in order: what stands behind sixteen multiplications waits for
+// fifteen of them and then runs beside the last one only. So every multiplication is followed by its share of the reads and
+// fetches, and nothing crosses it (2.16 PFLOP/s with the reads and fetches in one go).
 //
 // No branch in the loop: rows past the matrix fetch its last row (results nobody stores), chunks past a row's codes fetch its last
-// chunk and are zeroed in x's fragments, which only the last step needs.
+// chunk and are zeroed in x's fragments, which only the last block needs; phases past the end fetch the last block again.
 //
-// The fetches are issued from inline assembly: they have no register result, and the compiler, which cannot tell the two buffers
-// apart, would otherwise wait for the step in flight before it reads the one that has landed. Every wait for them is the explicit one
-// below; nothing else of this loop may leave a vector load pending across it (the scale bytes are taken before the fetches).
+// The fetches are issued from inline assembly: they have no register result, and the compiler, which cannot tell the buffers apart,
+// would otherwise wait for the phases in flight before it reads the one that has landed. Every wait for them is the explicit one below,
+// by their number; so nothing else may load to registers in the loop: the exponents lie in LDS, 64 blocks at a time.
 __device__ __forceinline__ void fetch16(const uint8_t* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
 
-// Chunk h of fragment i of a wave's rows, one half block: a lane holds 32 codes of one of 32 rows, chunks 2 (lane / 32) and the next
-// of the half's four.
-__device__ __forceinline__ void read_chunk(const uint8_t* lds, int lane, int half, int i, int h, i32x8& f) {
-  const int r = lane & 31, c = half * 4 + (lane >> 5) * 2 + h, sw = (r >> 1) & 7;
-  const uint4 v = *reinterpret_cast<const uint4*>(lds + r * 128 + i * 4096 + (c ^ sw) * 16);
+// Chunk 2 (lane / 32) + h of fragment i of a wave's rows: a lane holds 32 codes of one of 32 rows.
+__device__ __forceinline__ void read_chunk(const uint8_t* lds, int lane, int i, int h, i32x8& f) {
+  const int r = lane & 31, c = (lane >> 5) * 2 + h;
+  const uint4 v = *reinterpret_cast<const uint4*>(lds + r * 64 + i * 2048 + (c ^ ((r >> 2) & 3)) * 16);
   f[4 * h] = (int)v.x; f[4 * h + 1] = (int)v.y; f[4 * h + 2] = (int)v.z; f[4 * h + 3] = (int)v.w;
 }
 
@@ -121,8 +119,10 @@ template <int FMT, int MT, int NT, typename Y>
 __global__ void __launch_bounds__(256, 1)
 gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
   constexpr bool EXACT = sizeof(Y) == 4;
-  constexpr int TM = 64 * MT, TN = 64 * NT, BYTES = (TM + TN) * 128;
-  extern __shared__ __align__(16) uint8_t s_tiles[];
+  constexpr int TM = 64 * MT, TN = 64 * NT, BYTES = (TM + TN) * 64, EXPS = 64, EPITCH = EXPS + 4;
+  extern __shared__ __align__(16) uint8_t s_tiles[];          // four buffers, then the exponents of 64 blocks: TM rows, TN / 128 columns
+  uint8_t* const s_ex = s_tiles + 4 * BYTES;
+  uint8_t* const s_ew = s_ex + TM * EPITCH;
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s_tiles;
   // Workgroups go round the 8 XCDs in turn: give each XCD one run of tiles (its own L2 sees neighbouring rows and columns), and
   // inside a run walk 8 tiles down before the next column.
@@ -136,58 +136,64 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
   const int64_t kend = (o.K + 15) / 16 * 16;
   const int KB = (int)((o.K + BLOCK - 1) / BLOCK);
 
-  // Instruction i of a wave's fetches of an operand: rows 32 i + 8 wave + lane / 8, the lane's chunk. (The swizzle does not depend on i.)
-  const int fr = wave * 8 + (lane >> 3), fc = (lane & 7) ^ ((fr >> 1) & 7);
+  // Instruction i of a wave's fetches of an operand: rows 64 i + 16 wave + lane / 4, the lane's chunk. (The swizzle does not depend on i.)
+  constexpr int FX = MT, FW = NT, FETCHES = FX + FW, READS = 2 * (MT + NT), MULS = MULTIPLICATIONS<EXACT, MT, NT>;
+  const int fr = wave * 16 + (lane >> 2), fc = (lane & 3) ^ ((fr >> 2) & 3);
   const int last_chunks = (int)((kend - (int64_t)(KB - 1) * BLOCK) / 16);
-  const unsigned last_shift = (unsigned)(min(fc, last_chunks - 1) - fc) * 16u;       // (0, or negative)
-  unsigned offx[2 * MT], offw[2 * NT];
+  // from a lane's offset in a block to its chunk of the last block's halves (with the offset never below zero: it is unsigned)
+  const unsigned shift0 = (unsigned)(min(fc, last_chunks - 1) - fc) * 16u, shift1 = (unsigned)(min(4 + fc, last_chunks - 1) - fc) * 16u;
+  unsigned offx[FX], offw[FW];
 #pragma unroll
-  for (int i = 0; i < 2 * MT; ++i) offx[i] = (unsigned)min((int64_t)(fr + i * 32), o.M - 1 - m0) * (unsigned)o.ldx + fc * 16;
+  for (int i = 0; i < FX; ++i) offx[i] = (unsigned)min((int64_t)(fr + i * 64), o.M - 1 - m0) * (unsigned)o.ldx + fc * 16;
 #pragma unroll
-  for (int i = 0; i < 2 * NT; ++i) offw[i] = (unsigned)min((int64_t)(fr + i * 32), o.N - 1 - n0) * (unsigned)o.ldw + fc * 16;
+  for (int i = 0; i < FW; ++i) offw[i] = (unsigned)min((int64_t)(fr + i * 64), o.N - 1 - n0) * (unsigned)o.ldw + fc * 16;
   const uint8_t *xt = o.x + m0 * o.ldx, *wt = o.w + n0 * o.ldw;
-  constexpr int PARTS = 2 * (MT + NT), MULS = MULTIPLICATIONS<EXACT, MT, NT>;
-  auto fetch = [&](int kb, int p) {          // instruction p of PARTS
-    const unsigned lds = lds0 + (kb & 1) * BYTES + wave * 1024;
-    const unsigned shift = kb + 1 == KB ? last_shift : 0u;
-    if (p < 2 * MT) fetch16(xt + (int64_t)kb * BLOCK, offx[p] + shift, lds + p * 4096);
-    else fetch16(wt + (int64_t)kb * BLOCK, offw[p - 2 * MT] + shift, lds + TM * 128 + (p - 2 * MT) * 4096);
+  auto fetch = [&](int kb, int half, int buf, int p) {        // instruction p of FETCHES
+    const unsigned lds = lds0 + buf * BYTES + wave * 1024;
+    const unsigned shift = kb + 1 == KB ? (half ? shift1 : shift0) : half * 64u;
+    const int64_t at = (int64_t)kb * BLOCK;
+    if (p < FX) fetch16(xt + at, offx[p] + shift, lds + p * 4096);
+    else fetch16(wt + at, offw[p - FX] + shift, lds + TM * 64 + (p - FX) * 4096);
   };
-  const uint8_t* ex = o.ex + m0 * o.ldex;
-  unsigned exo[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) exo[i] = (unsigned)(min((int64_t)(wm + i * 32 + (lane & 31)), o.M - 1 - m0) * o.ldex);
-  const uint8_t* ew = o.ew + min(n0 + wn, o.N - 1) / BLOCK * o.ldew;         // a wave's 32 NT columns lie in one block
-
+  auto read = [&](int buf, i32x8 (&a)[MT], i32x8 (&b)[NT], int p) {                  // instruction p of READS
+    const uint8_t* lds = s_tiles + buf * BYTES;
+    if (p < 2 * MT) read_chunk(lds + wm * 64, lane, p >> 1, p & 1, a[p >> 1]);
+    else read_chunk(lds + (TM + wn) * 64, lane, (p - 2 * MT) >> 1, p & 1, b[(p - 2 * MT) >> 1]);
+  };
+  // the exponents of blocks kb .. kb + 63 (four at a time: their rows are multiples of four bytes)
+  auto exponents = [&](int kb) {
+    const int n4 = (min(KB - kb, EXPS) + 3) >> 2;
+    for (int t = threadIdx.x; t < (TM + TN / BLOCK + 1) * n4; t += 256) {
+      const int r = t / n4, c = t - r * n4;
+      const uint8_t* e = r < TM ? o.ex + min(m0 + r, o.M - 1) * o.ldex : o.ew + min(n0 + (r - TM) * BLOCK, o.N - 1) / BLOCK * o.ldew;
+      *reinterpret_cast<unsigned*>(s_ex + r * EPITCH + c * 4) = *reinterpret_cast<const unsigned*>(e + kb + c * 4);
+    }
+  };
   i32x8 a0[MT], b0[NT], a1[MT], b1[NT];
   int sx[MT], sw, sx_next[MT], sw_next;
-  // (whole dwords, four blocks at a time, the byte picked when it is taken: a byte's zero extension would wait for its load, and so
-  // for the fetches behind it, where the load stands)
+  const uint8_t *exl = s_ex + (wm + (lane & 31)) * EPITCH, *ewl = s_ew + wn / BLOCK * EPITCH;
   auto scales = [&](int kb) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sx_next[i] = *reinterpret_cast<const int*>(ex + (kb & ~3) + exo[i]);
-    sw_next = *reinterpret_cast<const int*>(ew + (kb & ~3));
+    for (int i = 0; i < MT; ++i) sx_next[i] = exl[i * 32 * EPITCH + (kb & (EXPS - 1))];
+    sw_next = ewl[kb & (EXPS - 1)];
   };
-  auto take_scales = [&](int kb) {           // the scales are in registers from here on: no wait for them further down
-    const int shift = (kb & 3) * 8;
+  auto take_scales = [&]() {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) { asm volatile("" : "+v"(sx_next[i])); sx[i] = (int)((unsigned)sx_next[i] >> shift & 0xffu); }
-    asm volatile("" : "+v"(sw_next));
-    sw = (int)((unsigned)sw_next >> shift & 0xffu);
+    for (int i = 0; i < MT; ++i) sx[i] = sx_next[i];
+    sw = sw_next;
   };
-  auto landed = [&]() {                      // this wave's fetches have arrived; after the barrier, every wave's
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  // this wave's fetches have arrived but for the two newest phases'; after the barrier, every wave's
+  auto landed = [&]() {
+    static_assert(FETCHES == 8 || FETCHES == 4, "the wait below counts two phases of fetches");
+    if (FETCHES == 8) asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
 
-  auto read = [&](int kb, int half, i32x8 (&a)[MT], i32x8 (&b)[NT], int p) {       // instruction p of PARTS
-    const uint8_t* lds = s_tiles + (kb & 1) * BYTES;
-    if (p < 2 * MT) read_chunk(lds + wm * 128, lane, half, p >> 1, p & 1, a[p >> 1]);
-    else read_chunk(lds + (TM + wn) * 128, lane, half, (p - 2 * MT) >> 1, p & 1, b[(p - 2 * MT) >> 1]);
-  };
-
-  scales(0);
+  exponents(0);
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) fetch(0, p);
+  for (int h = 0; h < 4; ++h)
+#pragma unroll
+    for (int p = 0; p < FETCHES; ++p) fetch(min(h >> 1, KB - 1), h & 1, h, p);
   // the sums start at the bias (its loads run beside the first fetch)
   f32x16 acc[NT][MT];
   auto start = [&](auto bias) {
@@ -202,45 +208,43 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
   };
   if (!o.bias) start([](int64_t) { return 0.f; });
   else GANET_BY_TYPE(o.btype, B, start([&](int64_t n) { return (float)static_cast<const B*>(o.bias)[n]; }));
-  landed();
-  take_scales(0);
-  if (KB > 1) {
-    scales(1);
+  // phase 0 (all but the three newest) for its first reads; the loop waits for phase 1 itself
+  if (FETCHES == 8) asm volatile("s_waitcnt vmcnt(24) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(12) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  scales(0);
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) fetch(1, p);
-  }
-#pragma unroll
-  for (int p = 0; p < PARTS; ++p) read(0, 0, a0, b0, p);
+  for (int p = 0; p < READS; ++p) read(0, a0, b0, p);
   for (int kb = 0; kb + 1 < KB; ++kb) {
+    const int buf = (kb & 1) * 2, next = min(kb + 2, KB - 1);
+    landed();
+    take_scales();
     __builtin_amdgcn_sched_barrier(0);
     multiply<FMT, MT, NT, EXACT>(a0, b0, sx, sw, acc, [&](int q) {
 #pragma unroll
-      for (int p = PARTS * q / MULS; p < PARTS * (q + 1) / MULS; ++p) read(kb, 1, a1, b1, p);
+      for (int p = READS * q / MULS; p < READS * (q + 1) / MULS; ++p) read(buf + 1, a1, b1, p);
+#pragma unroll
+      for (int p = FETCHES * q / MULS; p < FETCHES * (q + 1) / MULS; ++p) fetch(next, 0, buf, p);
       __builtin_amdgcn_sched_barrier(0);
     });
-    landed();                                // step kb + 1 is there, and nobody reads this step's buffer any more
-    int px[MT];
-    const int pw = sw;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) px[i] = sx[i];
-    take_scales(kb + 1);
-    const int next = min(kb + 2, KB - 1);    // (behind the last step the last one is fetched again, into the buffer nobody reads)
-    scales(next);
+    landed();
+    if ((kb + 1) % EXPS == 0) {              // the next 64 blocks' exponents (nobody reads the old ones any more)
+      exponents(kb + 1);
+      __syncthreads();
+    }
+    scales(kb + 1);
     __builtin_amdgcn_sched_barrier(0);
-    multiply<FMT, MT, NT, EXACT>(a1, b1, px, pw, acc, [&](int q) {
+    multiply<FMT, MT, NT, EXACT>(a1, b1, sx, sw, acc, [&](int q) {
 #pragma unroll
-      for (int p = PARTS * q / MULS; p < PARTS * (q + 1) / MULS; ++p) {
-        read(kb + 1, 0, a0, b0, p);
-        const unsigned lds = lds0 + (kb & 1) * BYTES + wave * 1024;
-        const unsigned shift = next + 1 == KB ? last_shift : 0u;
-        if (p < 2 * MT) fetch16(xt + (int64_t)next * BLOCK, offx[p] + shift, lds + p * 4096);
-        else fetch16(wt + (int64_t)next * BLOCK, offw[p - 2 * MT] + shift, lds + TM * 128 + (p - 2 * MT) * 4096);
-      }
+      for (int p = READS * q / MULS; p < READS * (q + 1) / MULS; ++p) read(2 - buf, a0, b0, p);
+#pragma unroll
+      for (int p = FETCHES * q / MULS; p < FETCHES * (q + 1) / MULS; ++p) fetch(next, 1, buf + 1, p);
       __builtin_amdgcn_sched_barrier(0);
     });
   }
+  landed();
+  take_scales();
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) read(KB - 1, 1, a1, b1, p);
+  for (int p = 0; p < READS; ++p) read(((KB - 1) & 1) * 2 + 1, a1, b1, p);
   if (last_chunks < 8) {                     // what was fetched past the rows' codes
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -405,7 +409,7 @@ int launch_few(const Operands& o, hipStream_t stream) {
 template <int FMT, int MT, int NT, typename Y>
 int launch_tile(const Operands& o, hipStream_t stream) {
   static PerDeviceFlag ready;
-  constexpr int steps = 2 * 64 * (MT + NT) * 128, out = 64 * MT * (64 * NT * (int)sizeof(Y) + 16), lds = steps > out ? steps : out;
+  constexpr int steps = 4 * 64 * (MT + NT) * 64 + (64 * MT + NT / 2 + 1) * 68, out = 64 * MT * (64 * NT * (int)sizeof(Y) + 16), lds = steps > out ? steps : out;
   auto k = gemm8_tile_kernel<FMT, MT, NT, Y>;
   if (!ready) {
     const int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
