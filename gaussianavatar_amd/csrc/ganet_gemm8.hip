@@ -263,7 +263,7 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // (the fetches behind the last step)
   // A lane holds one row m and, four at a time, consecutive columns n. Stored from there, an instruction would touch 32 rows with 16
   // or 32 bytes each; through LDS (rows of 16 bytes more than the tile's: the 32 rows of a write fall into different banks) every
-  // row leaves in full 16-byte pieces: 57 -> 8 us per 256 x 256 tile.
+  // row leaves in full 16-byte pieces.
   constexpr int V = 16 / (int)sizeof(Y), PITCH = TN + V;
   Y* s_y = reinterpret_cast<Y*>(s_tiles);
   __syncthreads();
@@ -462,7 +462,7 @@ int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes,
   }
   if (M == 0) return 0;
   if (!y || (ldy < N && M > 1) || !held_ok(M, K, codes, ldc, exps, lde) || !held_ok(N, K, wcodes, ldwc, wexps, ldwe)) {
-    set_error("ganet_gemm8: NULL or misaligned argument, or a row stride too small");
+    set_error("ganet_gemm8: NULL or misaligned argument, or a row stride outside columns .. 2^24");
     return 1;
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);

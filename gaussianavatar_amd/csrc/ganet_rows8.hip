@@ -170,6 +170,12 @@ weight8_pack_kernel(int64_t N, int64_t K, const T* __restrict__ w, int64_t ldw, 
   }
 }
 
+// The rows of one launch: a grid has fewer than 2^32 threads in all
+int64_t rows_per_launch(const Map& m, int64_t KB) {
+  constexpr int64_t most = (1ll << 23);
+  return KB > GROUPS ? most / m.segs : most * (GROUPS >> m.log2p);
+}
+
 bool codes_ok(const void* codes, int64_t ldc, int64_t C, const uint8_t* exps, int64_t lde) {
   return codes && exps && ldc % 16 == 0 && ldc >= pad16(C) && (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && lde % 4 == 0 &&
          lde >= cdiv(C, BLOCK) && (reinterpret_cast<uintptr_t>(exps) & 3) == 0;
@@ -195,13 +201,16 @@ int ganet_rows8_pack(int64_t M, int64_t C, int32_t type, int32_t fmt, const void
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   const int64_t KB = cdiv(C, BLOCK);
-  const Map map = make_map(M, KB);
-  if (map.grid >= (1ll << 31)) { set_error("ganet_rows8_pack: too many blocks"); return 4; }
-  GANET_BY_TYPE(type, T, {
-    auto k = fmt == GANET_E4M3 ? rows8_pack_kernel<T, GANET_E4M3> : rows8_pack_kernel<T, GANET_E5M2>;
-    hipLaunchKernelGGL(k, dim3((unsigned)map.grid), dim3(WG), 0, stream, M, C, static_cast<const T*>(x), ldx,
-                       static_cast<uint8_t*>(codes), ldc, exps, lde, KB, map);
-  });
+  const int64_t most = rows_per_launch(make_map(M, KB), KB);
+  for (int64_t m = 0; m < M; m += most) {
+    const int64_t rows = M - m < most ? M - m : most;
+    const Map map = make_map(rows, KB);
+    GANET_BY_TYPE(type, T, {
+      auto k = fmt == GANET_E4M3 ? rows8_pack_kernel<T, GANET_E4M3> : rows8_pack_kernel<T, GANET_E5M2>;
+      hipLaunchKernelGGL(k, dim3((unsigned)map.grid), dim3(WG), 0, stream, rows, C, static_cast<const T*>(x) + m * ldx, ldx,
+                         static_cast<uint8_t*>(codes) + m * ldc, ldc, exps + m * lde, lde, KB, map);
+    });
+  }
   return check_hip(hipGetLastError(), "ganet_rows8_pack");
 }
 
@@ -218,13 +227,16 @@ int ganet_rows8_unpack(int64_t M, int64_t C, int32_t type, int32_t fmt, const vo
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   const int64_t KB = cdiv(C, BLOCK);
-  const Map map = make_map(M, KB);
-  if (map.grid >= (1ll << 31)) { set_error("ganet_rows8_unpack: too many blocks"); return 4; }
-  GANET_BY_TYPE(type, T, {
-    auto k = fmt == GANET_E4M3 ? rows8_unpack_kernel<T, GANET_E4M3> : rows8_unpack_kernel<T, GANET_E5M2>;
-    hipLaunchKernelGGL(k, dim3((unsigned)map.grid), dim3(WG), 0, stream, M, C, static_cast<const uint8_t*>(codes), ldc, exps,
-                       lde, static_cast<T*>(y), KB, map);
-  });
+  const int64_t most = rows_per_launch(make_map(M, KB), KB);
+  for (int64_t m = 0; m < M; m += most) {
+    const int64_t rows = M - m < most ? M - m : most;
+    const Map map = make_map(rows, KB);
+    GANET_BY_TYPE(type, T, {
+      auto k = fmt == GANET_E4M3 ? rows8_unpack_kernel<T, GANET_E4M3> : rows8_unpack_kernel<T, GANET_E5M2>;
+      hipLaunchKernelGGL(k, dim3((unsigned)map.grid), dim3(WG), 0, stream, rows, C, static_cast<const uint8_t*>(codes) + m * ldc, ldc,
+                         exps + m * lde, lde, static_cast<T*>(y) + m * C, KB, map);
+    });
+  }
   return check_hip(hipGetLastError(), "ganet_rows8_unpack");
 }
 

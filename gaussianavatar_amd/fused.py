@@ -125,7 +125,7 @@ class _LinearKept8Fn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         codes, exps, weight = ctx.saved_tensors
-        dx = g @ weight if ctx.needs_input_grad[0] else None
+        dx = g @ weight.to(g.dtype) if ctx.needs_input_grad[0] else None       # (g's type is autocast's where that is on)
         dW = db = None
         if ctx.needs_input_grad[1] or (ctx.btype is not None and ctx.needs_input_grad[2]):
             dW, db = rows8.wgrad8(g, rows8.Rows8(codes, exps, ctx.cols, ctx.lead), weight.dtype)
@@ -136,7 +136,7 @@ class _LinearKept8Fn(torch.autograd.Function):
 def linear(x, weight, bias, checkpoint8=False):
     """x [..., K] -> x @ weight^T + bias. checkpoint8: what the backward pass keeps of x is its 8-bit rows (a quarter of fp32), so
     dW is that of the rounded x (2^-4 of a value at most); y and dx are unchanged."""
-    if checkpoint8:
+    if checkpoint8 and torch.is_grad_enabled():
         return _LinearKept8Fn.apply(x, weight, bias)
     if x.is_cuda and x.dtype == torch.float32 and x.dim() == 2:
         return _LinearFn.apply(x, weight, bias)
@@ -221,6 +221,7 @@ class _LayerNormActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, act, kept8):
         x2 = rows8._rows2d(x)
+        weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
         M, C = x2.shape
         stats = torch.empty(M if kept8 else 2 * M, dtype=torch.float32, device=x.device)          # rstd, then the mean
         codes = torch.empty((M, (C + 15) // 16 * 16), dtype=torch.uint8, device=x.device) if kept8 else None
@@ -315,6 +316,7 @@ def layernorm_act(x, ln: torch.nn.LayerNorm, act: str = "softplus", checkpoint8:
     if x.is_cuda and known:
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)):
             return _LayerNormActFn.apply(x, weight, bias, ln.eps, act, checkpoint8)
+        weight, bias = (None if p is None else p.detach().contiguous() for p in (weight, bias))
         y = _ln_fwd(rows8._rows2d(x.detach()), weight, bias, ln.eps, act, None, None)
         return y if x.dim() == 2 else y.reshape(x.shape)
     if checkpoint8:

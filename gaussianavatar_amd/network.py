@@ -70,6 +70,7 @@ class ShapeDecoder(nn.Module):
     the rows' own type."""
 
     HEADS = ("", "N", "SH")
+    norm, bits8 = "batch", False               # (of a decoder unpickled from before it had a choice)
 
     def __init__(self, in_size, hsize=256, actv_fn="softplus", norm="batch", bits8=False):
         super().__init__()

@@ -50,10 +50,10 @@ def _type_code(t, what):
 
 
 def _rows2d(x):
-    """x as [M, K] whose rows are adjacent in memory and do not overlap (a copy only where they are not)."""
+    """x as [M, K] whose rows are adjacent in memory, do not overlap and lie at most 2^24 elements apart (a copy only where they are not)."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     K = x2.shape[1]
-    if (K > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < K):
+    if (K > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and not K <= x2.stride(0) <= 1 << 24):
         x2 = x2.contiguous()
     return x2
 

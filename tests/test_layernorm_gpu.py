@@ -191,3 +191,37 @@ def test_what_the_kernels_do_not_take_runs_on_torch():
         fused.layernorm_act(x.cpu(), ln)
     with pytest.raises(TypeError):
         fused.layernorm_act(x, ln, checkpoint8=True)
+
+
+def test_strided_parameters():
+    from gaussianavatar_amd import fused
+    x, ln, dy = inputs(50, 72, torch.float32, torch.float32, 7)
+    want = fused.layernorm_act(x, ln, "softplus")
+    grads = torch.autograd.grad(want, (ln.weight, ln.bias), dy)
+    far = torch.nn.LayerNorm(72, device="cuda")
+    base = torch.full((72, 2, 3), 9.0, device="cuda")
+    base[:, 0, 0], base[:, 1, 2] = ln.weight.detach(), ln.bias.detach()
+    far.weight, far.bias = torch.nn.Parameter(base[:, 0, 0]), torch.nn.Parameter(base[:, 1, 2])
+    got = fused.layernorm_act(x, far, "softplus")
+    assert torch.equal(got, want)
+    with torch.no_grad():
+        assert torch.equal(fused.layernorm_act(x, far, "softplus"), want)
+    for a, b in zip(torch.autograd.grad(got, (far.weight, far.bias), dy), grads):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kept8", [False, True])
+def test_rows_behind_2_to_the_32_elements(kept8):
+    """A row's results do not depend on where it lies."""
+    from gaussianavatar_amd import fused
+    M, C = 2 ** 22 + 3, 1030
+    ln = torch.nn.LayerNorm(C, device="cuda")
+    x = torch.empty(M, C, dtype=torch.bfloat16, device="cuda").normal_().requires_grad_(True)
+    dy = torch.empty(M, C, dtype=torch.bfloat16, device="cuda").normal_()
+    y = fused.layernorm_act(x, ln, "relu", checkpoint8=kept8)
+    (dx,) = torch.autograd.grad(y, (x,), dy)
+    for lo, hi in ((0, 300), (2 ** 21, 2 ** 21 + 300), (M - 300, M)):
+        part = x.detach()[lo:hi].clone().requires_grad_(True)
+        want = fused.layernorm_act(part, ln, "relu", checkpoint8=kept8)
+        assert torch.equal(y[lo:hi], want)
+        assert torch.equal(dx[lo:hi], torch.autograd.grad(want, (part,), dy[lo:hi])[0])

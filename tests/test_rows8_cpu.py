@@ -180,3 +180,30 @@ def test_refusals_of_the_c_entry_points():
     assert lib.ganet_rows8_bytes(-1, 8) == 0 and lib.ganet_rows8_bytes(3, 66) == 3 * 80 + 3 * 4 and lib.ganet_weight8_bytes(130, 66) == 130 * 80 + 2 * 4
     assert lib.ganet_wgrad8_workspace(4, 8, 1 << 22, 0) == 0 and lib.ganet_ln_bwd_workspace(-1, 8, 0) == 0
     assert lib.ganet_rows8_pack(0, 8, 0, 0, None, 8, None, 16, None, 4, None) == 0
+
+
+def test_refusals_of_row_strides_beyond_32_bit_offsets():
+    lib = _native.ganet()
+    A, far = 1 << 20, (1 << 24) + 16
+    for ldg, ldc, lde in ((far, 16, 4), (8, far, 4), (8, 16, far)):
+        assert lib.ganet_wgrad8(4, 8, 8, 0, 0, A, ldg, A, ldc, A, lde, A, None, 0, None, 0, None) == 1
+        assert b"ganet_wgrad8" in lib.ganet_last_error()
+
+
+def test_linear_with_an_8_bit_checkpoint_under_autocast_on_the_cpu():
+    x, w = torch.randn(6, 20, requires_grad=True), torch.randn(5, 20, requires_grad=True)
+    with torch.autocast("cpu", torch.bfloat16):
+        y = fused.linear(x, w, None, checkpoint8=True)
+    dx, dw = torch.autograd.grad(y.sum(), (x, w))
+    assert y.dtype == torch.bfloat16 and dx.dtype == dw.dtype == torch.float32
+    with torch.no_grad():
+        assert torch.equal(fused.linear(x, w, None, checkpoint8=True), torch.nn.functional.linear(x, w))
+
+
+def test_a_decoder_unpickled_from_before_it_had_a_norm_runs():
+    dec = ShapeDecoder(4, 16)
+    x = torch.randn(1, 4, 12)
+    want = dec.eval()(x)
+    del dec.norm, dec.bits8
+    for a, b in zip(dec(x), want):
+        assert torch.equal(a, b)

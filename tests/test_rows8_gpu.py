@@ -412,3 +412,78 @@ def test_avatar_model_trains_with_the_8_bit_layer_norm_decoder():
     grads = [p.grad for n, p in model.net.decoder.named_parameters()]
     assert all(g is not None and torch.isfinite(g).all() for g in grads) and any(g.abs().max() > 0 for g in grads)
     model.step(1)
+
+
+# ---------------------------------------------------------------------------------------------- non-finite gradients, long and far rows
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(45, 20, 130), (4109, 1030, 1030)])
+def test_a_non_finite_gradient_stays_in_its_column(M, N, K, dtype):
+    """In the last row too, which the kernel's last step may load more than once."""
+    from gaussianavatar_amd import rows8
+    x, g = spread(M, K, dtype, 1), spread(M, N, dtype, 2)
+    g[M - 1, 3], g[M - 1, 6], g[10, 5] = float("inf"), -float("inf"), float("nan")
+    dW, db = rows8.wgrad8(g, rows8.quantize8(x))
+    assert db[3] == float("inf") and db[6] == -float("inf") and torch.isnan(db[5])
+    assert not torch.isfinite(dW[[3, 5, 6]]).any()
+    rest = [n for n in range(N) if n not in (3, 5, 6)]
+    assert_wgrad(dW[rest], db[rest], g[:, rest].double().cpu(), oracle.rows(x.cpu())[0], dtype)
+
+
+def test_rows_behind_4_gib_of_codes():
+    """2^28 rows are two launches of 2^27; codes lie past 2^32 bytes."""
+    from gaussianavatar_amd import rows8
+    M = 2 ** 28 + 37
+    x = torch.randn(M, 1, device="cuda", dtype=torch.float16)
+    r = rows8.quantize8(x)
+    y = r.dequantize(torch.float16)
+    for lo, hi in ((0, 999), (2 ** 27 - 500, 2 ** 27 + 500), (M - 999, M)):
+        want = rows8.quantize8(x[lo:hi])
+        assert torch.equal(r.codes[lo:hi].view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(r.exps[lo:hi, 0], want.exps[:, 0])
+        assert torch.equal(y[lo:hi], want.dequantize(torch.float16))
+
+
+def test_products_and_weight_gradients_behind_4_gib_of_codes():
+    from gaussianavatar_amd import rows8
+    M, N, K = 2 ** 20 + 3, 5, 4100
+    at = torch.tensor([0, 31, 12345, 2 ** 19, 2 ** 20 - 1, M - 2, M - 1], device="cuda")
+    some, some_g, w = spread(len(at), K, torch.bfloat16, 1), spread(len(at), N, torch.float32, 2), spread(N, K, torch.bfloat16, 3)
+    x, g = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda"), torch.zeros(M, N, device="cuda")
+    x[at], g[at] = some, some_g
+    r = rows8.quantize8(x)
+    del x
+    y = rows8.matmul8(r, rows8.quantize8_weight(w))
+    assert_product(y[at], oracle.rows(some.cpu())[0], oracle.weight(w.cpu())[0], None, torch.float32)
+    y[at] = 0
+    assert not y.any()
+    dW, db = rows8.wgrad8(g, r)
+    assert_wgrad(dW, db, some_g.double().cpu(), oracle.rows(some.cpu())[0], torch.float32)
+
+
+def test_rows_that_lie_far_apart():
+    from gaussianavatar_amd import rows8
+    base = torch.zeros(3 * (2 ** 24 + 8), device="cuda", dtype=torch.bfloat16)
+    g, x = base.as_strided((3, 8), (2 ** 24 + 8, 1)), base.as_strided((3, 40), (2 ** 24 + 8, 1), 16)
+    g.copy_(spread(3, 8, torch.bfloat16, 1)), x.copy_(spread(3, 40, torch.bfloat16, 2))
+    r, near = rows8.quantize8(x), rows8.quantize8(x.contiguous())
+    assert torch.equal(r.codes.view(torch.uint8), near.codes.view(torch.uint8))
+    for a, b in zip(rows8.wgrad8(g, r), rows8.wgrad8(g.contiguous(), r)):
+        assert torch.equal(a, b)
+
+
+def test_linear_with_an_8_bit_checkpoint_under_autocast_and_without_gradients():
+    from gaussianavatar_amd import fused
+    x, w, b = (spread(*s, torch.float32, i).requires_grad_(True) for i, s in enumerate(((70, 33), (9, 33), (1, 9))))
+    with torch.no_grad():
+        assert torch.equal(fused.linear(x, w, b[0], checkpoint8=True), fused.linear(x, w, b[0]))
+    with torch.autocast("cuda", torch.bfloat16):
+        y = fused.linear(x, w, b[0], checkpoint8=True)
+    assert y.dtype == torch.bfloat16
+    g = spread(70, 9, torch.bfloat16, 5)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    assert dx.dtype == dw.dtype == torch.float32
+    assert_wgrad(dw, db[0], g.double().cpu(), oracle.rows(x.detach().cpu())[0], torch.float32)
+    want = g.double() @ w.detach().double()
+    # w to bf16, products of up to 9 terms in fp32, one rounding to bf16
+    assert bool(((dx.double() - want).abs() <= 2.0 ** -7 * 1.01 * (g.double().abs() @ w.detach().double().abs())).all())
