@@ -523,10 +523,11 @@ Shape make_shape(int64_t C, int32_t type) {
   const int64_t n = cdiv(C, 16 / type_size(type));             // 16-byte vectors of a row
   Shape s{0, 1, 1, LN_WG};
   if (n <= 256) {
-    // two vectors per lane where the row gives them: half the shuffles, twice the loads in flight of one vector per lane
+    // two vectors per lane where the row gives them: half the shuffles, twice the loads in flight of one vector per lane (200000 x 256
+    // bf16, forward / backward: 57 / 85 us against 62 / 103). A workgroup per row for these: 65536 x 1024 bf16 157 / 351 against 70 / 116.
     while (s.G < 64 && s.G * 2 < n) s.G *= 2;
     s.NC = n <= s.G ? 1 : n <= 2 * s.G ? 2 : 4;
-  } else if (n <= 2048) {
+  } else if (n <= 2048) {                                      // (streaming instead: 8192 x 8192 bf16 153 / 387 against 72 / 121)
     s.form = 1;
     s.NC = 2;
     s.threads = n <= 512 ? 256 : n <= 1024 ? 512 : 1024;
@@ -538,25 +539,19 @@ Shape make_shape(int64_t C, int32_t type) {
   return s;
 }
 
-// One round of workgroups strides over the rows: as many as are resident at a time (256 CUs; by the kernels' registers), the same number on
-// every CU, and among those numbers the one that leaves the fewest idle in the last turn.
+// One round of workgroups strides over the rows: as many as are resident at a time (256 CUs; by the kernels' registers). (Fewer, where
+// that evens out the last turn: 200000 x 256 bf16 forward 57 against 53, 16384 x 4096 backward 121 against 104.)
 constexpr int CUS = 256, STREAM_SLICES = 64;
-int64_t even_grid(int64_t turns, int per_cu) {
-  if (turns <= (int64_t)CUS * per_cu) return turns;
-  int best = per_cu;
-  for (int k = per_cu; k > per_cu / 2; --k)
-    if (cdiv(turns, (int64_t)CUS * k) * k < cdiv(turns, (int64_t)CUS * best) * best) best = k;
-  return (int64_t)CUS * best;
-}
+int64_t one_round(int64_t turns, int per_cu) { return turns < (int64_t)CUS * per_cu ? turns : (int64_t)CUS * per_cu; }
 int64_t fwd_grid(const Shape& s, int32_t type, int64_t M) {
   if (s.form == 2) return M < 2 * CUS ? M : 2 * CUS;
   const int per_cu = s.threads == 1024 ? 1 : s.threads == 512 ? 2 : type == GANET_F32 ? 6 : 4;
-  return even_grid(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu);
+  return one_round(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu);
 }
 int64_t bwd_grid(const Shape& s, int32_t type, int64_t M) {
   if (s.form == 2) return M < STREAM_SLICES ? M : STREAM_SLICES;
   const int per_cu = s.threads >= 512 ? (type == GANET_F32 && s.threads == 512 ? 2 : 1) : type == GANET_F32 ? (s.NC > 2 ? 2 : 4) : s.NC > 2 ? 1 : s.form ? 3 : 2;
-  return even_grid(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu);
+  return one_round(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu);
 }
 
 bool ln_ok(int64_t M, int64_t C, int32_t type, int32_t wtype, int32_t act) {
