@@ -353,7 +353,7 @@ def ganet() -> ctypes.CDLL:
         lib.ganet_weight8_pack.argtypes = [L, L, I, P, L, P, L, P, L, P, L, P, L, P]
         lib.ganet_gemm8.restype = c_int
         lib.ganet_gemm8.argtypes = [L, L, L, I, P, L, P, L, P, L, P, L, P, I, P, L, I, P]
-        for name, args in (("ganet_rows8_bytes", [L, L]), ("ganet_weight8_bytes", [L, L]), ("ganet_linear8_held_workspace", [L, L]),
+        for name, args in (("ganet_rows8_bytes", [L, L]), ("ganet_weight8_bytes", [L, L]), ("ganet_linear8_held_workspace", [L, L, L, I]),
                            ("ganet_linear8_bwd_workspace", [L, L, L, I])):
             getattr(lib, name).restype = c_size_t
             getattr(lib, name).argtypes = args

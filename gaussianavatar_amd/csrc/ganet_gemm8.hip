@@ -301,8 +301,11 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
 // The weight's codes are the traffic: every wave streams its share of the blocks of 16 weight rows straight from global memory into matrix
 // operands (a lane: 32 codes of one row), the eight waves' sums meet in LDS. X: the rows' type. Rows that come as they are (not as
 // codes) are packed in registers, by the rule of ganet_rows8_pack: the four lanes that hold a row's block take its maximum and
-// convert; every workgroup repeats that, which costs less than a launch for up to 32 rows.
-constexpr int FEW_WAVES = 8, FEW_UNROLL = 4;
+// convert; every workgroup repeats that (packs_inside() below tells where that costs less than a launch).
+// What bounds it is latency: so everything that a wave needs of UNROLL blocks is asked for at once, without a branch between the
+// loads (rows past the last read the last one, as do blocks); a last block that is not full comes behind them. From codes, bf16:
+// 1 x 4096 x 4096 7.6 us, 16 rows 9.2 (12.1 and 19.6 with the loads under conditions), 1 x 16384 x 4096 15 us, 4.5 TB/s.
+constexpr int FEW_WAVES = 8;
 struct Codes;        // the rows' type where they are codes already
 
 // 32 values of a row's block, held by the four lanes l, l ^ 16, l ^ 32, l ^ 48 -> operand and biased exponent
@@ -319,67 +322,115 @@ __device__ __forceinline__ void pack_block(const float (&v)[32], i32x8& f, int& 
   e = x + 127;
 }
 
+// A lane's 32 values of a row's block as they were loaded, and the operand that they become
+template <typename X>
+struct Few {
+  X v[32];
+  __device__ __forceinline__ void load(const Operands& o, int64_t m, int64_t k, int) {
+    __builtin_memcpy(v, reinterpret_cast<const X*>(o.x) + m * o.ldx + k, sizeof(v));
+  }
+  __device__ __forceinline__ void operand(i32x8& f, int& e) const {
+    float t[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t[i] = (float)v[i];
+    pack_block(t, f, e);
+  }
+};
+template <>
+struct Few<Codes> {
+  uint4 v[2];
+  int e;
+  __device__ __forceinline__ void load(const Operands& o, int64_t m, int64_t k, int kb) {
+    const uint4* p = reinterpret_cast<const uint4*>(o.x + m * o.ldx + k);
+    v[0] = p[0];
+    v[1] = p[1];
+    e = o.ex[m * o.ldex + kb];
+  }
+  __device__ __forceinline__ void operand(i32x8& f, int& exponent) const {
+    f = join(v[0], v[1]);
+    exponent = e;
+  }
+};
+
 template <int FMT, int MT, typename X, typename Y>
 __global__ void __launch_bounds__(64 * FEW_WAVES)
 gemm8_few_kernel(Operands o) {
   constexpr bool CODES = __is_same(X, Codes), EXACT = sizeof(Y) == 4;
-  constexpr int UNROLL = CODES ? FEW_UNROLL : 2;
+  constexpr int UNROLL = MT * sizeof(Few<X>) <= 128 ? 4 : 2;
   __shared__ f32x4 s_acc[FEW_WAVES][MT][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int64_t kend = (o.K + 15) / 16 * 16;
-  const int KB = (int)((o.K + BLOCK - 1) / BLOCK);
+  const int full = (int)(o.K / BLOCK);
   const uint8_t* wr = o.w + min(n0 + r, o.N - 1) * o.ldw + q * 32;
   const uint8_t* ew = o.ew + n0 / BLOCK * o.ldew;
+  int64_t m[MT];
   f32x4 acc[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int kb0 = wave; kb0 < KB; kb0 += FEW_WAVES * UNROLL) {
-    uint4 w[UNROLL][2];
-    i32x8 x[UNROLL][MT];
-    int sw[UNROLL], sx[UNROLL][MT];
+  for (int i = 0; i < MT; ++i) {
+    m[i] = min((int64_t)(i * 16 + r), o.M - 1);
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto multiply = [&](const i32x8& w, int sw, const i32x8 (&x)[MT], const int (&sx)[MT]) {
+    if constexpr (!EXACT) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int kb = kb0 + u * FEW_WAVES;
-      const int64_t k = (int64_t)kb * BLOCK;
-      const bool lo = kb < KB && k + q * 32 < kend, hi = kb < KB && k + q * 32 + 16 < kend;
-      w[u][0] = lo ? *reinterpret_cast<const uint4*>(wr + k) : zero;
-      w[u][1] = hi ? *reinterpret_cast<const uint4*>(wr + k + 16) : zero;
-      sw[u] = kb < KB ? ew[kb] : 127;
+      for (int i = 0; i < MT; ++i)
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x[i], acc[i], GANET_E4M3, FMT, 0, sw, 0, sx[i]);
+    } else {
+      // fp32 results: bf16 instructions on decoded codes (see multiply() above)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int64_t m = min((int64_t)(i * 16 + r), o.M - 1);
-        if constexpr (CODES) {
-          const uint8_t* xr = o.x + m * o.ldx + k + q * 32;
-          x[u][i] = join(lo ? *reinterpret_cast<const uint4*>(xr) : zero, hi ? *reinterpret_cast<const uint4*>(xr + 16) : zero);
-          sx[u][i] = kb < KB ? o.ex[m * o.ldex + kb] : 127;
-        } else {
-          float v[32];
-          const X* xr = reinterpret_cast<const X*>(o.x) + m * o.ldx + k + q * 32;
-          load_n(xr, i * 16 + r < o.M && kb < KB ? o.K - (k + q * 32) : 0, v);
-          pack_block(v, x[u][i], sx[u][i]);
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const i32x8 b = join(w[u][0], w[u][1]);
-      if constexpr (!EXACT) {
+      for (int d = 0; d < 8; d += 2) {
+        const bf16x8 wd = decode8<GANET_E4M3>(w, d, pow2(sw - 127));
 #pragma unroll
         for (int i = 0; i < MT; ++i)
-          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, x[u][i], acc[i], GANET_E4M3, FMT, 0, sw[u], 0, sx[u][i]);
-      } else {
-        // fp32 results: bf16 instructions on decoded codes (see multiply() above)
-#pragma unroll
-        for (int d = 0; d < 8; d += 2) {
-          const bf16x8 wd = decode8<GANET_E4M3>(b, d, pow2(sw[u] - 127));
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd, decode8<FMT>(x[u][i], d, pow2(sx[u][i] - 127)), acc[i], 0, 0, 0);
-        }
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd, decode8<FMT>(x[i], d, pow2(sx[i] - 127)), acc[i], 0, 0, 0);
       }
     }
+  };
+  for (int kb0 = wave; kb0 < full; kb0 += FEW_WAVES * UNROLL) {
+    uint4 w[UNROLL][2];
+    Few<X> raw[UNROLL][MT];
+    int sw[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int kb = min(kb0 + u * FEW_WAVES, full - 1);
+      const uint4* p = reinterpret_cast<const uint4*>(wr + (int64_t)kb * BLOCK);
+      w[u][0] = p[0];
+      w[u][1] = p[1];
+      sw[u] = ew[kb];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) raw[u][i].load(o, m[i], (int64_t)kb * BLOCK + q * 32, kb);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (kb0 + u * FEW_WAVES >= full) break;
+      i32x8 x[MT];
+      int sx[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) raw[u][i].operand(x[i], sx[i]);
+      multiply(join(w[u][0], w[u][1]), sw[u], x, sx);
+    }
+  }
+  if (o.K % BLOCK && wave == full % FEW_WAVES) {
+    const int64_t k = (int64_t)full * BLOCK + q * 32, kend = (o.K + 15) / 16 * 16;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    auto codes = [&](const uint8_t* p) {                       // p: of column k
+      return join(k < kend ? *reinterpret_cast<const uint4*>(p) : zero, k + 16 < kend ? *reinterpret_cast<const uint4*>(p + 16) : zero);
+    };
+    i32x8 x[MT];
+    int sx[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if constexpr (CODES) {
+        x[i] = codes(o.x + m[i] * o.ldx + k);
+        sx[i] = o.ex[m[i] * o.ldex + full];
+      } else {
+        float v[32];
+        load_n(reinterpret_cast<const X*>(o.x) + m[i] * o.ldx + k, o.K - k, v);
+        pack_block(v, x[i], sx[i]);
+      }
+    }
+    multiply(codes(wr + (int64_t)full * BLOCK), ew[full], x, sx);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) s_acc[wave][i][lane] = acc[i];
@@ -389,14 +440,15 @@ gemm8_few_kernel(Operands o) {
   f32x4 t = s_acc[0][i][lane];
 #pragma unroll
   for (int v = 1; v < FEW_WAVES; ++v) t += s_acc[v][i][lane];
-  const int64_t m = i * 16 + r, n = n0 + q * 4;
-  if (m >= o.M) return;
+  const int64_t row = i * 16 + r, n = n0 + q * 4;
+  if (row >= o.M) return;
   float v[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) v[c] = t[c] + ((o.bias && n + c < o.N) ? load_param(o.bias, o.btype, n + c) : 0.f);
-  store_n(static_cast<Y*>(o.y) + m * o.ldy + n, o.N - n, v);
+  store_n(static_cast<Y*>(o.y) + row * o.ldy + n, o.N - n, v);
 }
 
+// (32 x 4096 x 4096 from codes, bf16 / fp32: 11.9 / 11.8 us; in tiles 17.6 / 32.7)
 constexpr int FEW_ROWS = 32;
 template <int FMT, typename X, typename Y>
 int launch_few(const Operands& o, hipStream_t stream) {
@@ -426,9 +478,18 @@ int launch_tile(const Operands& o, hipStream_t stream) {
 template <int FMT, typename Y>
 int launch(const Operands& o, hipStream_t stream) {
   if (o.M <= FEW_ROWS) return launch_few<FMT, Codes, Y>(o, stream);
+  // The tile: 256 x 256 for 16-bit results (an fp32 tile of that size does not fit LDS on its way out) where three quarters of the CUs get
+  // one, else 128 x 128. 192 tiles (3000 x 4096 x 4096): 52 us against 62; 128 (4096 x 2048 x 2048): 31 against 27.
   if constexpr (sizeof(Y) == 2)
-    if (cdiv(o.M, 256) * cdiv(o.N, 256) >= 256) return launch_tile<FMT, 4, 4, Y>(o, stream);
+    if (cdiv(o.M, 256) * cdiv(o.N, 256) >= 192) return launch_tile<FMT, 4, 4, Y>(o, stream);
   return launch_tile<FMT, 2, 2, Y>(o, stream);
+}
+
+// Whether few rows are packed inside the product's kernel: by what a CU has to pack then (16 rows, 4096 columns of the result, 1024 of the
+// rows: one unit, of fp32 two). Inside / with a launch of its own, in a graph, bf16: 1 x 1024 x 1024 7.4 / 8.8 us, 1 x 4096 x 4096
+// 8.9 / 9.3, 1 x 8192 x 4096 14.6 / 12.4, 32 x 4096 x 4096 16.7 / 14.6; fp32: 1 x 1024 x 1024 7.8 / 9.2, 16 x 4096 x 4096 14.7 / 11.8.
+bool packs_inside(int64_t M, int64_t N, int64_t K, int32_t type) {
+  return M <= FEW_ROWS && cdiv(M, 16) * cdiv(N, 4096) * cdiv(K, 1024) * (type == GANET_F32 ? 2 : 1) <= 4;
 }
 
 bool held_ok(int64_t N, int64_t K, const void* c, int64_t ld, const uint8_t* e, int64_t le) {
@@ -479,7 +540,9 @@ size_t ganet_weight8_bytes(int64_t N, int64_t K) {
   return rows_ok(N, K) ? (size_t)(N * pad16(K) + cdiv(N, BLOCK) * ((cdiv(K, BLOCK) + 3) / 4 * 4)) : 0;
 }
 
-size_t ganet_linear8_held_workspace(int64_t M, int64_t K) { return M <= FEW_ROWS ? 0 : ganet_rows8_bytes(M, K); }
+size_t ganet_linear8_held_workspace(int64_t M, int64_t N, int64_t K, int32_t type) {
+  return packs_inside(M, N, K, type) ? 0 : ganet_rows8_bytes(M, K);
+}
 
 int ganet_linear8_held(int64_t M, int64_t N, int64_t K, int32_t type, const void* x, int64_t ldx, const void* wcodes, int64_t ldwc,
                        const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y, void* workspace,
@@ -490,12 +553,12 @@ int ganet_linear8_held(int64_t M, int64_t N, int64_t K, int32_t type, const void
   }
   if (M == 0) return 0;
   if (!x || !y || (ldx < K && M > 1) || !held_ok(N, K, wcodes, ldwc, wexps, ldwe) ||
-      workspace_bytes < ganet_linear8_held_workspace(M, K) || (M > FEW_ROWS && !workspace)) {
+      workspace_bytes < ganet_linear8_held_workspace(M, N, K, type) || (!packs_inside(M, N, K, type) && !workspace)) {
     set_error("ganet_linear8_held: NULL or misaligned argument, a row stride or the workspace too small");
     return 1;
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  if (M <= FEW_ROWS) {
+  if (packs_inside(M, N, K, type)) {
     const Operands o{M, N, K, static_cast<const uint8_t*>(x), ldx, nullptr, 0, static_cast<const uint8_t*>(wcodes), ldwc, wexps, ldwe,
                      bias, btype, y, N};
     GANET_BY_TYPE(type, T, return (launch_few<GANET_E4M3, T, T>(o, stream)));

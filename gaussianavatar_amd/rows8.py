@@ -371,7 +371,7 @@ def linear8(x, weight, bias=None):
         M = x2.shape[0]
         lib = _native.ganet()
         y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-        nbytes = lib.ganet_linear8_held_workspace(M, K)
+        nbytes = lib.ganet_linear8_held_workspace(M, N, K, code)
         ws = _bytes(nbytes, x) if nbytes else None
         bias = None if bias is None else bias.detach().contiguous()
         _call(x.device, lib.ganet_linear8_held, M, N, K, code, x2.data_ptr(), _ld(x2), weight.codes.data_ptr(), weight.codes.stride(0),

@@ -424,14 +424,14 @@ int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, co
                  size_t workspace_bytes, void* stream);
 
 /* A linear layer on these, y [M, N] = Q(x) Q(W)^T + bias in x's type (e4m3 both), as one call each way.
- * _held: the weight is codes already; up to 32 rows are packed inside the product's kernel (no workspace).
+ * _held: the weight is codes already; a few rows are packed inside the product's kernel (workspace 0, may be NULL).
  * _fwd / _bwd: training. rows8 (ganet_rows8_bytes(M, K)) keeps Q(x) for the backward pass, weight8 (ganet_weight8_bytes(N, K)) holds Q(W)
  * during the call, tweight8 (ganet_weight8_bytes(K, N); NULL: no input gradient) its transposed codes for the backward pass; each
  * buffer: codes, row stride = columns up to a multiple of 16, then exponents, row stride = blocks of 128 up to a multiple of 4.
  * dx = Q(g) Q(W) (NULL: not needed), dW = g^T Q(x) and db in wtype (dW NULL: neither). */
 size_t ganet_rows8_bytes(int64_t M, int64_t C);
 size_t ganet_weight8_bytes(int64_t N, int64_t K);
-size_t ganet_linear8_held_workspace(int64_t M, int64_t K);
+size_t ganet_linear8_held_workspace(int64_t M, int64_t N, int64_t K, int32_t type);
 int ganet_linear8_held(int64_t M, int64_t N, int64_t K, int32_t type, const void* x, int64_t ldx, const void* wcodes, int64_t ldwc,
                        const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y, void* workspace,
                        size_t workspace_bytes, void* stream);
