@@ -111,18 +111,25 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int G, float* s_red, int&
 // A vector of a row as it was loaded: elements past the row's end, and all of a row that does not exist, are zero.
 template <typename T>
 struct Vec { T e[VEC<T>]; };
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ Vec<T> load_vec(const T* __restrict__ p, int n) {
   Vec<T> v;
-  if (n >= VEC<T>) __builtin_memcpy(&v, p, sizeof(v));
-  else {
+  if (n >= VEC<T>) {
+    if (STREAM) {
+      const u32x4 q = load_stream(p);
+      __builtin_memcpy(&v, &q, sizeof(v));
+    } else __builtin_memcpy(&v, p, sizeof(v));
+  } else {
 #pragma unroll
     for (int i = 0; i < VEC<T>; ++i) v.e[i] = i < n ? p[i] : (T)0.f;
   }
   return v;
 }
 
-template <typename T, int NC, bool WIDE, int THREADS>
+// STREAM: no backward pass reads x again (it reads codes, or there is none), so x passes the caches by. y does in any case: 262144 x 128
+// fp32 65 -> 49 us, its backward pass 76 -> 63, and what reads y next is no slower (with the packing of y: 89 -> 76 us, of 65536 rows 27 ->
+// 24). 16384 x 4096 bf16 to codes 78 -> 55 us with both; x that is kept and read again at once costs 12 us more in the backward pass.
+template <typename T, int NC, bool WIDE, int THREADS, bool STREAM>
 __global__ void __launch_bounds__(THREADS)
 ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
               const void* __restrict__ b, int32_t wtype, float eps, int act, T* __restrict__ y, float* __restrict__ mean_out,
@@ -151,7 +158,7 @@ ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       const int c = (j * G + l) * V;
-      next[j] = load_vec(x + r * ldx + c, r < M ? C - c : 0);
+      next[j] = load_vec<STREAM>(x + r * ldx + c, r < M ? C - c : 0);
     }
   };
   fetch(row);
@@ -204,7 +211,7 @@ ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
 #pragma unroll
       for (int i = 0; i < V; ++i) v[j][i] = fmaf(v[j][i], wv[j][i], bv[j][i]);
       act_fwd(v[j], act);
-      store_n(y + row * C + c, C - c, v[j]);
+      store_stream(y + row * C + c, C - c, v[j]);
     }
   }
 }
@@ -278,7 +285,7 @@ struct Kept {
 #pragma unroll
       for (int q = 0; q < VEC<T> / 4; ++q) c[q] = 0u;
       if (n > 0) __builtin_memcpy(c, __builtin_assume_aligned(cr + c0, VEC<T>), VEC<T>);
-    } else x = load_vec(xr + c0, n);
+    } else x = load_vec<false>(xr + c0, n);
   }
   __device__ __forceinline__ void values(float mean, float rstd, float code_unit, float (&xh)[VEC<T>]) const {
     if (KEPT8) {
@@ -334,7 +341,7 @@ ln_bwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       const int c = (j * G + l) * V, n = live ? C - c : 0;
-      gn[j] = load_vec(dy + r * lddy + c, n);
+      gn[j] = load_vec<false>(dy + r * lddy + c, n);
       xn[j].load(x + r * ldx, codes + r * ldc, c, n);
     }
     if (!KEPT8) mean_n = live ? mean_in[r] : 0.f;
@@ -374,7 +381,7 @@ ln_bwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
         if (c >= C) continue;
 #pragma unroll
         for (int i = 0; i < V; ++i) g[j][i] = rstd * (g[j][i] - fmaf(xh[j][i], m2, m1));
-        store_n(dx + row * C + c, C - c, g[j]);
+        store_stream(dx + row * C + c, C - c, g[j]);
       }
     }
   }
@@ -588,9 +595,10 @@ int ganet_ln_fwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
   const float cs = std::ldexp(1.0f, -ganet_ln_code_exponent(C));
   const dim3 grid((unsigned)fwd_grid(s, type, M));
   uint8_t* cd = static_cast<uint8_t*>(codes);
+  const bool again = mean != nullptr;
 #define LN_FWD(NC, WIDE, TH)                                                                                            \
-  hipLaunchKernelGGL((ln_fwd_kernel<T, NC, WIDE, TH>), grid, dim3(TH), 0, stream, M, (int)C, s.G, static_cast<const T*>(x), ldx, w, b, \
-                     wtype, eps, act, static_cast<T*>(y), mean, rstd, cd, ldc, cs)
+  hipLaunchKernelGGL((again ? ln_fwd_kernel<T, NC, WIDE, TH, false> : ln_fwd_kernel<T, NC, WIDE, TH, true>), grid, dim3(TH), 0, stream, M, \
+                     (int)C, s.G, static_cast<const T*>(x), ldx, w, b, wtype, eps, act, static_cast<T*>(y), mean, rstd, cd, ldc, cs)
   GANET_BY_TYPE(type, T, {
     if (s.form == 2)
       hipLaunchKernelGGL(ln_fwd_stream_kernel<T>, grid, dim3(1024), 0, stream, M, C, static_cast<const T*>(x), ldx, w, b,

@@ -50,6 +50,24 @@ __device__ __forceinline__ void store_n(T* __restrict__ p, int64_t n, const floa
   }
 }
 
+// The same past the caches, 16 bytes at a time: for what this operator does not touch again.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_loose __attribute__((aligned(2)));
+template <typename T>
+__device__ __forceinline__ u32x4 load_stream(const T* p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4_loose*>(p)); }
+template <int N, typename T>
+__device__ __forceinline__ void store_stream(T* __restrict__ p, int64_t n, const float (&v)[N]) {
+  static_assert(N * sizeof(T) == 16, "one 16-byte store");
+  if (n >= N) {
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = (T)v[i];
+    u32x4 q;
+    __builtin_memcpy(&q, t, 16);
+    __builtin_nontemporal_store(q, reinterpret_cast<u32x4_loose*>(p));
+  } else store_n(p, n, v);
+}
+
 // one parameter of a type known at run time (a uniform branch)
 __device__ __forceinline__ float load_param(const void* p, int32_t type, int64_t i) {
   return type == GANET_F32 ? static_cast<const float*>(p)[i]
