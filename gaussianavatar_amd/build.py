@@ -21,10 +21,9 @@ OBJ = os.path.join(OUT, "obj")
 ARCH = "gfx950"
 
 COMMON = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-I" + os.path.join(ROOT, "include"),
-          "-I" + CSRC, "-fhip-fp32-correctly-rounded-divide-sqrt", "-Wall", "-Wno-unused-function"]
-
-# scalar fp32 instructions only (no v_pk_add / mul / fma_f32)
-NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+          "-I" + CSRC, "-fhip-fp32-correctly-rounded-divide-sqrt", "-Wall", "-Wno-unused-function",
+          # scalar fp32 instructions only (no v_pk_add / mul / fma_f32)
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # (source, extra flags). gsr_preprocess.hip decides the integer outputs (radii, tile rects):
 # no FMA contraction there, so that it follows the operation order shared with the oracle.
@@ -55,10 +54,10 @@ LIBS = {
         ("ganet_unet.hip", []),
         ("ganet_conv.hip", []),
         ("ganet_optim.hip", []),
-        ("ganet_norm.hip", NO_PACKED_FP32),
-        ("ganet_rows8.hip", NO_PACKED_FP32),
-        ("ganet_gemm8.hip", NO_PACKED_FP32),
-        ("ganet_wgrad8.hip", NO_PACKED_FP32),
+        ("ganet_norm.hip", []),
+        ("ganet_rows8.hip", []),
+        ("ganet_gemm8.hip", []),
+        ("ganet_wgrad8.hip", []),
     ],
 }
 

@@ -101,7 +101,7 @@ __device__ __forceinline__ void buf_store(float v, __amdgpu_buffer_rsrc_t r, uin
 //     the 11 output rows it contributes to; the oldest one is then complete);
 //   * (backward) the SIDE ring: the image pixels the finished output row needs, fetched a round ahead too.
 // The maps of a row travel through LDS interleaved (one 8- or 16-byte entry per column), so a tap is one
-// ds_read and the filters run on packed pairs (v_pk_fma_f32).
+// ds_read.
 
 __global__ void __launch_bounds__(64 * WAVES)
 ssim_fwd_kernel(int H, int W, const float* __restrict__ img1, const float* __restrict__ img2,

@@ -7,7 +7,7 @@ set -e
 out=$1; shift
 mkdir -p $out/obj
 cp gaussianavatar_amd/_lib/libgalbs_hip.so $out/
-common="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Iinclude -Igaussianavatar_amd/csrc -fhip-fp32-correctly-rounded-divide-sqrt"
+common="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Iinclude -Igaussianavatar_amd/csrc -fhip-fp32-correctly-rounded-divide-sqrt -Xclang -target-feature -Xclang -packed-fp32-ops"
 objs=""
 for f in ganet_bn ganet_wgrad ganet_ssim ganet_mlp ganet_mlp_bwd ganet_mlp_split ganet_wgrad_split ganet_layer_bwd ganet_layer_fwd ganet_decoder ganet_pack ganet_upsample ganet_optim ganet_conv; do
   [ -f gaussianavatar_amd/csrc/$f.hip ] || continue
