@@ -5,7 +5,7 @@
 //
 // Bound: HBM. Forward reads x and writes y once, backward reads x (or its 8-bit xh) and dy and writes dx once: a row stays in
 // registers between its reduction and its use, the variance is taken about the mean (no E[x^2] - mean^2). A group of G lanes holds
-// a row, NC vectors of 16 bytes each: G = 1 .. 64 lanes of a wave for rows up to 4 KiB, a whole workgroup of 256 .. 1024 threads
+// a row, NC vectors of 16 bytes each: G = 1 .. 64 lanes of a wave for rows up to 4 KiB (backward: 2), a workgroup of 256 .. 1024 threads
 // up to 32 KiB, and a streaming form that reads the row three times (from cache) beyond. Groups stride over the rows, so
 // a lane always sees the same columns: w and b are loaded once, dw and db are summed in registers and leave as ONE partial row pair per workgroup,
 // added in a fixed order by a second kernel (no atomics: bit-reproducible).
@@ -546,6 +546,13 @@ Shape make_shape(int64_t C, int32_t type) {
   return s;
 }
 
+// Backward, four vectors per lane would take all registers: a workgroup per row, one vector per lane (32768 x 2048 bf16 143 -> 98 us).
+Shape bwd_shape(int64_t C, int32_t type) {
+  Shape s = make_shape(C, type);
+  if (s.NC == 4) s = Shape{1, 256, 1, 256};
+  return s;
+}
+
 // One round of workgroups strides over the rows: as many as are resident at a time (256 CUs; by the kernels' registers). (Fewer, where
 // that evens out the last turn: 200000 x 256 bf16 forward 57 against 53, 16384 x 4096 backward 121 against 104.)
 constexpr int CUS = 256, STREAM_SLICES = 64;
@@ -555,10 +562,13 @@ int64_t fwd_grid(const Shape& s, int32_t type, int64_t M) {
   const int per_cu = s.threads == 1024 ? 1 : s.threads == 512 ? 2 : type == GANET_F32 ? 6 : 4;
   return one_round(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu);
 }
+// (a workgroup per row leaves a row of partial sums: at least four rows each, where that gives half of the CUs one: 1000 x 2048 bf16
+// 25 -> 16 us, 300 x 4096 20 -> 17)
 int64_t bwd_grid(const Shape& s, int32_t type, int64_t M) {
   if (s.form == 2) return M < STREAM_SLICES ? M : STREAM_SLICES;
-  const int per_cu = s.threads >= 512 ? (type == GANET_F32 && s.threads == 512 ? 2 : 1) : type == GANET_F32 ? (s.NC > 2 ? 2 : 4) : s.NC > 2 ? 1 : s.form ? 3 : 2;
-  return one_round(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu);
+  const int per_cu = s.threads >= 512 ? (type == GANET_F32 && s.threads == 512 ? 2 : 1) : type == GANET_F32 || (s.form && s.NC == 1) ? 4 : s.form ? 3 : 2;
+  const int64_t n = one_round(cdiv(M, s.form ? 1 : s.threads / s.G), per_cu), few = cdiv(M, 4) > CUS / 2 ? cdiv(M, 4) : CUS / 2;
+  return s.form && few < n ? few : n;
 }
 
 bool ln_ok(int64_t M, int64_t C, int32_t type, int32_t wtype, int32_t act) {
@@ -619,7 +629,7 @@ int ganet_ln_fwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
 
 size_t ganet_ln_bwd_workspace(int64_t M, int64_t C, int32_t type) {
   if (!rows_ok(M, C) || !type_ok(type)) return 0;
-  return (size_t)bwd_grid(make_shape(C, type), type, M < 1 ? 1 : M) * 2 * (size_t)C * sizeof(float);
+  return (size_t)bwd_grid(bwd_shape(C, type), type, M < 1 ? 1 : M) * 2 * (size_t)C * sizeof(float);
 }
 
 int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* x, int64_t ldx, const float* mean,
@@ -638,7 +648,7 @@ int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
     return 1;
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  const Shape s = make_shape(C, type);
+  const Shape s = bwd_shape(C, type);
   const float cu = std::ldexp(1.0f, ganet_ln_code_exponent(C));
   float* part = sums ? static_cast<float*>(workspace) : nullptr;
   const uint8_t* cd = static_cast<const uint8_t*>(codes);
@@ -660,13 +670,13 @@ int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
                            0, stream, M, C, static_cast<const T*>(x), ldx, mean, cd, ldc, cu, rstd, w, b, wtype, act,          \
                            static_cast<const T*>(dy), lddy, part);                                                            \
     } else if (s.form == 1) {                                                                                                 \
-      if (s.threads == 256) LN_BWD(2, true, 256, K8);                                                                         \
+      if (s.NC == 1) LN_BWD(1, true, 256, K8);                                                                                \
+      else if (s.threads == 256) LN_BWD(2, true, 256, K8);                                                                    \
       else if (s.threads == 512) LN_BWD(2, true, 512, K8);                                                                    \
       else LN_BWD(2, true, 1024, K8);                                                                                         \
     } else {                                                                                                                  \
       if (s.NC == 1) LN_BWD(1, false, LN_WG, K8);                                                                             \
-      else if (s.NC == 2) LN_BWD(2, false, LN_WG, K8);                                                                        \
-      else LN_BWD(4, false, LN_WG, K8);                                                                                       \
+      else LN_BWD(2, false, LN_WG, K8);                                                                                       \
     }                                                                                                                         \
   } while (0)
   if (M > 0) {

@@ -225,3 +225,11 @@ def test_rows_behind_2_to_the_32_elements(kept8):
         want = fused.layernorm_act(part, ln, "relu", checkpoint8=kept8)
         assert torch.equal(y[lo:hi], want)
         assert torch.equal(dx[lo:hi], torch.autograd.grad(want, (part,), dy[lo:hi])[0])
+
+
+@pytest.mark.parametrize("kept8", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,C", [(1500, 2048), (900, 4096), (700, 1030), (5, 2047)])
+def test_several_rows_to_a_workgroup(M, C, dtype, kept8):
+    x, ln, dy = inputs(M, C, dtype, torch.float32, M)
+    check(x, ln, dy, "softplus", kept8)
