@@ -7,7 +7,7 @@
 // enters with no further rounding. g enters with all its bits as 1 (bf16), 2 (fp16) or 3 (fp32) bf16 pieces; sums are fp32.
 //
 // What bounds it: for wide layers the matrix instructions (P products per product of the layer), for the 128 columns of a point decoder
-// the reads (262144 x 128 x 128 fp32, 169 MB: 47 us with the reduction, 33 of them at a copy's rate).
+// the reads (262144 x 128 x 128 fp32, 169 MB: 45 us with the reduction, 33 of them at a copy's rate).
 // Both operands need the row index as the matrix instruction's k: tiles lie in LDS as they lie in memory ([row][column], bf16) and
 // ds_read_b64_tr_b16 hands each lane four rows of its column.
 #include "ganet_rows8.h"
@@ -67,26 +67,28 @@ struct Job {
 struct Where { int tn, tk, split; };
 
 // A workgroup computes a tile of dW, COLS x COLS, over its range of rows; a wave 32 TI x 32 TJ of it. A step is 32 rows: thread t brings row
-// t / (COLS / 16), 16 columns of g and of x, from global memory into registers two steps ahead, and as bf16 into one of two LDS buffers
+// t / TPR, 16 (8) columns of g and of x, from global memory into registers two steps ahead, and as bf16 into one of two LDS buffers
 // one step ahead, so that one barrier per step is enough and a load has two steps to arrive. Two waves stand on a SIMD: one converts,
 // reads and writes LDS while the other one's matrix instructions run. 8192 x 4096 x 4096 bf16: 274 us, 1.0 PFLOP/s (a large library
-// product reaches 1.13). With one wave on a SIMD, four of 128 x 128 in a workgroup, which have a third less to read from LDS, 320 us.
-// INSIDE: the tile ends before column N of g (vectors of 8; else element by element).
+// product reaches 1.13). With one wave on a SIMD, four of 128 x 128 in a workgroup, which have a third less to read from LDS, 320 us (262144 x 128 x 128 fp32 47 us against 45).
+// INSIDE: no vector of 8 columns crosses column N of g (one behind it is read as the last one); else element by element
+// (300000 x 64 x 64 bf16: 29 us against 48).
 template <int TILE> struct Form;
-template <> struct Form<256> { static constexpr int TI = 4, TJ = 2, WN = 2; };
-template <> struct Form<128> { static constexpr int TI = 2, TJ = 2, WN = 2; };
+template <> struct Form<256> { static constexpr int TI = 4, TJ = 2, WN = 2, WAVES = 8; };
+template <> struct Form<128> { static constexpr int TI = 2, TJ = 1, WN = 2, WAVES = 8; };
 template <int FMT, typename G, int COLS, bool INSIDE>
 __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsigned short* s_mem) {
   typedef Form<COLS> F;
   constexpr int TI = F::TI, TJ = F::TJ;
   constexpr int P = PIECES<G>, PITCH = pitch(COLS), PLANE = STEP * PITCH, BUF = (P + 1) * PLANE;
-  constexpr int GV = 8, GC = 2;                                // g: two vectors of 8 elements, COLS / 2 columns apart
+  constexpr int PER = STEP * COLS / (64 * F::WAVES), GV = 8, GC = PER / GV, TPR = COLS / PER;    // g: GC vectors of 8 elements, COLS / GC apart
+  typedef unsigned codes_t __attribute__((ext_vector_type(PER / 4)));
   const int64_t n0 = (int64_t)w.tn * COLS, k0 = (int64_t)w.tk * COLS;
   const int split = w.split;
   const int64_t m_lo = split * o.rows, m_hi = min(m_lo + o.rows, o.M);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wn = wave % F::WN * 32 * TI, wk = wave / F::WN * 32 * TJ;
-  const int sr = threadIdx.x / (COLS / 16), st = threadIdx.x % (COLS / 16);
+  const int sr = threadIdx.x / TPR, st = threadIdx.x % TPR;
   const int64_t kend = (o.K + 15) / 16 * 16;
   const G* g = static_cast<const G*>(o.g);
 
@@ -108,16 +110,16 @@ __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsign
   // (vectors of g are values, not memory: copied to memory and on, the compiler loads them again where they are put)
   typedef G vec __attribute__((ext_vector_type(8)));
   typedef G loose __attribute__((ext_vector_type(8), aligned(sizeof(G))));
-  struct Raw { vec g[GC]; uint4 x; int e; bool live; };
+  struct Raw { vec g[GC]; codes_t x; int e; bool live; };
   const unsigned lrow = (unsigned)min((int64_t)sr, m_hi - m_lo - 1);
   unsigned go[INSIDE ? 1 : GC * GV];
-  if constexpr (INSIDE) go[0] = (lrow * (unsigned)o.ldg + st * GV) * (unsigned)sizeof(G);
+  if constexpr (INSIDE) go[0] = (lrow * (unsigned)o.ldg + (GC == 1 ? min(st * GV, (int)(o.N - n0) - GV) : st * GV)) * (unsigned)sizeof(G);
   else {
 #pragma unroll
     for (int i = 0; i < GC * GV; ++i)
-      go[i] = (lrow * (unsigned)o.ldg + min((int)(o.N - 1 - n0), i / GV * (COLS / 2) + st * GV + i % GV)) * (unsigned)sizeof(G);
+      go[i] = (lrow * (unsigned)o.ldg + min((int)(o.N - 1 - n0), i / GV * (COLS / GC) + st * GV + i % GV)) * (unsigned)sizeof(G);
   }
-  const int xk = min(st * 16, (int)min(kend - k0, (int64_t)COLS) - 16);
+  const int xk = min(st * PER, (int)min(kend - k0, (int64_t)COLS) - PER);
   const unsigned xo = lrow * (unsigned)o.ldc + xk, eo = lrow * (unsigned)o.lde + xk / BLOCK;
   auto load = [&](Raw& v, int64_t m) {
     const int64_t at = max(m_lo, min(m, m_hi - STEP));
@@ -125,28 +127,29 @@ __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsign
     const char* gb = reinterpret_cast<const char*>(g + at * o.ldg + n0);
 #pragma unroll
     for (int i = 0; i < GC; ++i) {
-      if constexpr (INSIDE) v.g[i] = *reinterpret_cast<const loose*>(gb + i * (COLS / 2) * sizeof(G) + go[0]);
+      if constexpr (INSIDE) v.g[i] = *reinterpret_cast<const loose*>(gb + i * (COLS / GC) * sizeof(G) + go[0]);
       else {
 #pragma unroll
         for (int j = 0; j < GV; ++j) v.g[i][j] = *reinterpret_cast<const G*>(gb + go[i * GV + j]);
       }
     }
-    v.x = *reinterpret_cast<const uint4*>(o.codes + at * o.ldc + k0 + xo);
+    v.x = *reinterpret_cast<const codes_t*>(o.codes + at * o.ldc + k0 + xo);
     v.e = (o.exps + at * o.lde + k0 / BLOCK)[eo];
   };
   auto put = [&](const Raw& v, int buf) {
     unsigned short* base = s_mem + buf * BUF + sr * PITCH;
     const unsigned in = v.live ? ~0u : 0u;
     const float scale = pow2(v.e - 127);
-    const unsigned c[4] = {v.x.x & in, v.x.y & in, v.x.z & in, v.x.w & in};
-    uint4* d = reinterpret_cast<uint4*>(base + P * PLANE + st * 16);
-    d[0] = make_uint4(decode2<FMT>(c[0], scale, false), decode2<FMT>(c[0], scale, true), decode2<FMT>(c[1], scale, false),
-                      decode2<FMT>(c[1], scale, true));
-    d[1] = make_uint4(decode2<FMT>(c[2], scale, false), decode2<FMT>(c[2], scale, true), decode2<FMT>(c[3], scale, false),
-                      decode2<FMT>(c[3], scale, true));
+    uint4* d = reinterpret_cast<uint4*>(base + P * PLANE + st * PER);
+#pragma unroll
+    for (int i = 0; i < PER / 8; ++i) {
+      const unsigned a = v.x[2 * i] & in, b = v.x[2 * i + 1] & in;
+      d[i] = make_uint4(decode2<FMT>(a, scale, false), decode2<FMT>(a, scale, true), decode2<FMT>(b, scale, false),
+                        decode2<FMT>(b, scale, true));
+    }
 #pragma unroll
     for (int i = 0; i < GC; ++i) {
-      d = reinterpret_cast<uint4*>(base + i * (COLS / 2) + st * GV);
+      d = reinterpret_cast<uint4*>(base + i * (COLS / GC) + st * GV);
       float f[GV];
       if constexpr (P == 1) {                                  // bf16
         uint4 raw = __builtin_bit_cast(uint4, v.g[i]);
@@ -245,7 +248,7 @@ __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsign
 #pragma unroll
   for (int i = 0; i < GC; ++i)
 #pragma unroll
-    for (int j = 0; j < GV; ++j) s_b[sr * COLS + i * (COLS / 2) + st * GV + j] = bias[i][j];
+    for (int j = 0; j < GV; ++j) s_b[sr * COLS + i * (COLS / GC) + st * GV + j] = bias[i][j];
   __syncthreads();
   if (threadIdx.x >= COLS || n0 + threadIdx.x >= o.N) return;
   float t = 0.f;
@@ -255,7 +258,7 @@ __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsign
 }
 
 template <int FMT, typename G, int COLS>
-__global__ void __launch_bounds__(2 * COLS, 2)
+__global__ void __launch_bounds__(64 * Form<COLS>::WAVES, 2)
 wgrad8_kernel(Job o) {
   extern __shared__ __align__(16) unsigned short s_mem[];      // two buffers: the planes of g, one of x
   // Workgroups go round the 8 XCDs in turn: give each XCD one run of tiles, walked 4 tiles of n before the next tile of k, so that its 32
@@ -266,7 +269,7 @@ wgrad8_kernel(Job o) {
   // (in scalar registers: the divisions are done in vector ones)
   const Where w{__builtin_amdgcn_readfirstlane(group * 4 + in % gn), __builtin_amdgcn_readfirstlane(in / gn),
                 __builtin_amdgcn_readfirstlane(t / tiles)};
-  if ((int64_t)(w.tn + 1) * COLS <= o.N) wgrad8_tile<FMT, G, COLS, true>(o, w, s_mem);
+  if ((int64_t)(w.tn + 1) * COLS <= o.N || (COLS == 128 && o.N % 8 == 0)) wgrad8_tile<FMT, G, COLS, true>(o, w, s_mem);
   else wgrad8_tile<FMT, G, COLS, false>(o, w, s_mem);
 }
 
@@ -292,10 +295,10 @@ wgrad8_reduce_kernel(int64_t NK, int64_t N, int splits, const float* __restrict_
 }
 
 // The tile: 256 x 256 (one workgroup per CU) where that still gives every CU a tile and a range of at least 256 rows, else 128 x 128.
-// 8192 x 4096 x 4096, fp32 / fp16 / bf16: 715 / 459 / 275 us against 873 / 575 / 360; 1024 rows: 101 / 72 / 55 against 116 / 92 / 67;
-// 65536 x 512 x 512: 114 / 90 / 68 against 121 / 94 / 68.
-// The ranges: as many as give every CU a workgroup, none shorter than 128 rows. (Two small ones per CU: 262144 x 128 x 128 bf16 34 us
-// against 31, 4096 x 512 x 512 26 against 23. Ranges of 512 rows at least: 20000 x 128 x 128 17 against 18, 2000 x 128 x 128 15
+// 8192 x 4096 x 4096, fp32 / fp16 / bf16: 679 / 436 / 264 us against 873 / 587 / 366; 1024 rows: 96 / 69 / 53 against 114 / 85 / 63;
+// 65536 x 512 x 512: 110 / 87 / 67 against 128 / 101 / 76.
+// The ranges: as many as give every CU a workgroup, none shorter than 128 rows. (Two small ones per CU: 262144 x 128 x 128 bf16 33 us
+// against 30, 4096 x 512 x 512 26 against 23. Ranges of 512 rows at least: 20000 x 128 x 128 17 against 18, 2000 x 128 x 128 15
 // against 11; of 32: 25 and 13.)
 struct Plan { int cols; int64_t tiles_n, tiles_k; int splits; int64_t rows; };
 Plan make_plan(int64_t M, int64_t N, int64_t K) {
@@ -327,7 +330,7 @@ int launch_tile(const Job& o, hipStream_t stream) {
   }
   const int64_t grid = (int64_t)o.tiles_n * o.tiles_k * o.splits;
   if (grid >= (1ll << 30)) { set_error("ganet_wgrad8: too many tiles"); return 4; }
-  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(2 * COLS), lds, stream, o);
+  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * Form<COLS>::WAVES), lds, stream, o);
   return check_hip(hipGetLastError(), "ganet_wgrad8");
 }
 

@@ -487,3 +487,12 @@ def test_linear_with_an_8_bit_checkpoint_under_autocast_and_without_gradients():
     want = g.double() @ w.detach().double()
     # w to bf16, products of up to 9 terms in fp32, one rounding to bf16
     assert bool(((dx.double() - want).abs() <= 2.0 ** -7 * 1.01 * (g.double().abs() @ w.detach().double().abs())).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 8, 16), (45, 64, 128), (700, 136, 64), (259, 120, 300), (3000, 264, 24)])
+def test_weight_gradients_of_whole_vectors_that_end_inside_a_tile(M, N, K, dtype):
+    from gaussianavatar_amd import rows8
+    x, g = spread(M, K, dtype, M), spread(M, N + 3, dtype, N)[:, 1:N + 1]
+    dW, db = rows8.wgrad8(g, rows8.quantize8(x))
+    assert_wgrad(dW, db, g.double().cpu(), oracle.rows(x.cpu())[0], dtype)
