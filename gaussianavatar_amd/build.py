@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -81,27 +82,26 @@ def build(force: bool = False, verbose: bool = False) -> dict:
     hipcc = _hipcc()
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     headers += [os.path.join(ROOT, "include", f) for f in os.listdir(os.path.join(ROOT, "include"))]
+    headers.append(os.path.abspath(__file__))                # (the flags)
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+
+    libs = {lib: [(s, fl) for s, fl in sources if os.path.exists(os.path.join(CSRC, s))] for lib, sources in LIBS.items()}
+    obj = lambda src: os.path.join(OBJ, src.replace(".hip", ".o"))
+    stale = [(src, flags) for sources in libs.values() for src, flags in sources
+             if force or not _newer(obj(src), [os.path.join(CSRC, src)] + headers)]
+    with ThreadPoolExecutor(max(1, int(os.environ.get("MAX_JOBS", "0")) or min(8, os.cpu_count() or 1))) as pool:
+        list(pool.map(lambda s: run([hipcc] + COMMON + s[1] + ["-c", os.path.join(CSRC, s[0]), "-o", obj(s[0])]), stale))
     built = {}
-    for lib, sources in LIBS.items():
-        sources = [(s, fl) for s, fl in sources if os.path.exists(os.path.join(CSRC, s))]
+    for lib, sources in libs.items():
         if not sources:
             continue
-        objs = []
-        for src, flags in sources:
-            sp = os.path.join(CSRC, src)
-            op = os.path.join(OBJ, src.replace(".hip", ".o"))
-            if force or not _newer(op, [sp] + headers):
-                cmd = [hipcc] + COMMON + flags + ["-c", sp, "-o", op]
-                if verbose:
-                    print(" ".join(cmd), flush=True)
-                subprocess.check_call(cmd)
-            objs.append(op)
-        target = os.path.join(OUT, lib)
+        objs, target = [obj(src) for src, _ in sources], os.path.join(OUT, lib)
         if force or not _newer(target, objs):
-            cmd = [hipcc, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", target] + objs
-            if verbose:
-                print(" ".join(cmd), flush=True)
-            subprocess.check_call(cmd)
+            run([hipcc, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", target] + objs)
         built[lib] = target
     return built
 
