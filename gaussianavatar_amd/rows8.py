@@ -251,7 +251,7 @@ def matmul8(rows, w8, bias=None, dtype=torch.float32):
 
 def wgrad8(g, rows, dtype=None):
     """(dW [N, K], db [N]) = (g^T rows, column sums of g) for g [..., N] over the same rows, in `dtype` (g's own by default). g enters with
-    all its bits, sums are fp32."""
+    all its bits (of an fp32 value, those down to 2^-133), sums are fp32. A non-finite g makes its row of dW non-finite."""
     code = _type_code(g, "wgrad8")
     dtype = g.dtype if dtype is None else dtype
     if dtype not in _TYPE_CODE:

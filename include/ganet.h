@@ -412,12 +412,13 @@ int ganet_rows8_unpack(int64_t M, int64_t C, int32_t type, int32_t fmt, const vo
 int ganet_weight8_pack(int64_t N, int64_t K, int32_t type, const void* w, int64_t ldw, void* codes, int64_t ldc, uint8_t* exps,
                        int64_t lde, void* tcodes, int64_t ldtc, uint8_t* texps, int64_t ldte, void* stream);
 /* y [M, N] = rows [M, K] weight [N, K]^T + bias (btype, NULL: none): e4m3 or e5m2 rows, e4m3 weight; the matrix cores apply the
- * powers of two and accumulate in fp32; one rounding to ytype. */
+ * powers of two and accumulate in fp32; one rounding to ytype. Row strides of codes and exponents up to 2^24. */
 int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes, int64_t ldc, const uint8_t* exps, int64_t lde,
                 const void* wcodes, int64_t ldwc, const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y,
                 int64_t ldy, int32_t ytype, void* stream);
 /* dW [N, K] = g^T rows, db [N] = column sums of g (NULL: not needed), both contiguous in otype: the weight gradient of a layer
- * whose input is kept as rows in 8 bits. g [M, N] in gtype enters with all its bits. */
+ * whose input is kept as rows in 8 bits. g [M, N] in gtype enters with all its bits (of an fp32 value, those down to 2^-133). Row
+ * strides up to 2^24, K < 2^22. */
 size_t ganet_wgrad8_workspace(int64_t M, int64_t N, int64_t K, int32_t gtype);
 int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, const void* g, int64_t ldg, const void* codes,
                  int64_t ldc, const uint8_t* exps, int64_t lde, void* dW, void* db, int32_t otype, void* workspace,
