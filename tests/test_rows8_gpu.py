@@ -496,3 +496,16 @@ def test_weight_gradients_of_whole_vectors_that_end_inside_a_tile(M, N, K, dtype
     x, g = spread(M, K, dtype, M), spread(M, N + 3, dtype, N)[:, 1:N + 1]
     dW, db = rows8.wgrad8(g, rows8.quantize8(x))
     assert_wgrad(dW, db, g.double().cpu(), oracle.rows(x.cpu())[0], dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K", [(1, 256), (20, 300), (32, 1300), (40, 515)])
+def test_rows_that_start_anywhere(M, K, dtype):
+    from gaussianavatar_amd import rows8
+    x = spread(M, K + 6, dtype, M)[:, 1:K + 1]
+    w, b = spread(70, K + 3, dtype, 2)[:, 2:K + 2], spread(1, 72, dtype, 3)[0, 1:71]
+    w8 = rows8.quantize8_weight(w)
+    with torch.no_grad():
+        got, want = rows8.linear8(x, w8, b), rows8.linear8(x.contiguous(), rows8.quantize8_weight(w.contiguous()), b.contiguous())
+        assert torch.equal(got, want)
+        assert torch.equal(rows8.linear8(x, w, b), rows8.linear8(x.contiguous(), w.contiguous(), b.contiguous()))
