@@ -256,7 +256,7 @@ ln_fwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx,
     for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
       load_n(xr + c, C - c, v);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = (v[i] - mean) * rstd;
+      for (int i = 0; i < V; ++i) v[i] = c + i < C ? (v[i] - mean) * rstd : 0.f;    // (the backward pass reads a row's last vector whole)
       if (codes) {
         uint8_t* p = codes + row * ldc + c;
 #pragma unroll

@@ -1,0 +1,71 @@
+"""Layer norm, 8-bit rows and their products where they can go wrong: what the backward pass reads of kept rows, means far from zero,
+types of gradients, sums that cancel, and the largest sizes and values (tests/rows8_oracle.py in 64 bits).
+
+Tolerances as in test_layernorm_gpu.py and test_rows8_gpu.py; where one is new, its test derives it."""
+import pytest
+import torch
+
+from tests import rows8_oracle as oracle
+from tests.test_layernorm_gpu import U, TYPES, inputs
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------- layer norm kept in 8 bits
+
+
+def check_kept(x, ln, dy, kind):
+    """Gradients of every row and column, against the formula at the codes that the forward pass kept; each code is the nearest to a
+    value within the forward's own error of xh."""
+    from gaussianavatar_amd import fused
+    x = x.detach().requires_grad_(True)
+    M, C = x.shape
+    y = fused.layernorm_act(x, ln, kind, checkpoint8=True)
+    codes = y.grad_fn.saved_tensors[4][:, :C].view(torch.float8_e4m3fn).cpu().double()
+    dx, dw, db = (t.double().cpu() for t in torch.autograd.grad(y, (x, ln.weight, ln.bias), dy))
+    w, b = ln.weight.detach().double().cpu(), ln.bias.detach().double().cpu()
+    g = dy.double().cpu()
+    _, xh, rstd = oracle.layer_norm(x.detach().cpu(), w, b, ln.eps, kind)
+    size = x.detach().double().cpu().abs().amax(1, keepdim=True) * rstd
+    s = oracle.kept_scale(C)
+    off = 64 * U * (xh.abs() + size) / s
+    assert (codes >= oracle.grid(xh / s - off, "e4m3")).all() and (codes <= oracle.grid(xh / s + off, "e4m3")).all()
+    xh = codes * s
+    want = oracle.layer_norm_grads(xh, rstd, w, b, kind, g)
+    gw = (g * w).abs().amax(1, keepdim=True) * (1 + xh.abs().amax(1, keepdim=True) ** 2) * (1 + w.abs().max())
+    ph, deep = oracle.half_step(ln.weight.dtype), (M / 256 + 128) * U
+    tols = (256 * U * rstd * gw * (1 + size) + oracle.half_step(x.dtype) * want[0].abs() + 1e-37,
+            deep * (g * xh).abs().sum(0) + 2.0 ** -21 * (g * xh).abs().sum(0) + ph * want[1].abs() + 1e-37,
+            deep * g.abs().sum(0) + 2.0 ** -21 * g.abs().sum(0) + ph * want[2].abs() + 1e-37)
+    for got, o, tol in zip((dx, dw, db), want, tols):
+        assert got.isfinite().all() and ((got - o).abs() <= tol).all(), float(((got - o).abs() / tol).max())
+
+
+@pytest.mark.parametrize("kind", ["identity", "softplus", "relu"])
+@pytest.mark.parametrize("C,dtype", [(8193, torch.float32), (10001, torch.float32), (16385, torch.bfloat16), (17001, torch.float16), (130, torch.float32),
+                                     (1030, torch.bfloat16), (4099, torch.float16)])
+def test_kept_rows_that_end_inside_a_vector_far_from_zero(C, dtype, kind):
+    """Rows whose mean is hundreds of deviations: what lies past a row's end in its last vector must not reach the row's sums."""
+    _, ln, dy = inputs(5, C, dtype, torch.float32, C)
+    gen = torch.Generator().manual_seed(C)
+    # 300 with one element in twenty at 302 (a step of bf16 there): a deviation of 0.44; fp32 rows: 300 +- 0.3
+    x = 300.0 + (0.3 * torch.randn(5, C, generator=gen) if dtype == torch.float32 else 2.0 * (torch.rand(5, C, generator=gen) < 0.05))
+    x[1] -= 600.0
+    check_kept(x.to(dtype).cuda(), ln, dy, kind)
+
+
+KEPT_WIDTHS = [1, 5, 66, 128, 300, 771, 1030, 2047, 4096, 5000, 9000, 16384, 17000, 40000]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", KEPT_WIDTHS)
+def test_kept_gradients_of_every_width(C, dtype):
+    x, ln, dy = inputs(11, C, dtype, dtype, C)
+    check_kept(x, ln, dy, "softplus" if C % 2 else "identity")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,C", [(1, 100), (4097, 100), (1500, 2048), (900, 4096), (20000, 128)])
+def test_kept_gradients_of_many_rows(M, C, dtype):
+    x, ln, dy = inputs(M, C, dtype, torch.float32, M)
+    check_kept(x, ln, dy, "softplus")
