@@ -62,7 +62,7 @@ __device__ __forceinline__ bf16x8 column8(const unsigned short* plane, int m0, i
 struct Job {
   int64_t M, N, K;
   const void* g; int64_t ldg; const uint8_t* codes; int64_t ldc; const uint8_t* exps; int64_t lde;
-  void* dW; void* db; int32_t otype; float* part; int splits; int64_t rows; int tiles_n, tiles_k;
+  void* dW; void* db; int32_t otype, btype; float* part; int splits; int64_t rows; int tiles_n, tiles_k;
 };
 
 struct Where { int tn, tk, split; };
@@ -255,7 +255,7 @@ __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsign
   float t = 0.f;
   for (int i = 0; i < STEP; ++i) t += s_b[i * COLS + threadIdx.x];
   if (part) part[o.N * o.K + n0 + threadIdx.x] = t;
-  else store_param(o.db, o.otype, n0 + threadIdx.x, t);
+  else store_param(o.db, o.btype, n0 + threadIdx.x, t);
 }
 
 template <int FMT, typename G, int COLS>
@@ -277,7 +277,7 @@ wgrad8_kernel(Job o) {
 // The ranges' partial sums, added in a fixed order: a workgroup takes 64 adjacent results, its four waves a quarter of the ranges each.
 __global__ void __launch_bounds__(REDUCE_WG)
 wgrad8_reduce_kernel(int64_t NK, int64_t N, int splits, const float* __restrict__ part, void* __restrict__ dW,
-                     void* __restrict__ db, int32_t otype) {
+                     void* __restrict__ db, int32_t otype, int32_t btype) {
   __shared__ float s_t[REDUCE_WG];
   const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63), total = NK + (db ? N : 0);
   const int wave = threadIdx.x >> 6;
@@ -292,7 +292,7 @@ wgrad8_reduce_kernel(int64_t NK, int64_t N, int splits, const float* __restrict_
   if (wave || i >= total) return;
   t = (s_t[threadIdx.x] + s_t[threadIdx.x + 64]) + (s_t[threadIdx.x + 128] + s_t[threadIdx.x + 192]);
   if (i < NK) store_param(dW, otype, i, t);
-  else store_param(db, otype, i - NK, t);
+  else store_param(db, btype, i - NK, t);
 }
 
 // The tile: 256 x 256 (one workgroup per CU) where that still gives every CU a tile and a range of at least 256 rows, else 128 x 128.
@@ -341,7 +341,7 @@ int launch(const Job& o, int cols, hipStream_t stream) {
   if (rc || o.splits == 1) return rc;
   const int64_t total = o.N * o.K + (o.db ? o.N : 0);
   hipLaunchKernelGGL(wgrad8_reduce_kernel, dim3((unsigned)cdiv(total, 64)), dim3(REDUCE_WG), 0, stream, o.N * o.K, o.N, o.splits, o.part,
-                     o.dW, o.db, o.otype);
+                     o.dW, o.db, o.otype, o.btype);
   return check_hip(hipGetLastError(), "ganet_wgrad8");
 }
 
@@ -359,11 +359,12 @@ size_t ganet_wgrad8_workspace(int64_t M, int64_t N, int64_t K, int32_t gtype) {
 }
 
 int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, const void* g, int64_t ldg, const void* codes,
-                 int64_t ldc, const uint8_t* exps, int64_t lde, void* dW, void* db, int32_t otype, void* workspace,
+                 int64_t ldc, const uint8_t* exps, int64_t lde, void* dW, void* db, int32_t otypes, void* workspace,
                  size_t workspace_bytes, void* stream_) {
-  if (!wgrad_ok(M, N, K) || (fmt != GANET_E4M3 && fmt != GANET_E5M2) || !type_ok(gtype) || !type_ok(otype)) {
+  const int32_t otype = otypes & 0xff, btype = otypes >> 8 ? (otypes >> 8) - 1 : otype;
+  if (!wgrad_ok(M, N, K) || (fmt != GANET_E4M3 && fmt != GANET_E5M2) || !type_ok(gtype) || !type_ok(otype) || !type_ok(btype)) {
     set_error("ganet_wgrad8: unsupported M=%lld N=%lld K=%lld format=%d types=%d,%d", (long long)M, (long long)N, (long long)K, fmt,
-              gtype, otype);
+              gtype, otypes);
     return 4;
   }
   // (offsets inside a step of 32 rows are 32 bits)
@@ -375,7 +376,7 @@ int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, co
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   const Plan p = make_plan(M, N, K);
-  const Job o{M, N, K, g, ldg, static_cast<const uint8_t*>(codes), ldc, exps, lde, dW, db, otype, static_cast<float*>(workspace),
+  const Job o{M, N, K, g, ldg, static_cast<const uint8_t*>(codes), ldc, exps, lde, dW, db, otype, btype, static_cast<float*>(workspace),
               p.splits, p.rows, (int)p.tiles_n, (int)p.tiles_k};
   GANET_BY_TYPE(gtype, T, return fmt == GANET_E4M3 ? launch<GANET_E4M3, T>(o, p.cols, stream) : launch<GANET_E5M2, T>(o, p.cols, stream));
 }

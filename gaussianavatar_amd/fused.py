@@ -128,8 +128,8 @@ class _LinearKept8Fn(torch.autograd.Function):
         dx = g @ weight.to(g.dtype) if ctx.needs_input_grad[0] else None       # (g's type is autocast's where that is on)
         dW = db = None
         if ctx.needs_input_grad[1] or (ctx.btype is not None and ctx.needs_input_grad[2]):
-            dW, db = rows8.wgrad8(g, rows8.Rows8(codes, exps, ctx.cols, ctx.lead), weight.dtype)
-            db = None if ctx.btype is None else db.to(ctx.btype)
+            dW, db = rows8.wgrad8(g, rows8.Rows8(codes, exps, ctx.cols, ctx.lead), weight.dtype, ctx.btype)
+            db = None if ctx.btype is None else db
         return dx, dW, db
 
 

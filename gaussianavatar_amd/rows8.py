@@ -23,6 +23,7 @@ from . import _native
 FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 _FMT_CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _TYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_DB_TYPE = {t: c + 1 << 8 for t, c in _TYPE_CODE.items()}          # GANET_DB_TYPE
 BLOCK = 128
 
 
@@ -249,13 +250,16 @@ def matmul8(rows, w8, bias=None, dtype=torch.float32):
     return y.reshape(*rows.lead, N)
 
 
-def wgrad8(g, rows, dtype=None):
-    """(dW [N, K], db [N]) = (g^T rows, column sums of g) for g [..., N] over the same rows, in `dtype` (g's own by default). g enters with
-    all its bits (of an fp32 value, those down to 2^-133), sums are fp32. A non-finite g makes its row of dW non-finite."""
+def wgrad8(g, rows, dtype=None, bias_dtype=None):
+    """(dW [N, K], db [N]) = (g^T rows, column sums of g) for g [..., N] over the same rows, in `dtype` (g's own by default), db in
+    `bias_dtype` (dtype by default). g enters with all its bits (of an fp32 value, those down to 2^-133), sums are fp32, each result is
+    rounded once. A non-finite g makes its row of dW non-finite."""
     code = _type_code(g, "wgrad8")
     dtype = g.dtype if dtype is None else dtype
-    if dtype not in _TYPE_CODE:
-        raise TypeError(f"wgrad8: float32, bfloat16 or float16 expected, got {dtype}")
+    bias_dtype = dtype if bias_dtype is None else bias_dtype
+    for t in (dtype, bias_dtype):
+        if t not in _TYPE_CODE:
+            raise TypeError(f"wgrad8: float32, bfloat16 or float16 expected, got {t}")
     if g.dim() < 1 or g.shape[-1] < 1:
         raise ValueError(f"wgrad8: [..., N] with N >= 1 expected, got {tuple(g.shape)}")
     g2 = _rows2d(g.detach())
@@ -266,14 +270,14 @@ def wgrad8(g, rows, dtype=None):
     _same_device("wgrad8", g, rows.codes)
     if not g.is_cuda:
         gf = g2.double()
-        return (gf.t() @ _plain_values(rows.codes, rows.exps, K).double()).to(dtype), gf.sum(0).to(dtype)
+        return (gf.t() @ _plain_values(rows.codes, rows.exps, K).double()).to(dtype), gf.sum(0).to(bias_dtype)
     lib = _native.ganet()
     dW = torch.empty((N, K), dtype=dtype, device=g.device)
-    db = torch.empty(N, dtype=dtype, device=g.device)
+    db = torch.empty(N, dtype=bias_dtype, device=g.device)
     nbytes = lib.ganet_wgrad8_workspace(M, N, K, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
     _call(g.device, lib.ganet_wgrad8, M, N, K, _FMT_CODE[rows.codes.dtype], code, _ptr(g2), _ld(g2), _ptr(rows.codes),
-          rows.codes.stride(0), _ptr(rows.exps), rows.exps.stride(0), _ptr(dW), _ptr(db), _TYPE_CODE[dtype], _ptr(ws), nbytes)
+          rows.codes.stride(0), _ptr(rows.exps), rows.exps.stride(0), _ptr(dW), _ptr(db), _TYPE_CODE[dtype] | _DB_TYPE[bias_dtype], _ptr(ws), nbytes)
     return dW, db
 
 
@@ -315,14 +319,14 @@ class _Linear8Fn(torch.autograd.Function):
         new = lambda shape, t: torch.empty(shape, dtype=t, device=g.device)
         dx = new((M, K), xt) if need_x else None
         dW = new((N, K), wt) if need_w or need_b else None
-        db = new(N, wt) if need_b else None
+        db = new(N, bt) if need_b else None
         code = _TYPE_CODE[xt]
         ws = _bytes(max(16, lib.ganet_linear8_bwd_workspace(M, N, K, code)), g)
         _call(g.device, lib.ganet_linear8_bwd, M, N, K, code, g2.data_ptr(), _ld(g2), rows.data_ptr(), _ptr(back), _ptr(dx), _ptr(dW),
-              _ptr(db), _TYPE_CODE[wt], ws.data_ptr(), ws.numel())
+              _ptr(db), _TYPE_CODE[wt] | _DB_TYPE[bt or wt], ws.data_ptr(), ws.numel())
         if need_x and len(ctx.shape) != 2:
             dx = dx.reshape(ctx.shape)
-        return dx, dW if need_w else None, db.to(bt) if need_b else None
+        return dx, dW if need_w else None, db
 
 
 class _Linear8Plain(torch.autograd.Function):
@@ -344,8 +348,8 @@ class _Linear8Plain(torch.autograd.Function):
         w = Weight8(w_codes, w_exps, ctx.shape[-1]).dequantize()
         q = quantize8(g)
         dx = (q.dequantize() @ w).to(xt)
-        dW, db = wgrad8(g, Rows8(codes, exps, ctx.shape[-1], ctx.shape[:-1]), wt)
-        return dx, dW, None if bt is None else db.to(bt)
+        dW, db = wgrad8(g, Rows8(codes, exps, ctx.shape[-1], ctx.shape[:-1]), wt, bt)
+        return dx, dW, None if bt is None else db
 
 
 def linear8(x, weight, bias=None):

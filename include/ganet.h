@@ -416,9 +416,10 @@ int ganet_weight8_pack(int64_t N, int64_t K, int32_t type, const void* w, int64_
 int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes, int64_t ldc, const uint8_t* exps, int64_t lde,
                 const void* wcodes, int64_t ldwc, const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y,
                 int64_t ldy, int32_t ytype, void* stream);
-/* dW [N, K] = g^T rows, db [N] = column sums of g (NULL: not needed), both contiguous in otype: the weight gradient of a layer
- * whose input is kept as rows in 8 bits. g [M, N] in gtype enters with all its bits (of an fp32 value, those down to 2^-133). Row
+/* dW [N, K] = g^T rows, db [N] = column sums of g (NULL: not needed), both contiguous: the weight gradient of a layer whose input is
+ * kept as rows in 8 bits. otype: the type of both, or type of dW | GANET_DB_TYPE(type of db). g [M, N] in gtype enters with all its bits (of an fp32 value, those down to 2^-133). Row
  * strides up to 2^24, K < 2^22. */
+#define GANET_DB_TYPE(type) (((type) + 1) << 8)
 size_t ganet_wgrad8_workspace(int64_t M, int64_t N, int64_t K, int32_t gtype);
 int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, const void* g, int64_t ldg, const void* codes,
                  int64_t ldc, const uint8_t* exps, int64_t lde, void* dW, void* db, int32_t otype, void* workspace,
@@ -429,7 +430,7 @@ int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, co
  * _fwd / _bwd: training. rows8 (ganet_rows8_bytes(M, K)) keeps Q(x) for the backward pass, weight8 (ganet_weight8_bytes(N, K)) holds Q(W)
  * during the call, tweight8 (ganet_weight8_bytes(K, N); NULL: no input gradient) its transposed codes for the backward pass; each
  * buffer: codes, row stride = columns up to a multiple of 16, then exponents, row stride = blocks of 128 up to a multiple of 4.
- * dx = Q(g) Q(W) (NULL: not needed), dW = g^T Q(x) and db in wtype (dW NULL: neither). */
+ * dx = Q(g) Q(W) (NULL: not needed), dW = g^T Q(x) and db in wtype (as ganet_wgrad8's otype; dW NULL: neither). */
 size_t ganet_rows8_bytes(int64_t M, int64_t C);
 size_t ganet_weight8_bytes(int64_t N, int64_t K);
 size_t ganet_linear8_held_workspace(int64_t M, int64_t N, int64_t K, int32_t type);

@@ -1,0 +1,35 @@
+"""Layer norm, 8-bit rows and their products on the CPU where they can go wrong."""
+import pytest
+import torch
+
+from gaussianavatar_amd import _native, fused, rows8
+
+
+@pytest.mark.parametrize("form", ["linear8", "checkpoint8"])
+@pytest.mark.parametrize("wt", [torch.bfloat16, torch.float16])
+def test_a_bias_gradient_is_rounded_once_to_the_bias_own_type(wt, form):
+    """A 16-bit weight and an fp32 bias: the columns' sums in 64 bits, one rounding to fp32."""
+    torch.manual_seed(1)
+    x, w, b = torch.randn(3000, 64).to(wt), torch.randn(9, 64).to(wt).requires_grad_(True), torch.zeros(9, requires_grad=True)
+    g = torch.randn(3000, 9).to(wt)
+    g[:, 3] = 300.0                                             # past 65504
+    if form == "linear8":
+        y = rows8.linear8(x, w, b)
+    else:
+        with torch.autocast("cpu", wt):
+            y = fused.linear(x, w, b, checkpoint8=True)
+    dw, db = torch.autograd.grad(y, (w, b), g)
+    assert dw.dtype == wt and torch.equal(db, g.double().sum(0).float())
+    dW, db = rows8.wgrad8(g, rows8.quantize8(x), bias_dtype=torch.float32)
+    assert dW.dtype == wt and torch.equal(db, g.double().sum(0).float())
+    with pytest.raises(TypeError):
+        rows8.wgrad8(g, rows8.quantize8(x), bias_dtype=torch.float64)
+
+
+def test_the_bias_gradients_type_at_the_c_entry_points():
+    """otype carries the type of dW and, where it is another, GANET_DB_TYPE (type + 1 in bits 8 ..) of db."""
+    lib = _native.ganet()
+    A = 1 << 20                                                    # an aligned address that nobody reads
+    for otype in (3, 0x400, 0x501, 0x10001, -1):
+        assert lib.ganet_wgrad8(4, 8, 8, 0, 0, A, 8, A, 16, A, 4, A, None, otype, None, 0, None) == 4
+        assert b"ganet_wgrad8" in lib.ganet_last_error()

@@ -7,6 +7,7 @@ import torch
 
 from tests import rows8_oracle as oracle
 from tests.test_layernorm_gpu import U, TYPES, inputs
+from tests.test_rows8_gpu import spread
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,34 @@ def test_kept_gradients_of_every_width(C, dtype):
 def test_kept_gradients_of_many_rows(M, C, dtype):
     x, ln, dy = inputs(M, C, dtype, torch.float32, M)
     check_kept(x, ln, dy, "softplus")
+
+
+# ---------------------------------------------------------------------------------------------- types of gradients
+
+
+@pytest.mark.parametrize("form", ["linear8", "checkpoint8"])
+@pytest.mark.parametrize("wt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [40, 3000, 30000])
+def test_a_bias_gradient_is_rounded_once_to_the_bias_own_type(M, wt, form):
+    """A 16-bit weight and an fp32 bias: the sums of the columns in fp32, beyond the largest fp16 too."""
+    from gaussianavatar_amd import fused, rows8
+    x, w = spread(M, 64, wt, 1), spread(9, 64, wt, 2).requires_grad_(True)
+    g = spread(M, 9, wt, 4)
+    g[:, 3] = 300.0                                             # 3000 of them: past 65504
+    for bt in (torch.float32, wt):
+        b = torch.zeros(9, device="cuda", dtype=bt, requires_grad=True)
+        if form == "linear8":
+            y = rows8.linear8(x, w, b)
+        elif bt == wt:
+            y = fused.linear(x, w, b, checkpoint8=True)
+        else:
+            with torch.autocast("cuda", wt):
+                y = fused.linear(x, w, b, checkpoint8=True)
+        dw, db = torch.autograd.grad(y, (w, b), g)
+        assert dw.dtype == wt and db.dtype == bt
+        want, size = g.double().cpu().sum(0), g.double().cpu().abs().sum(0)
+        if bt == torch.float16:
+            want = torch.where(want.abs() < 65520, want, want.sign() * float("inf"))
+        tol = (M + 600) * U * size + oracle.half_step(bt) * want.abs()
+        fine = torch.isfinite(want)
+        assert torch.equal(db.double().cpu()[~fine], want[~fine]) and ((db.double().cpu() - want).abs() <= tol)[fine].all()
