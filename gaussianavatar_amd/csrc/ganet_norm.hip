@@ -4,7 +4,9 @@
 //   g = dy act'(u), dw = sum_rows g xh, db = sum_rows g, dx = rstd (g w - mean_c(g w) - xh mean_c(g w xh))
 //
 // Bound: HBM. Forward reads x and writes y once, backward reads x (or its 8-bit xh) and dy and writes dx once: a row stays in
-// registers between its reduction and its use, the variance is taken about the mean (no E[x^2] - mean^2). A group of G lanes holds
+// registers between its reduction and its use, the variance is taken about the mean (no E[x^2] - mean^2), with the mean's own rounding
+// taken back: the deviations d = x - mean are summed beside their squares, delta = sum(d) / C is what the first mean was off by, xh =
+// (d - delta) rstd, var = sum(d^2) / C - delta^2. (Rows of equal values far from zero: xh = 0 and not a few units of x over sqrt(eps).) A group of G lanes holds
 // a row, NC vectors of 16 bytes each: G = 1 .. 64 lanes of a wave for rows up to 4 KiB (backward: 2), a workgroup of 256 .. 1024 threads
 // up to 32 KiB, and a streaming form that reads the row three times (from cache) beyond. Groups stride over the rows, so
 // a lane always sees the same columns: w and b are loaded once, dw and db are summed in registers and leave as ONE partial row pair per workgroup,
@@ -174,23 +176,24 @@ ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
     if (t + 1 < turns) fetch(row + turn);
     row_sum<WIDE>(s, G, s_red, phase);
     const float mean = s[0] * inv;
-    s[0] = 0.f;
+    float d[2] = {0.f, 0.f};                               // the deviations' sum, and their squares'
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       const int left = C - (j * G + l) * V;
       if (full) {
         const float m = left > 0 ? mean : 0.f;             // (a vector past the row is zero: it stays so)
 #pragma unroll
-        for (int i = 0; i < V; ++i) { v[j][i] -= m; s[0] = fmaf(v[j][i], v[j][i], s[0]); }
+        for (int i = 0; i < V; ++i) { v[j][i] -= m; d[0] += v[j][i]; d[1] = fmaf(v[j][i], v[j][i], d[1]); }
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) { v[j][i] = i < left ? v[j][i] - mean : 0.f; s[0] = fmaf(v[j][i], v[j][i], s[0]); }
+        for (int i = 0; i < V; ++i) { v[j][i] = i < left ? v[j][i] - mean : 0.f; d[0] += v[j][i]; d[1] = fmaf(v[j][i], v[j][i], d[1]); }
       }
     }
-    row_sum<WIDE>(s, G, s_red, phase);
-    const float rstd = rsqrtf(fmaf(s[0], inv, eps));
+    row_sum<WIDE>(d, G, s_red, phase);
+    const float delta = d[0] * inv;
+    const float rstd = rsqrtf(fmaxf(fmaf(d[1], inv, -delta * delta), 0.f) + eps), shift = -delta * rstd;
     if (live && l == 0) {
-      if (mean_out) mean_out[row] = mean;
+      if (mean_out) mean_out[row] = mean + delta;
       if (rstd_out) rstd_out[row] = rstd;
     }
     if (!live) continue;
@@ -199,7 +202,11 @@ ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
       const int c = (j * G + l) * V;
       if (c >= C) continue;
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[j][i] *= rstd;
+      for (int i = 0; i < V; ++i) v[j][i] = fmaf(v[j][i], rstd, shift);
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = i < C - c ? v[j][i] : 0.f;
+      }
       if (codes) {
         uint8_t* p = codes + row * ldc + c;                // c is a multiple of V: aligned to V bytes; ldc covers the last vector
 #pragma unroll
@@ -238,25 +245,27 @@ ln_fwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx,
     }
     row_sum<true>(s, 0, s_red, phase);
     const float mean = (float)(s[0] * inv);
-    s[0] = 0.f;
+    float sd[2] = {0.f, 0.f};                              // the deviations' sum, and their squares'
     for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
       load_n(xr + c, C - c, v);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float d = c + i < C ? v[i] - mean : 0.f;
-        s[0] = fmaf(d, d, s[0]);
+        sd[0] += d;
+        sd[1] = fmaf(d, d, sd[1]);
       }
     }
-    row_sum<true>(s, 0, s_red, phase);
-    const float rstd = rsqrtf((float)(s[0] * inv) + eps);
+    row_sum<true>(sd, 0, s_red, phase);
+    const float delta = (float)(sd[0] * inv);
+    const float rstd = rsqrtf(fmaxf((float)(sd[1] * inv) - delta * delta, 0.f) + eps);
     if (threadIdx.x == 0) {
-      if (mean_out) mean_out[row] = mean;
+      if (mean_out) mean_out[row] = mean + delta;
       if (rstd_out) rstd_out[row] = rstd;
     }
     for (int64_t c = (int64_t)threadIdx.x * V; c < C; c += 1024 * V) {
       load_n(xr + c, C - c, v);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = c + i < C ? (v[i] - mean) * rstd : 0.f;    // (the backward pass reads a row's last vector whole)
+      for (int i = 0; i < V; ++i) v[i] = c + i < C ? (v[i] - mean - delta) * rstd : 0.f;    // (the backward pass reads a row's last vector whole)
       if (codes) {
         uint8_t* p = codes + row * ldc + c;
 #pragma unroll

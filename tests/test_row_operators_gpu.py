@@ -72,6 +72,44 @@ def test_kept_gradients_of_many_rows(M, C, dtype):
     check_kept(x, ln, dy, "softplus")
 
 
+# ---------------------------------------------------------------------------------------------- means
+
+
+@pytest.mark.parametrize("C", [3, 100, 300, 771, 4096, 12000])
+@pytest.mark.parametrize("value", [12345.678, -0.1, 1.0e6])
+def test_rows_of_equal_values_that_do_not_add_up_exactly(C, value):
+    """No deviation: xh = 0. The first sum's mean is off by at most 64 u |x| (a tree of 40 additions, the rounded 1 / C); what is left after
+    its residual is taken off is as much of that: 2 (64 u)^2 |x| rstd, rstd <= eps^-1/2 = 316. For dx, the mean that the backward
+    pass reads is the fp32 number nearest to the value, the value itself: xh = 0 there."""
+    from gaussianavatar_amd import fused
+    ln = torch.nn.LayerNorm(C, device="cuda")
+    x = torch.full((3, C), value, device="cuda", requires_grad=True)
+    y = fused.layernorm_act(x, ln, "identity")
+    assert float(y.detach().abs().max()) <= 2 * (64 * U) ** 2 * abs(value) * 317
+    dy = torch.randn(3, C, generator=torch.Generator().manual_seed(C)).cuda()
+    dx, dw = torch.autograd.grad(y, (x, ln.weight), dy)
+    assert not dw.any()
+    g = dy.double().cpu()
+    want = (g - g.mean(1, keepdim=True)) / ln.eps ** 0.5
+    assert ((dx.double().cpu() - want).abs() <= 256 * U * g.abs().max() / ln.eps ** 0.5).all()
+
+
+@pytest.mark.parametrize("C,dtype", [(77, torch.float32), (1000, torch.float32), (5000, torch.float32), (20000, torch.float32), (300, torch.bfloat16),
+                                     (300, torch.float16)])
+def test_the_forward_of_rows_far_from_zero(C, dtype):
+    """The residual of the mean is taken off: what is left of the mean's error is that of the sum of the deviations, 64 u of their mean size (one, in
+    units of the deviation at most), and as much of the first mean's own error, 64 u (64 u max|x|) rstd. y is rounded once more."""
+    from gaussianavatar_amd import fused
+    gen = torch.Generator().manual_seed(C)
+    x = (3000.0 + torch.randn(9, C, generator=gen) * (1.0 if dtype == torch.float32 else 40.0)).to(dtype).cuda()
+    ln = torch.nn.LayerNorm(C, device="cuda")
+    with torch.no_grad():
+        y = fused.layernorm_act(x, ln, "identity").double().cpu()
+    want, xh, rstd = oracle.layer_norm(x.cpu(), 1.0, 0.0, ln.eps, "identity")
+    tol = 64 * U * (xh.abs() + 1 + 64 * U * x.double().cpu().abs().amax(1, keepdim=True) * rstd) + oracle.half_step(dtype) * want.abs()
+    assert ((y - want).abs() <= tol).all(), float(((y - want).abs() / tol).max())
+
+
 # ---------------------------------------------------------------------------------------------- types of gradients
 
 
