@@ -26,25 +26,37 @@ namespace {
 constexpr int ACT_NONE = 0, ACT_SOFTPLUS = 1, ACT_RELU = 2;
 constexpr int LN_WG = 256;
 
-// softplus = max(u, 0) + log1p(exp(-|u|)): relative accuracy on both sides (torch's threshold of 20 differs by 2e-9 of the value).
-// log1p by its series where exp(-|u|) < 1/32, where it leaves out e^4 / 5 = 2e-7: the hardware logarithm of 1 + e is good to 1e-7
-// absolute only. Both are computed and one is taken (a branch per element costs more); a NaN goes through exp and log.
-constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+// softplus = max(u, 0) + log1p(e), e = exp(-|u|) (torch's threshold of 20 differs by 2e-9 of the value). With s = e / (2 + e), log1p(e) =
+// log((1 + s) / (1 - s)) = 2 s (1 + z / 3 + z^2 / 5 + ..), z = s^2 <= 1/9: one polynomial in z (Chebyshev interpolation, 4e-9 relative), relatively
+// accurate on both sides. The hardware logarithm of 1 + e instead is good to 1e-7 absolute only, 50 units of fp32 at u = -3.4.
+// FULL (fp32 results): exp's argument -|u| log2(e) is rounded at the size of |u|, 2^-17 of e at |u| = 86; what the rounding and the constant
+// lost is put back to first order: 2^-20 of the value (8 2^-24 in fp32 numpy). 16-bit results, 2^-12 at best, do without: 2^-16.
+constexpr float LOG2E = 1.44269504f, LOG2E_REST = 1.925963e-8f, LN2 = 0.693147181f;
+template <bool FULL>
 __device__ __forceinline__ float softplus(float u) {
-  const float e = __builtin_amdgcn_exp2f(-LOG2E * fabsf(u));
-  const float series = e * fmaf(e, fmaf(e, fmaf(e, -0.25f, 0.333333333f), -0.5f), 1.f);
-  const float log = LN2 * __builtin_amdgcn_logf(1.f + e);
-  return fmaxf(u, 0.f) + (e < 0.03125f ? series : log);
+  float e, top;
+  if (FULL) {
+    const float a = fminf(fabsf(u), 110.f);                // (beyond: 0, and the correction stays a number)
+    const float t = a * -LOG2E, rest = fmaf(a, -LOG2E_REST, fmaf(a, -LOG2E, -t));
+    e = __builtin_amdgcn_exp2f(t);
+    e = fmaf(e, rest * LN2, e);
+    top = u < 0.f ? 0.f : u;                               // (a NaN stays one)
+  } else {
+    e = __builtin_amdgcn_exp2f(-LOG2E * fabsf(u));
+    top = fmaxf(u, 0.f);
+  }
+  const float s = e * __builtin_amdgcn_rcpf(2.f + e), z = s * s;
+  return fmaf(s, fmaf(z, fmaf(z, fmaf(z, fmaf(z, 0.281577796f, 0.279651582f), 0.400245965f), 0.666663229f), 2.f), top);
 }
 // sigmoid(u) = 1 / (1 + exp(-u)); exp(-u) = infinity gives 0. The hardware reciprocal: 1 ulp.
 __device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * u)); }
 
 // act of N values, and g times its derivative (the kind is uniform: one branch per vector)
-template <int N>
+template <bool FULL, int N>
 __device__ __forceinline__ void act_fwd(float (&v)[N], int act) {
   if (act == ACT_SOFTPLUS) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = softplus(v[i]);
+    for (int i = 0; i < N; ++i) v[i] = softplus<FULL>(v[i]);
   } else if (act == ACT_RELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];
@@ -217,7 +229,7 @@ ln_fwd_kernel(int64_t M, int C, int G, const T* __restrict__ x, int64_t ldx, con
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) v[j][i] = fmaf(v[j][i], wv[j][i], bv[j][i]);
-      act_fwd(v[j], act);
+      act_fwd<sizeof(T) == 4>(v[j], act);
       store_stream(y + row * C + c, C - c, v[j]);
     }
   }
@@ -278,7 +290,7 @@ ln_fwd_stream_kernel(int64_t M, int64_t C, const T* __restrict__ x, int64_t ldx,
       load_params(b, wtype, (int)c, (int)(C - c), 0.f, bv);
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = fmaf(v[i], wv[i], bv[i]);
-      act_fwd(v, act);
+      act_fwd<sizeof(T) == 4>(v, act);
       store_n(y + row * C + c, C - c, v);
     }
   }

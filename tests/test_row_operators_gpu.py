@@ -110,6 +110,32 @@ def test_the_forward_of_rows_far_from_zero(C, dtype):
     assert ((y - want).abs() <= tol).all(), float(((y - want).abs() / tol).max())
 
 
+# ---------------------------------------------------------------------------------------------- softplus
+
+
+def test_softplus_is_accurate_relative_to_itself():
+    """w = 0 leaves act(b). fp32: exp with its argument's rounding taken back, a reciprocal, a polynomial, five operations more: sixteen
+    roundings of half a step at most, 2^-20 of the value, everywhere above the smallest normal numbers."""
+    from gaussianavatar_amd import fused
+    b = torch.cat([torch.linspace(-86, 86, 6001), torch.linspace(-6, 6, 2191)])
+    ln = torch.nn.LayerNorm(len(b), device="cuda")
+    with torch.no_grad():
+        ln.weight.zero_(), ln.bias.copy_(b)
+        y = fused.layernorm_act(torch.randn(2, len(b), device="cuda"), ln, "softplus")[1].double().cpu()
+    want = torch.log1p(torch.exp(b.double()))
+    assert ((y - want).abs() <= 2.0 ** -20 * want).all(), float(((y - want).abs() / want).max() * 2 ** 20)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_softplus_of_no_number_and_of_infinities(dtype):
+    from gaussianavatar_amd import fused
+    ln = torch.nn.LayerNorm(5, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        ln.weight.zero_(), ln.bias.copy_(torch.tensor([float("nan"), float("inf"), -float("inf"), 0.0, -200.0]))
+        y = fused.layernorm_act(torch.randn(2, 5, device="cuda").to(dtype), ln, "softplus")[0]
+    assert torch.isnan(y[0]) and y[1] == float("inf") and y[2] == 0 and y[4] == 0
+
+
 # ---------------------------------------------------------------------------------------------- types of gradients
 
 
