@@ -292,9 +292,9 @@ class _LayerNormKept8Plain(torch.autograd.Function):
         g = dy.float()
         if ctx.act != "identity":
             g = g * (torch.sigmoid(u) if ctx.act == "softplus" else (u > 0).float())
-        rows = tuple(range(dy.dim() - 1))
-        dw = (g * xh).sum(rows).to(weight.dtype) if weight is not None else None
-        db = g.sum(rows).to(bias.dtype) if bias is not None else None
+        C = dy.shape[-1]
+        dw = (g * xh).reshape(-1, C).sum(0).to(weight.dtype) if weight is not None else None
+        db = g.reshape(-1, C).sum(0).to(bias.dtype) if bias is not None else None
         gw = g if weight is None else g * weight.float()
         dx = rstd * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
         return dx.to(dy.dtype), dw, db, None, None

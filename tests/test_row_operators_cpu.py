@@ -5,6 +5,21 @@ import torch
 from gaussianavatar_amd import _native, fused, rows8
 
 
+@pytest.mark.parametrize("kind", ["softplus", "identity", "relu"])
+def test_one_row_without_leading_dimensions_kept_in_8_bits(kind):
+    """x [C] gives what x [1, C] gives."""
+    torch.manual_seed(0)
+    x, dy, ln = torch.randn(50), torch.randn(50), torch.nn.LayerNorm(50)
+    got = []
+    for shape in ((50,), (1, 50)):
+        t = x.reshape(shape).requires_grad_(True)
+        y = fused.layernorm_act(t, ln, kind, checkpoint8=True)
+        got.append([y] + list(torch.autograd.grad(y, (t, ln.weight, ln.bias), dy.reshape(shape))))
+    for a, b in zip(*got):
+        assert torch.equal(a.flatten(), b.flatten())
+    assert got[0][2].shape == (50,)
+
+
 @pytest.mark.parametrize("form", ["linear8", "checkpoint8"])
 @pytest.mark.parametrize("wt", [torch.bfloat16, torch.float16])
 def test_a_bias_gradient_is_rounded_once_to_the_bias_own_type(wt, form):
