@@ -273,6 +273,7 @@ class _LayerNormKept8Plain(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, act):
         xf = x.float()
         d = xf - xf.mean(-1, keepdim=True)
+        d = d - d.mean(-1, keepdim=True)                   # (the first mean's rounding)
         rstd = torch.rsqrt((d * d).mean(-1, keepdim=True) + eps)
         xh = d * rstd
         e = _native.ganet().ganet_ln_code_exponent(x.shape[-1])

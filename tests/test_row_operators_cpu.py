@@ -48,3 +48,12 @@ def test_the_bias_gradients_type_at_the_c_entry_points():
     for otype in (3, 0x400, 0x501, 0x10001, -1):
         assert lib.ganet_wgrad8(4, 8, 8, 0, 0, A, 8, A, 16, A, 4, A, None, otype, None, 0, None) == 4
         assert b"ganet_wgrad8" in lib.ganet_last_error()
+
+
+@pytest.mark.parametrize("value", [12345.678, -0.1, 1.0e6])
+def test_rows_of_equal_values_kept_in_8_bits(value):
+    """No deviation: xh = 0. The mean is off by at most 16 u |x| (pairwise sums), what is left of it by as much of that again, rstd <= 317."""
+    for C in (3, 100, 771, 4096):
+        ln, x = torch.nn.LayerNorm(C), torch.full((2, C), value, requires_grad=True)
+        y = fused.layernorm_act(x, ln, "identity", checkpoint8=True)
+        assert float(y.detach().abs().max()) <= 2 * (16 * 2.0 ** -24) ** 2 * abs(value) * 317
