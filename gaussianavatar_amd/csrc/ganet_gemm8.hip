@@ -4,7 +4,8 @@
 //
 // The scaled matrix instructions (v_mfma_scale_f32_*_f8f6f4) multiply 64 or 128 codes at a time and take a biased exponent per
 // lane and operand: a power of two per block of 128 costs no vector instruction, where an arbitrary fp32 scale would cost an
-// accumulator update per block. Products of codes are exact; sums are fp32; y is rounded once.
+// accumulator update per block. Products of codes are exact. Up to 32 rows, and fp32 results of any number, add them in fp32, on bf16 instructions;
+// 16-bit results of more rows on the 8-bit ones, which cut products that are small in their group of eight (see multiply()). y is rounded once.
 #include "ganet_rows8.h"
 
 namespace ganet {
@@ -81,8 +82,10 @@ __device__ __forceinline__ bf16x8 decode8(const i32x8& f, int d, float scale) {
 
 // acc += b a^T over one half block. The 8-bit instructions add products in groups of eight adjacent k, each cut to a multiple of 2^-13 of the
 // group's largest power of two, before they go on in fp32: 1.2e-5 to 2.5e-5 of a result's norm (measured against 64 bits; the older
-// 16-deep instructions are the same). That is below the rounding of a 16-bit result and above that of fp32, so an fp32 result (EXACT)
-// takes the bf16 instructions on decoded codes, at half the rate: error 4e-8 on the same inputs.
+// 16-deep instructions are the same). That is below the rounding of a 16-bit result, 1/70 of bf16's 1.7e-3 of the norm and 1/8 of fp16's
+// 2.1e-4 (whose results are 1 to 2 % farther from 64 bits for it), and a small part of what the codes themselves are off by, 2^-5; but where large products of one group cancel, what
+// is left is no better than 2^-13 of them. It is above the rounding of fp32, so an fp32 result (EXACT) takes the bf16 instructions on decoded codes: error
+// 4e-8 on the same inputs. 16-bit results keep the 8-bit instructions for their rate: 8192 x 4096 -> 8192 bf16 248 us against 437.
 // between(q) is called behind multiplication q of MULTIPLICATIONS.
 template <bool EXACT, int MT, int NT> constexpr int MULTIPLICATIONS = (EXACT ? 4 : 1) * MT * NT;
 template <int FMT, int MT, int NT, bool EXACT, typename Between>
@@ -360,7 +363,7 @@ struct Few<Codes> {
 template <int FMT, int MT, typename X, typename Y>
 __global__ void __launch_bounds__(64 * FEW_WAVES)
 gemm8_few_kernel(Operands o) {
-  constexpr bool CODES = __is_same(X, Codes), EXACT = sizeof(Y) == 4;
+  constexpr bool CODES = __is_same(X, Codes);
   constexpr int UNROLL = MT * sizeof(Few<X>) <= 128 ? 4 : 2;
   __shared__ f32x4 s_acc[FEW_WAVES][MT][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
@@ -376,19 +379,14 @@ gemm8_few_kernel(Operands o) {
     acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   auto multiply = [&](const i32x8& w, int sw, const i32x8 (&x)[MT], const int (&sx)[MT]) {
-    if constexpr (!EXACT) {
+    // bf16 instructions on decoded codes whatever the result's type (see multiply() above): what the 8-bit ones would save is not what
+    // bounds these (8-bit instructions: 1 x 4096 x 4096 bf16 7.3 us against 7.8, 32 rows 16.2 against 16.4)
+#pragma unroll
+    for (int d = 0; d < 8; d += 2) {
+      const bf16x8 wd = decode8<GANET_E4M3>(w, d, pow2(sw - 127));
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x[i], acc[i], GANET_E4M3, FMT, 0, sw, 0, sx[i]);
-    } else {
-      // fp32 results: bf16 instructions on decoded codes (see multiply() above)
-#pragma unroll
-      for (int d = 0; d < 8; d += 2) {
-        const bf16x8 wd = decode8<GANET_E4M3>(w, d, pow2(sw - 127));
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd, decode8<FMT>(x[i], d, pow2(sx[i] - 127)), acc[i], 0, 0, 0);
-      }
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd, decode8<FMT>(x[i], d, pow2(sx[i] - 127)), acc[i], 0, 0, 0);
     }
   };
   for (int kb0 = wave; kb0 < full; kb0 += FEW_WAVES * UNROLL) {

@@ -411,8 +411,9 @@ int ganet_rows8_unpack(int64_t M, int64_t C, int32_t type, int32_t fmt, const vo
  * exponents transposed (tcodes [K, ldtc], texps [ceil(K / 128), ldte]) for products with the other side. */
 int ganet_weight8_pack(int64_t N, int64_t K, int32_t type, const void* w, int64_t ldw, void* codes, int64_t ldc, uint8_t* exps,
                        int64_t lde, void* tcodes, int64_t ldtc, uint8_t* texps, int64_t ldte, void* stream);
-/* y [M, N] = rows [M, K] weight [N, K]^T + bias (btype, NULL: none): e4m3 or e5m2 rows, e4m3 weight; the matrix cores apply the
- * powers of two and accumulate in fp32; one rounding to ytype. Row strides of codes and exponents up to 2^24. */
+/* y [M, N] = rows [M, K] weight [N, K]^T + bias (btype, NULL: none): e4m3 or e5m2 rows, e4m3 weight; one rounding to ytype.
+ * Up to 32 rows, and ytype GANET_F32: products are added in fp32. 16-bit results of more rows: in groups of eight adjacent k each product is first cut to 2^-13 of the
+ * group's largest power of two, then added in fp32. Row strides of codes and exponents up to 2^24. */
 int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes, int64_t ldc, const uint8_t* exps, int64_t lde,
                 const void* wcodes, int64_t ldwc, const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y,
                 int64_t ldy, int32_t ytype, void* stream);

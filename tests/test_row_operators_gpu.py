@@ -7,7 +7,7 @@ import torch
 
 from tests import rows8_oracle as oracle
 from tests.test_layernorm_gpu import U, TYPES, inputs
-from tests.test_rows8_gpu import spread
+from tests.test_rows8_gpu import assert_product, spread
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +165,51 @@ def test_a_bias_gradient_is_rounded_once_to_the_bias_own_type(M, wt, form):
         tol = (M + 600) * U * size + oracle.half_step(bt) * want.abs()
         fine = torch.isfinite(want)
         assert torch.equal(db.double().cpu()[~fine], want[~fine]) and ((db.double().cpu() - want).abs() <= tol)[fine].all()
+
+
+# ---------------------------------------------------------------------------------------------- products
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(40, 130, 8200), (33, 20, 16500), (150, 70, 24577)])
+def test_products_over_more_blocks_than_lds_holds_exponents_of(M, N, K, dtype):
+    """Beyond 64 blocks of 128 the exponents are fetched again inside the loop. Every block has a size of its own."""
+    from gaussianavatar_amd import rows8
+    sizes = torch.exp2(torch.randint(-3, 4, (1, -(-K // 128)), generator=torch.Generator().manual_seed(K)).float()).repeat_interleave(128, 1)[:, :K].cuda()
+    x, w = (spread(M, K, torch.float32, 1) * sizes).to(dtype), (spread(N, K, torch.float32, 2, K ** -0.5) / sizes.flip(1)).to(dtype)
+    w8 = rows8.quantize8_weight(w)
+    xo, wo = oracle.rows(x.cpu())[0], oracle.weight(w.cpu())[0]
+    assert_product(rows8.linear8(x, w8), xo, wo, None, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 16, 32])
+def test_few_rows_add_in_fp32_whatever_the_result_is(M, dtype):
+    """256 * 256 + 1 * 4 - 256 * 256 in three products: fp32 sums hold the 4."""
+    from gaussianavatar_amd import rows8
+    x, w = torch.zeros(M, 260, device="cuda", dtype=dtype), torch.zeros(20, 260, device="cuda", dtype=dtype)
+    for at in (0, 132, 256):                                     # the last one in a block that is not full
+        for p, (a, b) in enumerate(((256.0, 256.0), (1.0, 4.0), (256.0, -256.0))):
+            x[:, at + p], w[:, at + p] = a, b
+    w8 = rows8.quantize8_weight(w)
+    assert (rows8.linear8(x, w8) == 12).all() and (rows8.matmul8(rows8.quantize8(x), w8, None, dtype) == 12).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 300, 1000), (64, 128, 4096), (4100, 4096, 640)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_what_the_8_bit_instructions_lose_of_a_sum(M, N, K, dtype):
+    """Equal rows, and minus the exact result as an fp32 bias, with which the sums start: what is left is the sums' own error. In a group of
+    eight adjacent k a product that is no multiple of 2^-13 of the largest one's power of two loses less than one such unit, and no
+    other product loses anything; fp32 sums of K terms and the bias' rounding come on top."""
+    from gaussianavatar_amd import rows8
+    row, w = spread(1, K, dtype, 1), spread(N, K, dtype, 2, K ** -0.5)
+    p = oracle.rows(row.cpu())[0] * oracle.weight(w.cpu())[0]                        # the products, [N, K]
+    exact = p.sum(1)
+    groups = torch.nn.functional.pad(p, (0, -K % 8)).unflatten(1, (-1, 8))
+    most = groups.abs().amax(2, keepdim=True)
+    unit = torch.where(most > 0, oracle._two_to((torch.frexp(most).exponent - 14).clamp_min(-900)), torch.ones_like(most))
+    tol = (unit * (torch.remainder(groups, unit) != 0)).sum((1, 2)) + (K + 2) * U * (p.abs().sum(1) + exact.abs())
+    tol = tol + oracle.half_step(dtype) * tol
+    y = rows8.linear8(row.expand(M, K).contiguous(), rows8.quantize8_weight(w), (-exact).float().cuda()).double().cpu()
+    assert torch.equal(y, y[:1].expand(M, N))
+    assert (y[0].abs() <= tol + torch.finfo(dtype).smallest_normal).all(), float((y[0].abs() / tol).max())
