@@ -63,7 +63,7 @@ __device__ __forceinline__ void read_chunk(const uint8_t* lds, int lane, int i, 
   f[4 * h] = (int)v.x; f[4 * h + 1] = (int)v.y; f[4 * h + 2] = (int)v.z; f[4 * h + 3] = (int)v.w;
 }
 
-// Eight codes (dwords d, d + 1) times 2^e as bf16: exact.
+// Eight codes (dwords d, d + 1) times a power of two as bf16: exact, if it is at least 2^-133.
 template <int FMT>
 __device__ __forceinline__ bf16x8 decode8(const i32x8& f, int d, float scale) {
   union { bf16x2 h[4]; bf16x8 v; } r;
@@ -104,9 +104,9 @@ __device__ __forceinline__ void multiply(const i32x8 (&a)[MT], const i32x8 (&b)[
     for (int d = 0; d < 4; ++d) {                            // 16 products per instruction: eight codes of a lane
       bf16x8 x[MT], w[NT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) x[i] = decode8<FMT>(a[i], 2 * d, pow2(sx[i] - 127));
+      for (int i = 0; i < MT; ++i) x[i] = decode8<FMT>(a[i], 2 * d, half_scale(sx[i]));
 #pragma unroll
-      for (int j = 0; j < NT; ++j) w[j] = decode8<GANET_E4M3>(b[j], 2 * d, pow2(sw - 127));
+      for (int j = 0; j < NT; ++j) w[j] = decode8<GANET_E4M3>(b[j], 2 * d, half_scale(sw));
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -206,7 +206,7 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
       for (int r = 0; r < 16; ++r) {
         const float v = bias(min(n0 + wn + j * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3), o.N - 1));
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i][r] = v;
+        for (int i = 0; i < MT; ++i) acc[j][i][r] = EXACT ? 0.25f * v : v;
       }
   };
   if (!o.bias) start([](int64_t) { return 0.f; });
@@ -278,7 +278,7 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
       for (int g = 0; g < 4; ++g) {
         Y v[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = (Y)acc[j][i][g * 4 + r];
+        for (int r = 0; r < 4; ++r) v[r] = (Y)(EXACT ? 4.f * acc[j][i][g * 4 + r] : acc[j][i][g * 4 + r]);
         Y* d = s_y + (wm + i * 32 + (lane & 31)) * PITCH + wn + j * 32 + g * 8 + (lane >> 5) * 4;
         __builtin_memcpy(__builtin_assume_aligned(d, 4 * sizeof(Y)), v, sizeof(v));
       }
@@ -383,10 +383,10 @@ gemm8_few_kernel(Operands o) {
     // bounds these (8-bit instructions: 1 x 4096 x 4096 bf16 7.3 us against 7.8, 32 rows 16.2 against 16.4)
 #pragma unroll
     for (int d = 0; d < 8; d += 2) {
-      const bf16x8 wd = decode8<GANET_E4M3>(w, d, pow2(sw - 127));
+      const bf16x8 wd = decode8<GANET_E4M3>(w, d, half_scale(sw));
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd, decode8<FMT>(x[i], d, pow2(sx[i] - 127)), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd, decode8<FMT>(x[i], d, half_scale(sx[i])), acc[i], 0, 0, 0);
     }
   };
   for (int kb0 = wave; kb0 < full; kb0 += FEW_WAVES * UNROLL) {
@@ -447,7 +447,7 @@ gemm8_few_kernel(Operands o) {
   if (row >= o.M) return;
   float v[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) v[c] = t[c] + ((o.bias && n + c < o.N) ? load_param(o.bias, o.btype, n + c) : 0.f);
+  for (int c = 0; c < 4; ++c) v[c] = 4.f * t[c] + ((o.bias && n + c < o.N) ? load_param(o.bias, o.btype, n + c) : 0.f);
   store_n(static_cast<Y*>(o.y) + row * o.ldy + n, o.N - n, v);
 }
 

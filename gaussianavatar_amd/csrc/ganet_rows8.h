@@ -126,6 +126,11 @@ __device__ __forceinline__ void unpack4(unsigned codes, float (&v)[4]) {
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (e + 127) << 23); }
 
+// Half of a block's scale, from its biased exponent e + 127 >= 1. The largest numbers of fp32 and bf16 are rounded to 2^128 by their codes (256 2^120), which
+// bf16 has not: their halves it has. What is multiplied on bf16 instructions is decoded at half its size and doubled in the result.
+// (For e = -126 the bits are those of zero; the conversions read the exponent field alone, 2^-127.)
+__device__ __forceinline__ float half_scale(int biased) { return __builtin_bit_cast(float, (biased - 1) << 23); }
+
 // The block exponent: with a = 1.m 2^p, F = 1.75 2^q (448: q = 8; 57344: q = 15) the smallest e with a <= F 2^e is p - q, or p - q + 1
 // where 1.m > 1.75. Adding 0x1fffff to the bits carries into the exponent field exactly there. a is finite and >= 0;
 // below 2^-118 the exponent stays at -126 and the codes lose bits, as numbers that small do in the type itself.

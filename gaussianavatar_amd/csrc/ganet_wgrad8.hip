@@ -140,7 +140,7 @@ __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsign
   auto put = [&](const Raw& v, int buf) {
     unsigned short* base = s_mem + buf * BUF + sr * PITCH;
     const unsigned in = v.live ? ~0u : 0u;
-    const float scale = pow2(v.e - 127);
+    const float scale = half_scale(v.e);                      // (the results are doubled: store)
     uint4* d = reinterpret_cast<uint4*>(base + P * PLANE + st * PER);
 #pragma unroll
     for (int i = 0; i < PER / 8; ++i) {
@@ -238,7 +238,7 @@ __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsign
         const unsigned at = n * K + wk + (lane & 31);
 #pragma unroll
         for (int j = 0; j < TJ; ++j)
-          if (n < rows && wk + j * 32 + (lane & 31) < cols) out[at + j * 32] = acc[i][j][r];
+          if (n < rows && wk + j * 32 + (lane & 31) < cols) out[at + j * 32] = 2.f * acc[i][j][r];
         __builtin_amdgcn_sched_barrier(0);                     // one row's results in registers at a time
       }
   };

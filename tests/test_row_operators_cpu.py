@@ -57,3 +57,12 @@ def test_rows_of_equal_values_kept_in_8_bits(value):
         ln, x = torch.nn.LayerNorm(C), torch.full((2, C), value, requires_grad=True)
         y = fused.layernorm_act(x, ln, "identity", checkpoint8=True)
         assert float(y.detach().abs().max()) <= 2 * (16 * 2.0 ** -24) ** 2 * abs(value) * 317
+
+
+def test_the_types_largest_numbers_stay_finite_beside_zeros():
+    """A value past fp32's range is the largest number in a product too: times zero it is zero."""
+    x = torch.full((2, 4), torch.finfo(torch.float32).min)
+    r = rows8.quantize8(x)
+    y = rows8.matmul8(r, rows8.quantize8_weight(torch.tensor([[0.0, 0, 0, 0], [2.0 ** -10, 0, 0, 0]])))
+    dW, _ = rows8.wgrad8(torch.zeros(2, 3), r)
+    assert not y[:, 0].any() and torch.allclose(y[:, 1], torch.tensor(-2.0 ** 118), rtol=2 ** -22) and not dW.any()

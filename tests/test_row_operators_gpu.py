@@ -213,3 +213,53 @@ def test_what_the_8_bit_instructions_lose_of_a_sum(M, N, K, dtype):
     y = rows8.linear8(row.expand(M, K).contiguous(), rows8.quantize8_weight(w), (-exact).float().cuda()).double().cpu()
     assert torch.equal(y, y[:1].expand(M, N))
     assert (y[0].abs() <= tol + torch.finfo(dtype).smallest_normal).all(), float((y[0].abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M", [5, 40])
+def test_the_types_largest_numbers_stay_finite_beside_zeros(M, dtype):
+    """A masked place that holds the type's lowest value: its code stands for -2^128, past bf16's range. Times zero it is zero, in
+    products and weight gradients, and times a small number it is finite."""
+    from gaussianavatar_amd import rows8
+    x, w = torch.ones(M, 200, device="cuda", dtype=dtype), torch.zeros(3, 200, device="cuda", dtype=dtype)
+    x[2, 7] = torch.finfo(dtype).min
+    x[2, 8:128] = 0
+    w[1, 1], w[2, 7] = 2.0, 2.0 ** -10
+    y = rows8.linear8(x, rows8.quantize8_weight(w), torch.ones(3, device="cuda"))
+    assert (y[:, 0] == 1).all() and y[2, 2].double() == -2.0 ** 118 and y[1, 1] == 3
+    g = torch.ones(M, 4, device="cuda", dtype=dtype)
+    g[2] = 0
+    g[2, 1] = 2.0 ** -12
+    dW, db = rows8.wgrad8(g, rows8.quantize8(x), torch.float32)
+    assert dW.isfinite().all() and dW[0, 7] == M - 1 and dW[1, 7].double() == -2.0 ** 116 and db[0] == M - 1
+
+
+@pytest.mark.parametrize("M", [5, 40])
+def test_the_smallest_numbers_count_beside_large_ones(M):
+    """Blocks whose exponent is the least one, -126, times large numbers, in products and weight gradients."""
+    from gaussianavatar_amd import rows8
+    x, w = torch.zeros(M, 200, device="cuda"), torch.zeros(3, 200, device="cuda")
+    x[:, 5], x[:, 130], x[3, 131] = 2.0 ** -120, 2.0 ** -126, 2.0 ** -129
+    w[0, 5], w[1, 130], w[2, 131] = 2.0 ** 110, 2.0 ** 111, 2.0 ** 111
+    r, w8 = rows8.quantize8(x), rows8.quantize8_weight(w)
+    assert (r.exps[:, :2] == 1).all()
+    y = rows8.matmul8(r, w8)
+    want = (x.double() @ w.double().t())
+    assert want[0, 0] == 2.0 ** -10 and torch.equal(y.double(), want)
+    g = torch.full((M, 2), 2.0 ** 100, device="cuda")
+    dW, _ = rows8.wgrad8(g, r)
+    want = g.double().t() @ x.double()
+    assert torch.equal(dW.double(), want) and want[0, 131] == 2.0 ** -29
+
+
+def test_the_transposed_side_of_the_largest_numbers():
+    """The same in an input gradient: dx = Q(g) Q(W)."""
+    from gaussianavatar_amd import rows8
+    for M in (5, 40):
+        x, w = torch.zeros(M, 150, device="cuda").requires_grad_(True), torch.ones(20, 150, device="cuda")
+        g = torch.zeros(M, 20, device="cuda")
+        g[1, 3] = torch.finfo(torch.float32).max
+        w[3, 4:] = 0
+        w[3, 2] = 2.0 ** -10
+        dx = torch.autograd.grad(rows8.linear8(x, w), x, g)[0]
+        assert dx[1, 2].double() == 2.0 ** 118 and not dx[1, 4:].any() and not dx[0].any() and not dx[2:].any()
