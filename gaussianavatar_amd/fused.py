@@ -135,8 +135,10 @@ class _LinearKept8Fn(torch.autograd.Function):
 
 def linear(x, weight, bias, checkpoint8=False):
     """x [..., K] -> x @ weight^T + bias. checkpoint8: what the backward pass keeps of x is its 8-bit rows (a quarter of fp32), so
-    dW is that of the rounded x (2^-4 of a value at most); y and dx are unchanged."""
+    dW is that of the rounded x (2^-4 of a value at most); y and dx are unchanged. On a HIP device K < 2^22 then."""
     if checkpoint8 and torch.is_grad_enabled():
+        if x.is_cuda:
+            rows8.check_trains("linear", weight.shape[1], weight.shape[0], weight, bias)
         return _LinearKept8Fn.apply(x, weight, bias)
     if x.is_cuda and x.dtype == torch.float32 and x.dim() == 2:
         return _LinearFn.apply(x, weight, bias)

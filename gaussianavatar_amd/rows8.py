@@ -283,6 +283,12 @@ def wgrad8(g, rows, dtype=None, bias_dtype=None):
     return dW, db
 
 
+def check_trains(what, K, N, *params):
+    """Raises where a weight gradient on the kernels will be asked for that they do not take (columns: K < 2^22, N < 2^24)."""
+    if (K >= 1 << 22 or N >= 1 << 24) and torch.is_grad_enabled() and any(p is not None and p.requires_grad for p in params):
+        raise ValueError(f"{what}: a weight gradient of {N} x {K} (fewer than 2^22 columns in and 2^24 out expected); under torch.no_grad() the product itself runs")
+
+
 def _bytes(n, like):
     return torch.empty(n, dtype=torch.uint8, device=like.device)
 
@@ -356,7 +362,7 @@ class _Linear8Plain(torch.autograd.Function):
 
 def linear8(x, weight, bias=None):
     """x [..., K] -> [..., N] in x's type, in 8-bit floating point (see matmul8). weight: a tensor [N, K] (training: differentiable in x, weight
-    and bias; the weight is packed in the call) or a Weight8 held by the caller (evaluation: not differentiable)."""
+    and bias, K < 2^22 on a HIP device; the weight is packed in the call) or a Weight8 held by the caller (evaluation: not differentiable)."""
     if x.dim() < 1:
         raise ValueError("linear8: [..., K] expected")
     K = x.shape[-1]
@@ -392,4 +398,6 @@ def linear8(x, weight, bias=None):
     if bias is not None:
         _type_code(bias, "linear8: bias")
     _same_device("linear8", x, weight, bias)
+    if x.is_cuda:
+        check_trains("linear8", K, weight.shape[0], weight, bias)
     return (_Linear8Fn if x.is_cuda else _Linear8Plain).apply(x, weight, bias)

@@ -7,7 +7,7 @@ import torch
 
 from tests import rows8_oracle as oracle
 from tests.test_layernorm_gpu import U, TYPES, inputs
-from tests.test_rows8_gpu import assert_product, spread
+from tests.test_rows8_gpu import assert_product, assert_wgrad, spread
 
 pytestmark = pytest.mark.gpu
 
@@ -263,3 +263,18 @@ def test_the_transposed_side_of_the_largest_numbers():
         w[3, 2] = 2.0 ** -10
         dx = torch.autograd.grad(rows8.linear8(x, w), x, g)[0]
         assert dx[1, 2].double() == 2.0 ** 118 and not dx[1, 4:].any() and not dx[0].any() and not dx[2:].any()
+
+
+# ---------------------------------------------------------------------------------------------- refusals
+
+
+def test_what_the_backward_pass_cannot_do_is_refused_forward():
+    from gaussianavatar_amd import fused, rows8
+    K = 1 << 22
+    x, w = torch.ones(1, K, device="cuda", dtype=torch.bfloat16), torch.ones(1, K, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    for call in (lambda: rows8.linear8(x, w), lambda: fused.linear(x, w, None, checkpoint8=True)):
+        with pytest.raises(ValueError, match="columns"):
+            call()
+        with torch.no_grad():
+            assert float(call()) == K
+    assert float(rows8.linear8(x, w.detach())) == K
