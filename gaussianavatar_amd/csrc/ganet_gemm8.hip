@@ -53,7 +53,7 @@ struct Operands {
 // would otherwise wait for the phases in flight before it reads the one that has landed. Every wait for them is the explicit one below,
 // by their number; so nothing else may load to registers in the loop: the exponents lie in LDS, 64 blocks at a time.
 __device__ __forceinline__ void fetch16(const uint8_t* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 
 // Chunk 2 (lane / 32) + h of fragment i of a wave's rows: a lane holds 32 codes of one of 32 rows.
