@@ -377,9 +377,12 @@ class POP_no_unet(nn.Module):
             if getattr(self, "_zero_pad", (None, None))[0] != zkey:
                 self._zero_pad = (zkey, pts.new_zeros(b, HW, pad))
             parts.append(self._zero_pad[1])
-        x = torch.cat(parts, dim=2)                                           # [b, HW, C+2 (+pad)]
         if rows is not None:
-            raise NotImplementedError("texel sharding needs the fused up-sampling path (c_geom 64, separable uv grid)")
+            # (a decoder with BatchNorm refuses a share of the rows unless it runs fused; one with LayerNorm takes any)
+            assert b == 1, "texel sharding applies to the batch-invariant (stage-1) decoder"
+            parts = [p[:, rows[0]:rows[1]] for p in parts]
+            HW = rows[1] - rows[0]
+        x = torch.cat(parts, dim=2)                                           # [b, HW, C+2 (+pad)]
         r, s, c = self.decoder.forward_points(x.reshape(b * HW, x.shape[2]), raw_heads=raw_heads, m_global=m_global)
         r, s, c = (t.reshape(b, HW, -1) for t in (r, s, c))
         if shared:

@@ -66,3 +66,38 @@ def test_the_types_largest_numbers_stay_finite_beside_zeros():
     y = rows8.matmul8(r, rows8.quantize8_weight(torch.tensor([[0.0, 0, 0, 0], [2.0 ** -10, 0, 0, 0]])))
     dW, _ = rows8.wgrad8(torch.zeros(2, 3), r)
     assert not y[:, 0].any() and torch.allclose(y[:, 1], torch.tensor(-2.0 ** 118), rtol=2 ** -22) and not dW.any()
+
+
+def _net(norm, bits8=False):
+    from gaussianavatar_amd.network import POP_no_unet
+    torch.manual_seed(0)
+    net = POP_no_unet(c_geom=64, hsize=32, decoder_norm=norm, decoder_bits8=bits8)
+    u = (torch.arange(16) + 0.5) / 16
+    return net, torch.randn(1, 64, 8, 8), torch.stack(torch.meshgrid(u, u, indexing="ij"), -1).reshape(1, 256, 2)
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+def test_a_share_of_the_texels_through_the_layer_norm_decoder(bits8):
+    """Shares of the rows, each by itself: the outputs are the whole's, and the gradients add up to the whole's. Sums over the rows are in
+    another order: 16 * 2^-24 of the largest, through the layers; a code next to a border may go the other way for it."""
+    net, geom, uv = _net("layer", bits8)
+    geom.requires_grad_(True)
+    params = [geom] + list(net.parameters())
+    weights = torch.randn(256, 7)
+
+    def run(r0, r1, rows):
+        y = torch.cat(net.forward_points(None, geom, uv, raw_heads=True, rows=rows, m_global=256), 2)[0]
+        assert y.shape == (r1 - r0, 7)
+        return y, torch.autograd.grad((y * weights[r0:r1]).sum(), params)
+
+    whole, want = run(0, 256, None)
+    got = [run(a, b, (a, b)) for a, b in ((0, 100), (100, 101), (101, 256))]
+    assert torch.allclose(torch.cat([y for y, _ in got]), whole, rtol=0, atol=2.0 ** -16 * float(whole.detach().abs().max()))
+    for i, w in enumerate(want):
+        assert float((sum(g[i] for _, g in got) - w).norm()) <= (2.0 ** -6 if bits8 else 2.0 ** -16) * float(w.norm()) + 1e-6
+
+
+def test_a_share_of_the_texels_through_a_batch_norm_decoder_that_does_not_run_fused_is_refused():
+    net, geom, uv = _net("batch")
+    with pytest.raises(NotImplementedError):
+        net.forward_points(None, geom, uv, rows=(0, 100), m_global=256)
