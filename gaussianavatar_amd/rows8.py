@@ -23,6 +23,7 @@ from . import _native
 FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 _FMT_CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _TYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FAST = 1 << 8                                                       # GANET_FAST
 _DB_TYPE = {t: c + 1 << 8 for t, c in _TYPE_CODE.items()}          # GANET_DB_TYPE
 BLOCK = 128
 
@@ -226,11 +227,11 @@ def quantize8_weight(w, transposed=False):
     return Weight8(as8(codes), exps, K, as8(t_codes), t_exps)
 
 
-def matmul8(rows, w8, bias=None, dtype=torch.float32):
-    """rows [..., K] times w8 [N, K] transposed, plus bias [N]: [..., N] in `dtype`, rounded once. Not differentiable by itself
-    (linear8 is). Sums are fp32 up to 32 rows and in fp32 results. 16-bit results of more rows are summed by the 8-bit matrix instructions: they cut each product
-    to 2^-13 of the largest power of two among eight adjacent columns' before they add in fp32, 1.2e-5 to 2.5e-5 of the result's norm, but 2^-13 of
-    large products that cancel; dtype=torch.float32 sums in fp32 throughout."""
+def matmul8(rows, w8, bias=None, dtype=torch.float32, fast=False):
+    """rows [..., K] times w8 [N, K] transposed, plus bias [N]: [..., N] in `dtype`. Sums are fp32, rounded once. Not differentiable by
+    itself (linear8 is). fast: 16-bit results of more than 32 rows on a HIP device are summed by the 8-bit matrix instructions, up to 1.8 times as
+    fast; they first cut each product to 2^-13 of the largest power of two among eight adjacent columns' products: 3e-5 to 6e-5 of the result's norm, and 2^-13 of
+    large products that cancel."""
     if rows.cols != w8.cols:
         raise ValueError(f"matmul8: rows of {rows.cols} columns, a weight of {w8.cols}")
     if dtype not in _TYPE_CODE:
@@ -248,7 +249,7 @@ def matmul8(rows, w8, bias=None, dtype=torch.float32):
     bias = None if bias is None else bias.detach().contiguous()
     _call(y.device, _native.ganet().ganet_gemm8, M, N, K, _FMT_CODE[rows.codes.dtype], _ptr(rows.codes), rows.codes.stride(0),
           _ptr(rows.exps), rows.exps.stride(0), _ptr(w8.codes), w8.codes.stride(0), _ptr(w8.exps), w8.exps.stride(0), _ptr(bias), btype,
-          _ptr(y), N, _TYPE_CODE[dtype])
+          _ptr(y), N, _TYPE_CODE[dtype] | (_FAST if fast else 0))
     return y.reshape(*rows.lead, N)
 
 
@@ -297,7 +298,7 @@ class _Linear8Fn(torch.autograd.Function):
     """y = Q(x) Q(W)^T + b; dx = Q(g) Q(W); dW = g^T Q(x); db = sum g. The packed input of the product is what the backward pass keeps of x."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, fast):
         x2, w2 = _rows2d(x), _rows2d(weight)
         M, K = x2.shape
         N = w2.shape[0]
@@ -306,7 +307,8 @@ class _Linear8Fn(torch.autograd.Function):
         rows, held = _bytes(max(16, lib.ganet_rows8_bytes(M, K)), x), _bytes(lib.ganet_weight8_bytes(N, K), x)
         back = _bytes(lib.ganet_weight8_bytes(K, N), x) if ctx.needs_input_grad[0] else None
         b = None if bias is None else bias.contiguous()
-        _call(x.device, lib.ganet_linear8_fwd, M, N, K, _TYPE_CODE[x.dtype], x2.data_ptr(), _ld(x2), _TYPE_CODE[weight.dtype],
+        ctx.code = _TYPE_CODE[x.dtype] | (_FAST if fast else 0)
+        _call(x.device, lib.ganet_linear8_fwd, M, N, K, ctx.code, x2.data_ptr(), _ld(x2), _TYPE_CODE[weight.dtype],
               w2.data_ptr(), _ld(w2), _ptr(b), 0 if b is None else _TYPE_CODE[b.dtype], y.data_ptr(), rows.data_ptr(),
               held.data_ptr(), _ptr(back))
         ctx.save_for_backward(rows, back)
@@ -320,7 +322,7 @@ class _Linear8Fn(torch.autograd.Function):
         rows, back = ctx.saved_tensors
         M, N, K = ctx.dims
         xt, wt, bt = ctx.types
-        need_x, need_w, need_b = ctx.needs_input_grad
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         need_b = need_b and bt is not None
         lib = _native.ganet()
         g2 = _rows2d(g)
@@ -328,20 +330,20 @@ class _Linear8Fn(torch.autograd.Function):
         dx = new((M, K), xt) if need_x else None
         dW = new((N, K), wt) if need_w or need_b else None
         db = new(N, bt) if need_b else None
-        code = _TYPE_CODE[xt]
+        code = ctx.code
         ws = _bytes(max(16, lib.ganet_linear8_bwd_workspace(M, N, K, code)), g)
         _call(g.device, lib.ganet_linear8_bwd, M, N, K, code, g2.data_ptr(), _ld(g2), rows.data_ptr(), _ptr(back), _ptr(dx), _ptr(dW),
               _ptr(db), _TYPE_CODE[wt] | _DB_TYPE[bt or wt], ws.data_ptr(), ws.numel())
         if need_x and len(ctx.shape) != 2:
             dx = dx.reshape(ctx.shape)
-        return dx, dW if need_w else None, db
+        return dx, dW if need_w else None, db, None
 
 
 class _Linear8Plain(torch.autograd.Function):
     """The same in torch operations (CPU)."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, fast):
         rows = quantize8(x)
         w8 = quantize8_weight(weight)
         ctx.save_for_backward(rows.codes, rows.exps, w8.codes, w8.exps)
@@ -357,12 +359,13 @@ class _Linear8Plain(torch.autograd.Function):
         q = quantize8(g)
         dx = (q.dequantize() @ w).to(xt)
         dW, db = wgrad8(g, Rows8(codes, exps, ctx.shape[-1], ctx.shape[:-1]), wt, bt)
-        return dx, dW, None if bt is None else db
+        return dx, dW, None if bt is None else db, None
 
 
-def linear8(x, weight, bias=None):
+def linear8(x, weight, bias=None, fast=False):
     """x [..., K] -> [..., N] in x's type, in 8-bit floating point (see matmul8). weight: a tensor [N, K] (training: differentiable in x, weight
-    and bias, K < 2^22 on a HIP device; the weight is packed in the call) or a Weight8 held by the caller (evaluation: not differentiable)."""
+    and bias, K < 2^22 on a HIP device; the weight is packed in the call) or a Weight8 held by the caller (evaluation: not differentiable).
+    fast: as matmul8's, for the result and the input gradient."""
     if x.dim() < 1:
         raise ValueError("linear8: [..., K] expected")
     K = x.shape[-1]
@@ -376,7 +379,7 @@ def linear8(x, weight, bias=None):
         N = weight.codes.shape[0]
         if bias is not None and tuple(bias.shape) != (N,):
             raise ValueError(f"linear8: a bias of {tuple(bias.shape)} for {N} columns")
-        code = _type_code(x, "linear8")
+        code = _type_code(x, "linear8") | (_FAST if fast else 0)
         btype = 0 if bias is None else _type_code(bias, "linear8: bias")
         _same_device("linear8", x, weight.codes, bias)
         x2 = _rows2d(x.detach())
@@ -400,4 +403,4 @@ def linear8(x, weight, bias=None):
     _same_device("linear8", x, weight, bias)
     if x.is_cuda:
         check_trains("linear8", K, weight.shape[0], weight, bias)
-    return (_Linear8Fn if x.is_cuda else _Linear8Plain).apply(x, weight, bias)
+    return (_Linear8Fn if x.is_cuda else _Linear8Plain).apply(x, weight, bias, fast)

@@ -412,8 +412,10 @@ int ganet_rows8_unpack(int64_t M, int64_t C, int32_t type, int32_t fmt, const vo
 int ganet_weight8_pack(int64_t N, int64_t K, int32_t type, const void* w, int64_t ldw, void* codes, int64_t ldc, uint8_t* exps,
                        int64_t lde, void* tcodes, int64_t ldtc, uint8_t* texps, int64_t ldte, void* stream);
 /* y [M, N] = rows [M, K] weight [N, K]^T + bias (btype, NULL: none): e4m3 or e5m2 rows, e4m3 weight; one rounding to ytype.
- * Up to 32 rows, and ytype GANET_F32: products are added in fp32. 16-bit results of more rows: in groups of eight adjacent k each product is first cut to 2^-13 of the
- * group's largest power of two, then added in fp32. Row strides of codes and exponents up to 2^24. */
+ * Sums are fp32. ytype | GANET_FAST: 16-bit results of more than 32 rows are summed by the 8-bit matrix instructions, which are faster and first cut each product to
+ * 2^-13 of the largest power of two among eight adjacent k (3e-5 to 6e-5 of a result's norm; 2^-13 of large products that cancel). Row strides of
+ * codes and exponents up to 2^24. */
+#define GANET_FAST 0x100
 int ganet_gemm8(int64_t M, int64_t N, int64_t K, int32_t fmt, const void* codes, int64_t ldc, const uint8_t* exps, int64_t lde,
                 const void* wcodes, int64_t ldwc, const uint8_t* wexps, int64_t ldwe, const void* bias, int32_t btype, void* y,
                 int64_t ldy, int32_t ytype, void* stream);
@@ -431,6 +433,7 @@ int ganet_wgrad8(int64_t M, int64_t N, int64_t K, int32_t fmt, int32_t gtype, co
  * _fwd / _bwd: training. rows8 (ganet_rows8_bytes(M, K)) keeps Q(x) for the backward pass, weight8 (ganet_weight8_bytes(N, K)) holds Q(W)
  * during the call, tweight8 (ganet_weight8_bytes(K, N); NULL: no input gradient) its transposed codes for the backward pass; each
  * buffer: codes, row stride = columns up to a multiple of 16, then exponents, row stride = blocks of 128 up to a multiple of 4.
+ * type | GANET_FAST: as ganet_gemm8's ytype, for y and dx.
  * dx = Q(g) Q(W) (NULL: not needed), dW = g^T Q(x) and db in wtype (as ganet_wgrad8's otype; dW NULL: neither). */
 size_t ganet_rows8_bytes(int64_t M, int64_t C);
 size_t ganet_weight8_bytes(int64_t N, int64_t K);

@@ -183,11 +183,11 @@ def test_products_over_more_blocks_than_lds_holds_exponents_of(M, N, K, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M", [1, 16, 32])
-def test_few_rows_add_in_fp32_whatever_the_result_is(M, dtype):
-    """256 * 256 + 1 * 4 - 256 * 256 in three products: fp32 sums hold the 4."""
+@pytest.mark.parametrize("M,N", [(1, 20), (16, 20), (32, 20), (33, 20), (200, 150), (4096, 3000)])
+def test_products_add_in_fp32_whatever_the_result_is(M, N, dtype):
+    """256 * 256 + 1 * 4 - 256 * 256 in three products of one group: fp32 sums hold the 4."""
     from gaussianavatar_amd import rows8
-    x, w = torch.zeros(M, 260, device="cuda", dtype=dtype), torch.zeros(20, 260, device="cuda", dtype=dtype)
+    x, w = torch.zeros(M, 260, device="cuda", dtype=dtype), torch.zeros(N, 260, device="cuda", dtype=dtype)
     for at in (0, 132, 256):                                     # the last one in a block that is not full
         for p, (a, b) in enumerate(((256.0, 256.0), (1.0, 4.0), (256.0, -256.0))):
             x[:, at + p], w[:, at + p] = a, b
@@ -195,10 +195,34 @@ def test_few_rows_add_in_fp32_whatever_the_result_is(M, dtype):
     assert (rows8.linear8(x, w8) == 12).all() and (rows8.matmul8(rows8.quantize8(x), w8, None, dtype) == 12).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 300, 4096), (20, 250, 384), (45, 231, 1000), (130, 128, 66), (200, 500, 2110), (4100, 4090, 640)])
+def test_products_are_fp32_sums_rounded_once(M, N, K, dtype):
+    """In every form, forward and for the input gradient: within K u sum|terms| and half a step of the result's type."""
+    from gaussianavatar_amd import rows8
+    x, w, b = spread(M, K, dtype, 1), spread(N, K, dtype, 2, K ** -0.5), spread(1, N, torch.float32, 3)[0]
+    at = torch.arange(M) if M < 1000 else torch.cat([torch.arange(0, M, 97), torch.arange(M - 40, M)])
+    xo, wo = oracle.rows(x.cpu()[at])[0], oracle.weight(w.cpu())[0]
+
+    def check(y, p, q, bias):
+        want, size = p @ q.t(), p.abs() @ q.abs().t()
+        if bias is not None:
+            want, size = want + bias, size + bias.abs()
+        tol = (p.shape[1] + 2) * U * size + oracle.half_step(dtype) * want.abs() + torch.finfo(dtype).smallest_normal * 2.0 ** -8
+        off = (y[at.cuda()].double().cpu() - want).abs()
+        assert (off <= tol).all(), float((off / tol).max())
+
+    check(rows8.linear8(x, rows8.quantize8_weight(w), b), xo, wo, b.double().cpu())
+    x.requires_grad_(True)
+    y, g = rows8.linear8(x, w, b), spread(M, N, dtype, 4)
+    check(y.detach(), xo, wo, b.double().cpu())
+    check(torch.autograd.grad(y, x, g)[0], oracle.rows(g.cpu()[at])[0], wo.t().contiguous(), None)
+
+
 @pytest.mark.parametrize("M,N,K", [(40, 300, 1000), (64, 128, 4096), (4100, 4096, 640)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_what_the_8_bit_instructions_lose_of_a_sum(M, N, K, dtype):
-    """Equal rows, and minus the exact result as an fp32 bias, with which the sums start: what is left is the sums' own error. In a group of
+    """fast=True. Equal rows, and minus the exact result as an fp32 bias, with which the sums start: what is left is the sums' own error. In a group of
     eight adjacent k a product that is no multiple of 2^-13 of the largest one's power of two loses less than one such unit, and no
     other product loses anything; fp32 sums of K terms and the bias' rounding come on top."""
     from gaussianavatar_amd import rows8
@@ -210,9 +234,30 @@ def test_what_the_8_bit_instructions_lose_of_a_sum(M, N, K, dtype):
     unit = torch.where(most > 0, oracle._two_to((torch.frexp(most).exponent - 14).clamp_min(-900)), torch.ones_like(most))
     tol = (unit * (torch.remainder(groups, unit) != 0)).sum((1, 2)) + (K + 2) * U * (p.abs().sum(1) + exact.abs())
     tol = tol + oracle.half_step(dtype) * tol
-    y = rows8.linear8(row.expand(M, K).contiguous(), rows8.quantize8_weight(w), (-exact).float().cuda()).double().cpu()
+    y = rows8.linear8(row.expand(M, K).contiguous(), rows8.quantize8_weight(w), (-exact).float().cuda(), fast=True).double().cpu()
     assert torch.equal(y, y[:1].expand(M, N))
     assert (y[0].abs() <= tol + torch.finfo(dtype).smallest_normal).all(), float((y[0].abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(5, 40, 300), (70, 130, 300), (4100, 4096, 640)])
+def test_fast_products_and_their_gradients(M, N, K, dtype):
+    """What fast allows for y and dx (assert_product's bound), and nothing else: dW, db, fp32 results and few rows have the same bits."""
+    from gaussianavatar_amd import rows8
+    x, w, b = (t.requires_grad_(True) for t in (spread(M, K, dtype, 1), spread(N, K, dtype, 2, K ** -0.5), spread(1, N, dtype, 3)[0]))
+    g = spread(M, N, dtype, 4)
+    y, full = rows8.linear8(x, w, b, fast=True), rows8.linear8(x, w, b)
+    grads, want = torch.autograd.grad(y, (x, w, b), g), torch.autograd.grad(full, (x, w, b), g)
+    assert torch.equal(grads[1], want[1]) and torch.equal(grads[2], want[2])
+    if M <= 32 or dtype == torch.float32:
+        assert torch.equal(y, full) and torch.equal(grads[0], want[0])
+    at = torch.arange(M) if M < 1000 else torch.cat([torch.arange(0, M, 97), torch.arange(M - 40, M)])
+    xo, wo = oracle.rows(x.detach().cpu()[at])[0], oracle.weight(w.detach().cpu())[0]
+    assert_product(y.detach()[at.cuda()], xo, wo, b.detach().double().cpu(), dtype)
+    assert_product(grads[0][at.cuda()], oracle.rows(g.cpu()[at])[0], wo.t().contiguous(), None, dtype)
+    w8 = rows8.quantize8_weight(w)
+    with torch.no_grad():
+        assert torch.equal(rows8.linear8(x, w8, b, fast=True), y) and torch.equal(rows8.matmul8(rows8.quantize8(x), w8, b, dtype, fast=True), y)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
