@@ -44,7 +44,8 @@ struct Operands {
 // so that neither LDS nor memory latency stands between two multiplications, and a fetch has three phases to arrive (with whole blocks
 // and two buffers it had two: 8192^3 2.28 PFLOP/s). A wave issues in order: what stands behind sixteen multiplications waits for
 // fifteen of them and then runs beside the last one only. So every multiplication is followed by its share of the reads and
-// fetches, and nothing crosses it (2.16 PFLOP/s with the reads and fetches in one go).
+// fetches, and nothing crosses it (2.16 PFLOP/s with the reads and fetches in one go). These rates are of the 8-bit instructions; on bf16 ones,
+// four times as many at twice the time together, there is more to hide behind: 8192^3 1.39 PFLOP/s.
 //
 // No branch in the loop: rows past the matrix fetch its last row (results nobody stores), chunks past a row's codes fetch its last
 // chunk and are zeroed in x's fragments, which only the last block needs; phases past the end fetch the last block again.
@@ -287,8 +288,9 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
   const int64_t left = o.N - n0 - c;
   const int rows = (int)min((int64_t)TM, o.M - m0);
   // A result of half the last-level cache and more is written past the caches: what it would drive out there (the inputs, that the
-  // backward pass reads again) is worth more. 262144 x 128 x 128 fp32, both directions: 188 -> 166 us; a layer norm that reads the result
-  // next loses 8 of them. Of half that size it would lose more than is won.
+  // backward pass reads again) is worth more. fp32, 128 columns in and out, both directions alone / with a layer norm behind it, past the caches against through
+  // them: 131072 rows (64 MiB) 125 against 124 / 194 against 192 us, 196608 (96 MiB) 128 against 142 / 218 against 223, 262144 161 against 188 / 278
+  // against 292, 524288 330 against 395 / 551 against 594.
   const bool past = o.M * o.N * (int64_t)sizeof(Y) >= 1ll << 27;
   if (left >= V) {
 #pragma unroll 8
@@ -309,8 +311,8 @@ gemm8_tile_kernel(Operands o, int tiles_m, int tiles_n) {
 // codes) are packed in registers, by the rule of ganet_rows8_pack: the four lanes that hold a row's block take its maximum and
 // convert; every workgroup repeats that (packs_inside() below tells where that costs less than a launch).
 // What bounds it is latency: so everything that a wave needs of UNROLL blocks is asked for at once, without a branch between the
-// loads (rows past the last read the last one, as do blocks); a last block that is not full comes behind them. From codes, bf16:
-// 1 x 4096 x 4096 7.6 us, 16 rows 9.2 (12.1 and 19.6 with the loads under conditions), 1 x 16384 x 4096 15 us, 4.5 TB/s.
+// loads (rows past the last read the last one, as do blocks); a last block that is not full comes behind them. From codes, bf16, twenty in
+// a graph, one of them: 1 x 4096 x 4096 5.2 us, 16 rows 7.2, 1 x 16384 x 4096 15.9, 4.2 TB/s. (With the loads under conditions 4.5 and 10 us more for 1 and 16 rows.)
 constexpr int FEW_WAVES = 8;
 struct Codes;        // the rows' type where they are codes already
 
@@ -378,7 +380,7 @@ gemm8_few_kernel(Operands o) {
   }
   auto multiply = [&](const i32x8& w, int sw, const i32x8 (&x)[MT], const int (&sx)[MT]) {
     // bf16 instructions on decoded codes whatever the result's type (see multiply() above): what the 8-bit ones would save is not what
-    // bounds these (8-bit instructions: 1 x 4096 x 4096 bf16 7.3 us against 7.8, 32 rows 16.2 against 16.4)
+    // bounds these (1 x 4096 x 4096 bf16, packed inside: 7.3 us on the 8-bit ones against 7.8; 32 rows 16.2 against 16.4)
 #pragma unroll
     for (int d = 0; d < 8; d += 2) {
       const bf16x8 wd = decode8<GANET_E4M3>(w, d, half_scale(sw));
@@ -449,7 +451,7 @@ gemm8_few_kernel(Operands o) {
   store_n(static_cast<Y*>(o.y) + row * o.ldy + n, o.N - n, v);
 }
 
-// (32 x 4096 x 4096 from codes, bf16 / fp32: 11.9 / 11.8 us; in tiles 17.6 / 32.7)
+// (32 x 4096 x 4096 from codes, bf16 / fp32: 9.9 / 10.0 us; 64 x 4096 x 4128 in tiles 30, fast 16)
 constexpr int FEW_ROWS = 32;
 template <int FMT, typename X, typename Y>
 int launch_few(const Operands& o, hipStream_t stream) {
@@ -499,8 +501,9 @@ bool fast_of(int32_t type) { return type >= 0 && (type & GANET_FAST); }
 int32_t type_of(int32_t type) { return type < 0 ? type : type & ~GANET_FAST; }
 
 // Whether few rows are packed inside the product's kernel: by what a CU has to pack then (16 rows, 4096 columns of the result, 1024 of the
-// rows: one unit, of fp32 two). Inside / with a launch of its own, in a graph, bf16: 1 x 1024 x 1024 7.4 / 8.8 us, 1 x 4096 x 4096
-// 8.9 / 9.3, 1 x 8192 x 4096 14.6 / 12.4, 32 x 4096 x 4096 16.7 / 14.6; fp32: 1 x 1024 x 1024 7.8 / 9.2, 16 x 4096 x 4096 14.7 / 11.8.
+// rows: one unit, of fp32 two). Inside / with a launch of its own, twenty in a graph, bf16: 1 x 1024 x 1024 4.9 / 6.6 us, 1 x 4096 x 4096
+// 7.4 / 7.5, 1 x 8192 x 4096 12.1 / 11.0, 32 x 4096 x 4096 14.8 / 12.4; fp32: 1 x 1024 x 1024 5.7 / 6.5, 32 x 1024 x 4096 9.8 / 10.3, 1 x 4096 x 4096
+// 8.2 / 7.4, 16 x 4096 x 4096 12.8 / 9.7.
 bool packs_inside(int64_t M, int64_t N, int64_t K, int32_t type) {
   return M <= FEW_ROWS && cdiv(M, 16) * cdiv(N, 4096) * cdiv(K, 1024) * (type == GANET_F32 ? 2 : 1) <= 4;
 }

@@ -73,7 +73,8 @@ struct Where { int tn, tk, split; };
 // reads and writes LDS while the other one's matrix instructions run. 8192 x 4096 x 4096 bf16: 274 us, 1.0 PFLOP/s (a large library
 // product reaches 1.13). With one wave on a SIMD, four of 128 x 128 in a workgroup, which have a third less to read from LDS, 320 us (262144 x 128 x 128 fp32 47 us against 45).
 // INSIDE: no vector of 8 columns crosses column N of g (one behind it is read as the last one); else element by element
-// (300000 x 64 x 64 bf16: 29 us against 48).
+// (300000 x 64 x 64 bf16: 29 us against 48). In 256 x 256 tiles it is that form, run by the tiles past column N alone, that needs more registers than there are
+// (fp32 56 spilled, fp16 44, bf16 2); the other one has none spilled.
 template <int TILE> struct Form;
 template <> struct Form<256> { static constexpr int TI = 4, TJ = 2, WN = 2, WAVES = 8; };
 template <> struct Form<128> { static constexpr int TI = 2, TJ = 1, WN = 2, WAVES = 8; };
@@ -105,7 +106,7 @@ __device__ __forceinline__ void wgrad8_tile(const Job& o, const Where& w, unsign
 
   // Columns past the matrix load its last ones and give results that nobody stores. The last step loads the range's last 32 rows and
   // counts those that no step before it had (a range of fewer rows: its last row again and again); what does not count is
-  // zeroed in x only, so that a column of g with an infinity in such a row gives a NaN, as it may. Offsets inside a step's rows
+  // zeroed in x and in g: db adds g up, and an infinity of g that counts once must not meet a zero of x. Offsets inside a step's rows
   // are the same for every step and fit 32 bits: no branch and no address arithmetic in vector registers (a value that two paths may
   // have loaded is waited for where they meet).
   // (vectors of g are values, not memory: copied to memory and on, the compiler loads them again where they are put)

@@ -65,9 +65,9 @@ class ShapeDecoder(nn.Module):
     sigmoid). BatchNorm (batch statistics) + softplus after every hidden layer.
 
     norm="layer": LayerNorm over the channels of a point instead (parameters ln1 ..): no statistics over the rows, so a rank's
-    share of them needs no exchange, and evaluation is the same function as training. bits8: the hidden layers multiply in 8-bit
-    floating point (rows8.linear8) and keep 8 bits of every activation for the backward pass; the three output layers stay in
-    the rows' own type."""
+    share of them needs no exchange, and evaluation is the same function as training. bits8: the hidden layers multiply rows and weights
+    rounded to 8-bit floating point (rows8.linear8; the sums are fp32, on bf16 instructions) and keep 8 bits of every activation for the
+    backward pass; the three output layers multiply in the rows' own type."""
 
     HEADS = ("", "N", "SH")
     norm, bits8 = "batch", False               # (of a decoder unpickled from before it had a choice)

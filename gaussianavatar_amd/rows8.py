@@ -5,7 +5,7 @@ ganet_weight8_pack, ganet_gemm8, ganet_wgrad8).
     rows.dequantize(dtype)            the values that the codes stand for
     dW, db = wgrad8(g, rows)          a linear layer's weight gradient straight from its packed input
     w8 = quantize8_weight(w)          a weight [N, K], a power of two for every 128 x 128 block
-    matmul8(rows, w8, bias)           their product on the 8-bit matrix instructions
+    matmul8(rows, w8, bias)           their product (fast: on the 8-bit matrix instructions)
     linear8(x, w, bias)               a linear layer on these: forward and backward in training, or with a held Weight8
 
 With a = the largest finite magnitude of a block and F the largest value of the format (e4m3: 448, e5m2: 57344), the block's exponent e
@@ -88,7 +88,7 @@ def _check_codes(what, codes, exps, cols, kinds):
 
 class Rows8:
     """Rows in 8 bits. codes [M, K up to a multiple of 16] (float8_e4m3fn or float8_e5m2, zero past column K), exps [M, K / 128 up to
-    a multiple of 4] uint8 (the exponent of each 128 columns + 127), cols = K, lead = the leading dimensions of what was packed."""
+    a multiple of 4] uint8 (the exponent of each 128 columns + 127: 1 to 254), cols = K, lead = the leading dimensions of what was packed."""
     __slots__ = ("codes", "exps", "cols", "lead")
 
     def __init__(self, codes, exps, cols, lead=None):
@@ -113,7 +113,7 @@ class Rows8:
 
 class Weight8:
     """A weight [N, K] in 8 bits: codes [N, K up to a multiple of 16] in float8_e4m3fn, zero past column K, exps [N / 128, K / 128 up to a
-    multiple of 4] uint8, cols = K. t_codes, t_exps: the same for the transposed weight, or None."""
+    multiple of 4] uint8 (exponents + 127: 1 to 254), cols = K. t_codes, t_exps: the same for the transposed weight, or None."""
     __slots__ = ("codes", "exps", "cols", "t_codes", "t_exps")
 
     def __init__(self, codes, exps, cols, t_codes=None, t_exps=None):

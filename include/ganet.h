@@ -401,7 +401,8 @@ int ganet_ln_bwd(int64_t M, int64_t C, int32_t type, int32_t wtype, const void* 
 /* Rows in 8 bits: every 128 consecutive columns of a row share a power of two. With a the block's largest finite magnitude and
  * F the format's largest value, e = the smallest integer with a <= F 2^e, at least -126 (a = 0: e = 0); code = x 2^-e rounded to the
  * nearest value of the format (ties to even); value = code 2^e. A NaN stays NaN; an infinity becomes NaN in e4m3 and stays infinite
- * in e5m2. codes [M, ldc], columns C .. ldc are zero up to the next multiple of 16; exps [M, lde] hold e + 127, lde a multiple of 4. */
+ * in e5m2. codes [M, ldc], columns C .. ldc are zero up to the next multiple of 16; exps [M, lde] hold e + 127 (1 to 254 in what a caller
+ * makes: 0 and 255 are no exponents), lde a multiple of 4. */
 int ganet_rows8_pack(int64_t M, int64_t C, int32_t type, int32_t fmt, const void* x, int64_t ldx, void* codes, int64_t ldc,
                      uint8_t* exps, int64_t lde, void* stream);
 /* y [M, C] contiguous = the values; one beyond the type's range becomes its largest number. */
