@@ -369,7 +369,7 @@ def ganet() -> ctypes.CDLL:
         lib.ganet_wgrad8.argtypes = [L, L, L, I, I, P, L, P, L, P, L, P, P, I, P, c_size_t, P]
         lib.ganet_last_error.restype = c_char_p
         lib.ganet_abi_version.restype = c_int
-        if lib.ganet_abi_version() != 10:
+        if lib.ganet_abi_version() != 11:
             raise RuntimeError("libganet_hip.so ABI version mismatch; rebuild")
         _ganet = lib
     return _ganet

@@ -101,3 +101,22 @@ def test_a_share_of_the_texels_through_a_batch_norm_decoder_that_does_not_run_fu
     net, geom, uv = _net("batch")
     with pytest.raises(NotImplementedError):
         net.forward_points(None, geom, uv, rows=(0, 100), m_global=256)
+
+
+def test_fast_sums_at_the_entry_points():
+    """GANET_FAST (0x100) beside a type: workspaces are the type's, an unknown type is refused all the same; the CPU's sums are what they are."""
+    lib = _native.ganet()
+    A = 1 << 20                                                    # an aligned address that nobody reads
+    for ytype in (0x103, 0x201, -1, 3):
+        assert lib.ganet_gemm8(4, 8, 8, 0, A, 16, A, 4, A, 16, A, 4, None, 0, A, 8, ytype, None) == 4
+        assert lib.ganet_linear8_held(4, 8, 8, ytype, A, 8, A, 16, A, 4, None, 0, A, None, 0, None) == 4
+    for M, N, K in ((1, 64, 64), (1, 4096, 8192), (40, 100, 300)):
+        for t in range(3):
+            assert lib.ganet_linear8_held_workspace(M, N, K, t | 0x100) == lib.ganet_linear8_held_workspace(M, N, K, t)
+            assert lib.ganet_linear8_bwd_workspace(M, N, K, t | 0x100) == lib.ganet_linear8_bwd_workspace(M, N, K, t)
+    torch.manual_seed(0)
+    x, w = torch.randn(40, 70, requires_grad=True), torch.randn(9, 70, requires_grad=True)
+    got, want = rows8.linear8(x, w, fast=True), rows8.linear8(x, w)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got.sum(), (x, w)), torch.autograd.grad(want.sum(), (x, w))):
+        assert torch.equal(a, b)
