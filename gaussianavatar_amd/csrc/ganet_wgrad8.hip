@@ -4,7 +4,7 @@
 //
 // The sum runs over the rows, along which the powers of two change, so the 8-bit matrix instructions (one scale per 32 products of
 // a lane) do not apply to it as it lies. Codes become bf16 instead: 4 significand bits and a power of two fit bf16 exactly, so the kept input
-// enters with no further rounding. g enters with all its bits as 1 (bf16), 2 (fp16) or 3 (fp32) bf16 pieces, of
+// enters with no further rounding (at half its size, halves below 2^-133 lost, and the results doubled: half_scale()). g enters with all its bits as 1 (bf16), 2 (fp16) or 3 (fp32) bf16 pieces, of
 // which a piece below bf16's smallest number, 2^-133, is lost; sums are fp32.
 //
 // What bounds it: for wide layers the matrix instructions (P products per product of the layer), for the 128 columns of a point decoder
